@@ -267,6 +267,97 @@ int kvops_import_multi_noalloc(uint32_t node_num, const uint64_t *seg_bases, uin
                                uint32_t max_num_reqs, uint32_t stripe_rows, uint64_t status, uint64_t stream,
                                uint32_t block_dim, const KvopsRowOpts *opts);
 
+/* ---- 8-bit cache rows (no counterpart in the reference) ------------------------------------
+ *
+ * A row of quant_elems + plain_elems 16-bit values may be stored in the segments with its leading
+ * quant_elems in 8 bits. Each 128 of them share one fp32 scale: with a = max |x| over the 128 and
+ * Q = 448 (KVOPS_ROW_E4M3) or 127 (KVOPS_ROW_INT8),
+ *   scale = fl32(a / Q), code = round_to_nearest_even(fl32(x * fl32(Q / a)));
+ *   a < 2^-100: scale 0 and codes 0; a inf or NaN: scale 0x7FC00000 (NaN), codes 0.
+ * A stored row reads back as fl16(fl32(code * scale)) and its plain values unchanged.
+ * Stored layout: quant_elems code bytes; the scales, padded with zeros to 16 bytes; plain_elems 16-bit values:
+ * 656 bytes for a 1152-byte row (512 + 64 values).
+ * quant_elems is a multiple of 128 in [128, 4096], plain_elems a multiple of 8 in [0, 4096]; every
+ * base address and stride is 16-byte aligned. */
+#define KVOPS_ROW_RAW 0u
+#define KVOPS_ROW_E4M3 1u
+#define KVOPS_ROW_INT8 2u
+#define KVOPS_DTYPE_FP16 0u
+#define KVOPS_DTYPE_BF16 1u
+
+/* Bytes of a stored row in *out_bytes. */
+int kvops_quant_row_bytes(uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
+                          uint32_t *out_bytes);
+
+/* kvops_export_seg_alllayer_ex that quantises: the source rows have 2 * (quant_elems +
+ * plain_elems) bytes, the segment's rows are stored rows. */
+int kvops_export_quant_alllayer(uint64_t channel, uint64_t seg_base, uint32_t per_layer_seg_rows,
+                                uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
+                                uint32_t row_lo, uint32_t row_cnt, uint32_t layer_num, uint64_t src_layer0_base,
+                                uint64_t src_layer_stride, uint32_t stripe_rows, uint32_t node_num, uint32_t my_node,
+                                uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts);
+
+/* kvops_export_seg that quantises: the flagged hot rows are 16-bit rows, the segment's rows are
+ * stored rows. The form for single tokens. */
+int kvops_export_quant(uint64_t channel, uint64_t seg_base, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
+                       uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
+                       uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
+                       uint64_t topk_device_slots, uint64_t export_flags, uint64_t num_real, uint64_t hot_row_base,
+                       uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint32_t node_num,
+                       uint32_t my_node, uint64_t status, uint64_t stream, uint32_t block_dim,
+                       const KvopsRowOpts *opts);
+
+/* kvops_import_multi that reads stored rows back into 16-bit hot rows. */
+int kvops_import_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows,
+                       uint32_t per_layer_seg_rows, uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems,
+                       uint32_t plain_elems, uint64_t topk_indices, uint64_t req_pool_indices,
+                       uint64_t req_host_base, uint64_t topk_device_slots, uint64_t is_miss, uint64_t num_real,
+                       uint64_t hot_row_base, uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows,
+                       uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts);
+
+/* ---- attention over the hot rows (no counterpart in the reference) --------------------------
+ *
+ * For each request r < min(num_real, max_num_reqs), drafted token t and head h, with the 576-value
+ * query q and the keys
+ *   the hot row of every list position k < top_k whose slot lies in [0, hot_rows), and
+ *   the drafted row j < drafts for every set bit j of tree[r][t]:
+ *   s = scale * (q . key), p = softmax(s), out = sum over the keys of p * key[0:512],
+ *   lse = log(sum exp(s)).
+ * Each list position is a key of its own (a slot named twice counts twice). No key at all gives out
+ * 0 and lse -inf; hot rows that no position names and drafted rows that a token does not see may
+ * hold anything, NaN included. Requests from num_real on are left as they were. A request whose
+ * pool index is outside [0, pool_size) has no hot rows. One token without drafts is a plain decode
+ * step; tree 0 (no words) stands for a chain, token t seeing drafted rows 0..t.
+ * Scores, sums and outputs are accumulated in fp32; the probabilities are rounded to the rows'
+ * type for the second product, and out is rounded to it once. */
+typedef struct KvopsAttend {
+    uint64_t q;                    /* [max_num_reqs, tokens, heads, 576], 16-bit, 16-byte aligned rows */
+    uint64_t q_stride_req, q_stride_token, q_stride_head; /* in values, multiples of 8 */
+    uint64_t hot_row_base;         /* this layer's hot rows: 1152 bytes each, or 656 stored bytes */
+    uint64_t hot_req_stride_rows;  /* rows from one pool index to the next (0: all requests share) */
+    uint64_t req_pool_indices;     /* int64 [max_num_reqs] */
+    uint64_t topk_device_slots;    /* int32, top_k consecutive slots per list */
+    uint64_t slots_stride_req, slots_stride_token; /* in slots; stride_token 0: one list per request */
+    uint64_t num_real;             /* int32 [1] */
+    uint64_t draft_rows;           /* 16-bit rows of 576 values; 0 when drafts is 0 */
+    uint64_t draft_stride_req, draft_stride_row; /* in values, multiples of 8 */
+    uint64_t tree;                 /* uint64 [max_num_reqs, tokens], 0: a chain */
+    uint64_t out;                  /* [max_num_reqs, tokens, heads, 512], 16-bit, 16-byte aligned */
+    uint64_t lse;                  /* fp32 [max_num_reqs, tokens, heads], 0: not wanted */
+    uint64_t workspace;            /* kvops_attend_workspace bytes, 16-byte aligned; one launch at a time */
+    uint64_t workspace_bytes;
+    uint32_t max_num_reqs, tokens, heads, top_k, drafts; /* tokens and drafts <= 64, heads <= 128 */
+    uint32_t hot_rows;             /* rows per request that a slot may name */
+    uint32_t pool_size;
+    uint32_t row_format;           /* KVOPS_ROW_RAW, or how the hot rows are stored */
+    uint32_t row_dtype;            /* of q, the 16-bit rows and out */
+    float scale;
+} KvopsAttend;
+
+/* Bytes of workspace that kvops_attend_hot needs for this shape on the current device. */
+int kvops_attend_workspace(const KvopsAttend *a, uint64_t *out_bytes);
+int kvops_attend_hot(const KvopsAttend *a, uint64_t stream);
+
 /* Pool plumbing that replaces the EMS control plane (not a reference entry point):
  * segment memory on a device (or pinned host memory with device = -1), peer access,
  * and CUDA IPC so that one process per GPU can map the other GPUs' segments. Device

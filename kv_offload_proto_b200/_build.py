@@ -19,7 +19,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libkvops_b200.so")
 EXT = os.path.join(PKG, "kvops_ext", "_kvops" + sysconfig.get_config_var("EXT_SUFFIX"))
-CU_SOURCES = ["capi.cu", "sieve.cu", "rows.cu", "noalloc.cu"]
+CU_SOURCES = ["capi.cu", "sieve.cu", "rows.cu", "noalloc.cu", "quant.cu", "attend.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -37,7 +37,8 @@ def _run(cmd):
 
 
 def build_lib(force=False, verbose_ptxas=False):
-    deps = [os.path.join(CSRC, f) for f in CU_SOURCES + ["kvops_internal.cuh", "rows_common.cuh", "sieve_big.cuh"]]
+    deps = [os.path.join(CSRC, f) for f in CU_SOURCES + ["kvops_internal.cuh", "rows_common.cuh", "sieve_big.cuh",
+                                                          "quant.cuh"]]
     deps.append(os.path.join(ROOT, "include", "kvops_b200.h"))
     if not force and not _newer(LIB, deps):
         return LIB

@@ -103,6 +103,32 @@ struct ExportParams {
     StatusTarget st;
 };
 
+// A row codec (quant.cuh): rows of 16-bit values whose leading quant_elems are stored in 8 bits.
+struct RowCodec {
+    uint32_t format;       // KVOPS_ROW_E4M3 or KVOPS_ROW_INT8
+    uint32_t dtype;        // KVOPS_DTYPE_FP16 or KVOPS_DTYPE_BF16
+    uint32_t quant_elems;  // a multiple of kQuantGroup
+    uint32_t plain_elems;  // a multiple of 8
+};
+
+// Values that share one scale.
+constexpr uint32_t kQuantGroup = 128;
+
+// Bytes of the scales of one stored row (one fp32 each, padded to 16 bytes), of the stored row
+// (codes, scales, plain values) and of the 16-bit row it stands for.
+__host__ __device__ __forceinline__ uint32_t codec_scale_bytes(const RowCodec &c)
+{
+    return (c.quant_elems / kQuantGroup * 4u + 15u) & ~15u;
+}
+__host__ __device__ __forceinline__ uint32_t codec_stored_bytes(const RowCodec &c)
+{
+    return c.quant_elems + codec_scale_bytes(c) + 2u * c.plain_elems;
+}
+__host__ __device__ __forceinline__ uint32_t codec_row_bytes(const RowCodec &c)
+{
+    return 2u * (c.quant_elems + c.plain_elems);
+}
+
 // Extra arguments of the layer-step kernels (sieve.cu).
 // Words of one cooperative layer-step's block: epoch, arrival count, walk-list progress (layout in sieve.cu).
 constexpr uint32_t kCoopBlockWords = 2048;
@@ -177,6 +203,11 @@ cudaError_t launch_gather(const GatherParams &p, cudaStream_t s, int sm_count);
 // every position whose flag (p.is_miss) is set.
 cudaError_t launch_scatter(const GatherParams &p, cudaStream_t s, int sm_count);
 cudaError_t launch_export(const ExportParams &p, cudaStream_t s, int sm_count);
+// The same three copies between 16-bit rows and stored rows (quant.cu). p.row_bytes is the
+// stored row's size (the segments' rows); the hot or source rows have codec_row_bytes(c).
+cudaError_t launch_gather_quant(const GatherParams &p, const RowCodec &c, cudaStream_t s, int sm_count);
+cudaError_t launch_scatter_quant(const GatherParams &p, const RowCodec &c, cudaStream_t s, int sm_count);
+cudaError_t launch_export_quant(const ExportParams &p, const RowCodec &c, cudaStream_t s, int sm_count);
 // Fused SIEVE step + miss-row gather (one CTA per request). Sets *launched = false, launching
 // nothing, when the request's state and the copy ring do not fit shared memory; the caller
 // then runs launch_sieve_update and launch_gather instead.

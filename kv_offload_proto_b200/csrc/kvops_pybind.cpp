@@ -129,6 +129,130 @@ void export_seg_alllayer(uint64_t channel, uint64_t seg_base, uint32_t per_layer
                                        stream, block_dim, &o));
 }
 
+uint32_t row_format_of(const std::string &name)
+{
+    if (name == "raw") return KVOPS_ROW_RAW;
+    if (name == "e4m3") return KVOPS_ROW_E4M3;
+    if (name == "int8") return KVOPS_ROW_INT8;
+    throw std::invalid_argument("row_format must be 'raw', 'e4m3' or 'int8'");
+}
+
+uint32_t row_dtype_of(const std::string &name)
+{
+    if (name == "fp16") return KVOPS_DTYPE_FP16;
+    if (name == "bf16") return KVOPS_DTYPE_BF16;
+    throw std::invalid_argument("row_dtype must be 'fp16' or 'bf16'");
+}
+
+uint32_t quant_row_bytes(const std::string &row_format, const std::string &row_dtype, uint32_t quant_elems,
+                         uint32_t plain_elems)
+{
+    uint32_t n = 0;
+    check(kvops_quant_row_bytes(row_format_of(row_format), row_dtype_of(row_dtype), quant_elems, plain_elems, &n));
+    return n;
+}
+
+void export_quant_alllayer(uint64_t channel, uint64_t seg_base, uint32_t per_layer_seg_rows,
+                           const std::string &row_format, const std::string &row_dtype, uint32_t quant_elems,
+                           uint32_t plain_elems, uint32_t row_lo, uint32_t row_cnt, uint32_t layer_num,
+                           uint64_t src_layer0_base, uint64_t src_layer_stride, uint32_t stripe_rows,
+                           uint32_t node_num, uint32_t my_node, uint64_t status, uint64_t stream, uint32_t block_dim,
+                           bool injective, uint64_t err_word)
+{
+    const KvopsRowOpts o = row_opts(0, injective, err_word);
+    check(kvops_export_quant_alllayer(channel, seg_base, per_layer_seg_rows, row_format_of(row_format),
+                                      row_dtype_of(row_dtype), quant_elems, plain_elems, row_lo, row_cnt, layer_num,
+                                      src_layer0_base, src_layer_stride, stripe_rows, node_num, my_node, status,
+                                      stream, block_dim, &o));
+}
+
+void export_quant(uint64_t channel, uint64_t seg_base, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
+                  const std::string &row_format, const std::string &row_dtype, uint32_t quant_elems,
+                  uint32_t plain_elems, uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
+                  uint64_t topk_device_slots, uint64_t export_flags, uint64_t num_real, uint64_t hot_row_base,
+                  uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint32_t node_num, uint32_t my_node,
+                  uint64_t status, uint64_t stream, uint32_t block_dim, uint64_t hot_req_stride_rows, bool injective,
+                  uint64_t err_word)
+{
+    const KvopsRowOpts o = row_opts(hot_req_stride_rows, injective, err_word);
+    check(kvops_export_quant(channel, seg_base, layer_offset_rows, per_layer_seg_rows, row_format_of(row_format),
+                             row_dtype_of(row_dtype), quant_elems, plain_elems, topk_indices, req_pool_indices,
+                             req_host_base, topk_device_slots, export_flags, num_real, hot_row_base, top_k,
+                             max_num_reqs, stripe_rows, node_num, my_node, status, stream, block_dim, &o));
+}
+
+void import_quant(const std::vector<uint64_t> &seg_bases, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
+                  const std::string &row_format, const std::string &row_dtype, uint32_t quant_elems,
+                  uint32_t plain_elems, uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
+                  uint64_t topk_device_slots, uint64_t is_miss, uint64_t num_real, uint64_t hot_row_base,
+                  uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint64_t status, uint64_t stream,
+                  uint32_t block_dim, uint64_t hot_req_stride_rows, bool injective, uint64_t err_word)
+{
+    const KvopsRowOpts o = row_opts(hot_req_stride_rows, injective, err_word);
+    check(kvops_import_quant(static_cast<uint32_t>(seg_bases.size()), seg_bases.data(), layer_offset_rows,
+                             per_layer_seg_rows, row_format_of(row_format), row_dtype_of(row_dtype), quant_elems,
+                             plain_elems, topk_indices, req_pool_indices, req_host_base, topk_device_slots, is_miss,
+                             num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream, block_dim, &o));
+}
+
+KvopsAttend attend_shape(uint32_t max_num_reqs, uint32_t tokens, uint32_t heads, uint32_t top_k, uint32_t drafts,
+                         const std::string &row_format, const std::string &row_dtype)
+{
+    KvopsAttend a{};
+    a.max_num_reqs = max_num_reqs;
+    a.tokens = tokens;
+    a.heads = heads;
+    a.top_k = top_k;
+    a.drafts = drafts;
+    a.row_format = row_format_of(row_format);
+    a.row_dtype = row_dtype_of(row_dtype);
+    return a;
+}
+
+uint64_t attend_workspace(uint32_t max_num_reqs, uint32_t tokens, uint32_t heads, uint32_t top_k, uint32_t drafts,
+                          const std::string &row_format, const std::string &row_dtype)
+{
+    const KvopsAttend a = attend_shape(max_num_reqs, tokens, heads, top_k, drafts, row_format, row_dtype);
+    uint64_t bytes = 0;
+    check(kvops_attend_workspace(&a, &bytes));
+    return bytes;
+}
+
+void attend_hot(uint64_t q, uint64_t q_stride_req, uint64_t q_stride_token, uint64_t q_stride_head,
+                uint64_t hot_row_base, uint64_t hot_req_stride_rows, uint32_t hot_rows, uint64_t req_pool_indices,
+                uint32_t pool_size, uint64_t topk_device_slots, uint64_t slots_stride_req,
+                uint64_t slots_stride_token, uint64_t num_real, uint64_t draft_rows, uint64_t draft_stride_req,
+                uint64_t draft_stride_row, uint64_t tree, uint64_t out, uint64_t lse, uint64_t workspace,
+                uint64_t workspace_bytes, uint32_t max_num_reqs, uint32_t tokens, uint32_t heads, uint32_t top_k,
+                uint32_t drafts, const std::string &row_format, const std::string &row_dtype, float scale,
+                uint64_t stream)
+{
+    KvopsAttend a = attend_shape(max_num_reqs, tokens, heads, top_k, drafts, row_format, row_dtype);
+    a.q = q;
+    a.q_stride_req = q_stride_req;
+    a.q_stride_token = q_stride_token;
+    a.q_stride_head = q_stride_head;
+    a.hot_row_base = hot_row_base;
+    a.hot_req_stride_rows = hot_req_stride_rows;
+    a.hot_rows = hot_rows;
+    a.req_pool_indices = req_pool_indices;
+    a.pool_size = pool_size;
+    a.topk_device_slots = topk_device_slots;
+    a.slots_stride_req = slots_stride_req;
+    a.slots_stride_token = slots_stride_token;
+    a.num_real = num_real;
+    a.draft_rows = draft_rows;
+    a.draft_stride_req = draft_stride_req;
+    a.draft_stride_row = draft_stride_row;
+    a.tree = tree;
+    a.out = out;
+    a.lse = lse;
+    a.workspace = workspace;
+    a.workspace_bytes = workspace_bytes;
+    a.scale = scale;
+    check(kvops_attend_hot(&a, stream));
+}
+
 void sieve_update(uint64_t topk_indices, uint64_t req_pool_indices, uint64_t seq_lens, uint64_t prefill_lens,
                   uint64_t device_buffer_tokens, uint64_t device_buffer_visited, uint64_t device_buffer_ht,
                   uint64_t sieve_hand, uint64_t topk_device_slots, uint64_t is_miss, uint64_t num_real,
@@ -207,6 +331,38 @@ PYBIND11_MODULE(_kvops, m)
           py::arg("layer_num"), py::arg("src_layer0_base"), py::arg("src_layer_stride"), py::arg("stripe_rows"),
           py::arg("node_num"), py::arg("my_node"), py::arg("status"), py::arg("stream") = 0, py::arg("block_dim") = 1,
           py::kw_only(), py::arg("injective") = false, py::arg("err_word") = 0);
+    // 8-bit stored rows and the attention over the hot rows (not in the reference module).
+    m.def("quant_row_bytes", &quant_row_bytes, py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems") = 512,
+          py::arg("plain_elems") = 64);
+    m.def("export_quant_alllayer", &export_quant_alllayer, py::arg("channel"), py::arg("seg_base"),
+          py::arg("per_layer_seg_rows"), py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"),
+          py::arg("plain_elems"), py::arg("row_lo"), py::arg("row_cnt"), py::arg("layer_num"),
+          py::arg("src_layer0_base"), py::arg("src_layer_stride"), py::arg("stripe_rows"), py::arg("node_num"),
+          py::arg("my_node"), py::arg("status"), py::arg("stream") = 0, py::arg("block_dim") = 1, py::kw_only(),
+          py::arg("injective") = false, py::arg("err_word") = 0);
+    m.def("export_quant", &export_quant, py::arg("channel"), py::arg("seg_base"), py::arg("layer_offset_rows"),
+          py::arg("per_layer_seg_rows"), py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"),
+          py::arg("plain_elems"), py::arg("topk_indices"), py::arg("req_pool_indices"), py::arg("req_host_base"),
+          py::arg("topk_device_slots"), py::arg("export_flags"), py::arg("num_real"), py::arg("hot_row_base"),
+          py::arg("top_k"), py::arg("max_num_reqs"), py::arg("stripe_rows"), py::arg("node_num"), py::arg("my_node"),
+          py::arg("status"), py::arg("stream") = 0, py::arg("block_dim") = 1, py::kw_only(),
+          py::arg("hot_req_stride_rows") = 0, py::arg("injective") = false, py::arg("err_word") = 0);
+    m.def("import_quant", &import_quant, py::arg("seg_bases"), py::arg("layer_offset_rows"),
+          py::arg("per_layer_seg_rows"), py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"),
+          py::arg("plain_elems"), py::arg("topk_indices"), py::arg("req_pool_indices"), py::arg("req_host_base"),
+          py::arg("topk_device_slots"), py::arg("is_miss"), py::arg("num_real"), py::arg("hot_row_base"),
+          py::arg("top_k"), py::arg("max_num_reqs"), py::arg("stripe_rows"), py::arg("status"), py::arg("stream") = 0,
+          py::arg("block_dim") = 1, py::kw_only(), py::arg("hot_req_stride_rows") = 0, py::arg("injective") = false,
+          py::arg("err_word") = 0);
+    m.def("attend_workspace", &attend_workspace, py::arg("max_num_reqs"), py::arg("tokens"), py::arg("heads"),
+          py::arg("top_k"), py::arg("drafts"), py::arg("row_format") = "raw", py::arg("row_dtype") = "fp16");
+    m.def("attend_hot", &attend_hot, py::arg("q"), py::arg("q_stride_req"), py::arg("q_stride_token"),
+          py::arg("q_stride_head"), py::arg("hot_row_base"), py::arg("hot_req_stride_rows"), py::arg("hot_rows"),
+          py::arg("req_pool_indices"), py::arg("pool_size"), py::arg("topk_device_slots"), py::arg("slots_stride_req"),
+          py::arg("slots_stride_token"), py::arg("num_real"), py::arg("draft_rows"), py::arg("draft_stride_req"),
+          py::arg("draft_stride_row"), py::arg("tree"), py::arg("out"), py::arg("lse"), py::arg("workspace"),
+          py::arg("workspace_bytes"), py::arg("max_num_reqs"), py::arg("tokens"), py::arg("heads"), py::arg("top_k"),
+          py::arg("drafts"), py::arg("row_format"), py::arg("row_dtype"), py::arg("scale"), py::arg("stream") = 0);
     m.def("sieve_update", &sieve_update, py::arg("topk_indices"), py::arg("req_pool_indices"), py::arg("seq_lens"),
           py::arg("prefill_lens"), py::arg("device_buffer_tokens"), py::arg("device_buffer_visited"),
           py::arg("device_buffer_ht"), py::arg("sieve_hand"), py::arg("topk_device_slots"), py::arg("is_miss"),

@@ -1,0 +1,134 @@
+// quant.cuh — the 8-bit row codec: how 16-bit cache rows are stored and what they read back as.
+//
+// A row is quant_elems values followed by plain_elems ones. For each group of 128 of the former,
+// with a = max |x| over the group and Q the largest code (448 for e4m3, 127 for int8):
+//   a is inf or NaN:  scale = the quiet NaN 0x7FC00000, codes 0: the group reads back as NaN, never as wrong numbers;
+//   a < 2^-100:       scale = 0, codes 0 (Q / a would leave the fp32 range);
+//   otherwise:        scale = fl32(a / Q), code = round_to_nearest_even(fl32(x * fl32(Q / a))).
+// A code stands for fl16(fl32(code * scale)), fl16 rounding to the row's 16-bit type. Every step is
+// one IEEE fp32 operation, so the codes and the values are the same wherever they are computed.
+// The stored row is the codes, then the fp32 scales padded to 16 bytes, then the plain values:
+// 656 bytes for the 512 + 64 values of a 1152-byte row.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "kvops_internal.cuh"
+
+namespace kvb {
+
+// The 16-bit types of rows.
+struct Fp16 {
+    static constexpr uint32_t kInf = 0x7C00u;  // magnitude bits from which a value is not finite
+    __device__ static __forceinline__ float2 unpack(uint32_t v)
+    {
+        return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    }
+    __device__ static __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+struct Bf16 {
+    static constexpr uint32_t kInf = 0x7F80u;
+    __device__ static __forceinline__ float2 unpack(uint32_t v)
+    {
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+    }
+    __device__ static __forceinline__ uint32_t pack(float a, float b)
+    {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
+
+// The 8-bit codes: four at a time.
+struct E4m3 {
+    static constexpr float kMax = 448.f;
+    __device__ static __forceinline__ uint32_t encode4(float a, float b, float c, float d)
+    {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+        return lo | (hi << 16);
+    }
+    __device__ static __forceinline__ float4 decode4(uint32_t v)
+    {
+        const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xFFFFu), __NV_E4M3);
+        const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v >> 16), __NV_E4M3);
+        const float2 x = __half22float2(__half2(lo)), y = __half22float2(__half2(hi));
+        return make_float4(x.x, x.y, y.x, y.y);
+    }
+};
+struct Int8 {
+    static constexpr float kMax = 127.f;
+    __device__ static __forceinline__ uint32_t encode4(float a, float b, float c, float d)
+    {
+        // |x * fl(127 / a)| < 127.5, so no code leaves [-127, 127].
+        const uint32_t lo = __byte_perm(__float2int_rn(a), __float2int_rn(b), 0x0040);
+        const uint32_t hi = __byte_perm(__float2int_rn(c), __float2int_rn(d), 0x0040);
+        return __byte_perm(lo, hi, 0x5410);
+    }
+    // A code c as a float: its byte, offset by 128, in the low mantissa of 2^23, less 2^23 + 128
+    // (both exact), which costs a byte permute and an add instead of a conversion.
+    __device__ static __forceinline__ float4 decode4(uint32_t v)
+    {
+        const uint32_t u = v ^ 0x80808080u;
+        const float k = 8388608.f + 128.f;
+        return make_float4(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)) - k,
+                           __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)) - k,
+                           __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)) - k,
+                           __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - k);
+    }
+};
+
+// Eight 16-bit values (one 16-byte unit) -> eight codes and, in every lane of the 16 that hold the
+// group, its scale. Lanes of a half-warp hold the 16 units of one group in order.
+template <typename T, typename Code>
+__device__ __forceinline__ uint2 encode_unit(const uint4 &v, float *scale)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    // The largest magnitude by its bits, which order like the values and put inf and NaN on top.
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    const uint32_t top = max(m & 0xFFFFu, m >> 16);
+    const float a = T::unpack(top).x;
+    float inv = 0.f;
+    if (top >= T::kInf) {
+        *scale = __int_as_float(0x7FC00000);
+        return make_uint2(0u, 0u);
+    }
+    if (a < 0x1p-100f) {
+        *scale = 0.f;
+        return make_uint2(0u, 0u);
+    }
+    inv = __fdiv_rn(Code::kMax, a);
+    *scale = __fdiv_rn(a, Code::kMax);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = T::unpack(w[i]);
+        x[2 * i] = __fmul_rn(f.x, inv);
+        x[2 * i + 1] = __fmul_rn(f.y, inv);
+    }
+    return make_uint2(Code::encode4(x[0], x[1], x[2], x[3]), Code::encode4(x[4], x[5], x[6], x[7]));
+}
+
+// Eight codes -> the eight 16-bit values they stand for.
+template <typename T, typename Code>
+__device__ __forceinline__ uint4 decode_unit(const uint2 &c, float scale)
+{
+    const float4 a = Code::decode4(c.x), b = Code::decode4(c.y);
+    return make_uint4(T::pack(__fmul_rn(a.x, scale), __fmul_rn(a.y, scale)),
+                      T::pack(__fmul_rn(a.z, scale), __fmul_rn(a.w, scale)),
+                      T::pack(__fmul_rn(b.x, scale), __fmul_rn(b.y, scale)),
+                      T::pack(__fmul_rn(b.z, scale), __fmul_rn(b.w, scale)));
+}
+
+}  // namespace kvb

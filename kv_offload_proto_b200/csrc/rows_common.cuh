@@ -57,11 +57,11 @@ __device__ __forceinline__ void cta_copy_rows(const uint8_t *const *src, uint8_t
 }
 
 // The gather rule for flat position `pos` (= batch row * top_k + k) of one layer
-// (kvc_gather_rows.cpp:54-76) on its loaded inputs: true with the row's source and hot
-// destination when the position is a miss with a valid token, slot and pool row on a selected
-// node. Records KVOPS_ERR_SEG_NULL or the row band for a null segment or a row past the segment.
-__device__ __forceinline__ bool gather_eval(const GatherParams &p, int64_t pos, int8_t miss, int32_t t, int32_t slot,
-                                            int64_t req, int64_t base, const uint8_t **src_out, uint8_t **dst_out)
+// (kvc_gather_rows.cpp:54-76) on its loaded inputs: true with the row's segment address when the
+// position is a miss with a valid token, slot and pool row on a selected node. Records
+// KVOPS_ERR_SEG_NULL or the row band for a null segment or a row past the segment.
+__device__ __forceinline__ bool gather_source(const GatherParams &p, int64_t pos, int8_t miss, int32_t t, int32_t slot,
+                                              int64_t req, int64_t base, const uint8_t **src_out)
 {
     if (miss == 0) return false;                     // :55-57
     if (t < 0 || slot < 0 || req < 0) return false;  // :62-68
@@ -79,6 +79,14 @@ __device__ __forceinline__ bool gather_eval(const GatherParams &p, int64_t pos, 
         return false;
     }
     *src_out = seg + (p.layer_offset_rows + seg_row) * static_cast<uint64_t>(p.row_bytes);
+    return true;
+}
+
+// The same with the row's hot destination.
+__device__ __forceinline__ bool gather_eval(const GatherParams &p, int64_t pos, int8_t miss, int32_t t, int32_t slot,
+                                            int64_t req, int64_t base, const uint8_t **src_out, uint8_t **dst_out)
+{
+    if (!gather_source(p, pos, miss, t, slot, req, base, src_out)) return false;
     *dst_out = p.hot + static_cast<uint64_t>(req) * p.hot_req_stride_bytes +
                static_cast<uint64_t>(slot) * p.row_bytes;  // :73-76
     return true;
@@ -137,6 +145,34 @@ __device__ __forceinline__ void gather_tile(const GatherParams &p, int64_t base,
     __syncthreads();
     if (threadIdx.x == 0) *s_n = 0;
     __syncthreads();
+}
+
+// Destination unit k of one layer -> (source row, segment row); false if outside the range.
+// Reference map with S > 1: unit k is the k-th owned stripe and only its last row in range is
+// copied, because the reference's ascending per-row writes leave exactly that row in the
+// shared segment row (kvc_scatter_rows_alllayer.cpp:34-53).
+__device__ __forceinline__ bool export_unit(const ExportParams &p, uint64_t k, uint32_t *src_row, uint32_t *seg_row)
+{
+    const uint64_t lo = p.row_lo, hi = static_cast<uint64_t>(p.row_lo) + p.row_cnt - 1;
+    if (p.stripe == 0) {
+        *src_row = static_cast<uint32_t>(lo + k);
+        *seg_row = *src_row;
+        return true;
+    }
+    const uint64_t S = p.stripe;
+    if (!p.injective) {
+        const uint64_t g = p.g_first + k * p.nodes;
+        const uint64_t last = (g + 1) * S - 1;
+        *src_row = static_cast<uint32_t>(last < hi ? last : hi);
+        *seg_row = static_cast<uint32_t>(g / p.nodes);
+        return true;
+    }
+    const uint64_t g = p.g_first + (k / S) * p.nodes;
+    const uint64_t r = g * S + k % S;
+    if (r < lo || r > hi) return false;
+    *src_row = static_cast<uint32_t>(r);
+    *seg_row = static_cast<uint32_t>((g / p.nodes) * S + k % S);
+    return true;
 }
 
 }  // namespace kvb

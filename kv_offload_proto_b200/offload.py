@@ -12,8 +12,12 @@ import contextlib
 import torch
 
 from . import kvops as _kvops_module
+from .pool import dtype_name
 
-__all__ = ["XdsOffloadCoordinator", "align", "compute_ht_size"]
+__all__ = ["XdsOffloadCoordinator", "align", "compute_ht_size", "tree_masks"]
+
+KEY_DIM, VALUE_DIM = 576, 512  # values of a row that attention scores use, and that it sums
+ROW_BYTES = {"raw": 1152, "e4m3": 656, "int8": 656}
 
 
 def align(v, a):
@@ -28,6 +32,27 @@ def compute_ht_size(padded_buffer_size, top_k):
     while p < 2 * (padded_buffer_size + top_k):
         p <<= 1
     return p
+
+
+def tree_masks(parents):
+    """The words that `XdsOffloadCoordinator.attend` takes as `tree`, from each drafted token's
+    parent: parents[..., j] is the drafted token that token j continues (j's own index is larger),
+    or -1 where it continues the context. Bit i of word j is set where i is j or an ancestor of j.
+    Returns int64 of the same shape on the same device; up to 64 drafted tokens."""
+    parents = torch.as_tensor(parents)
+    n = parents.shape[-1]
+    if n > 64:
+        raise ValueError("at most 64 drafted tokens, got {}".format(n))
+    index = torch.arange(n, device=parents.device)
+    if parents.is_floating_point() or bool(((parents < -1) | (parents >= index)).any()):
+        raise ValueError("parents[..., j] must be an integer in [-1, j)")
+    parents = parents.to(torch.int64)
+    masks = torch.zeros(parents.shape, dtype=torch.int64, device=parents.device)
+    for j in range(n):
+        up = masks.gather(-1, parents[..., j:j + 1].clamp(min=0))[..., 0]
+        bit = 1 << j if j < 63 else -(1 << 63)
+        masks[..., j] = torch.where(parents[..., j] >= 0, up, torch.zeros_like(up)) | bit
+    return masks
 
 
 class XdsOffloadCoordinator:
@@ -133,3 +158,98 @@ class XdsOffloadCoordinator:
     def miss_count(self):
         """Device-side miss count tensor (xds_offload.py:103-106)."""
         return self.is_miss.sum()
+
+    def attend(self, q, hot_row_base, *, hot_req_stride_rows=0, hot_rows=None, row_format="raw", scale=None,
+               topk_device_slots=None, draft_rows=None, tree=None, out=None, lse=None, workspace=None, stream=None):
+        """Attention of this step's tokens over one layer's hot rows (kvops_attend_hot).
+
+        q: float16 or bfloat16 [B, heads, 576] (one token a request) or [B, tokens, heads, 576],
+        B <= max_num_reqs; its batch rows are set_batch's. The keys of request r are the hot rows
+        of its slots (the last sieve_update's top_k_device_slots, or `topk_device_slots`: int32
+        [B, K], or [B, tokens, K] for a list per token), entries outside [0, hot_rows) left out,
+        and of draft_rows [B, drafts, 576] those whose bit is set in tree[r, token] (int64
+        [B, tokens], see tree_masks; None: a chain, token t seeing drafted rows 0..t). A row's
+        first 512 values are its value. hot_row_base: the layer's hot rows (a tensor, or an
+        address), hot_req_stride_rows from one pool row to the next (0: shared), of row_format
+        "raw" (the type of q) or stored in 8 bits. hot_rows: rows a slot may name (default: the
+        stride, or device_buffer_size for shared rows). scale: of the scores, default 576 ** -0.5.
+
+        Returns (out, lse): [.., heads, 512] in q's type and fp32 [.., heads], written for the
+        batch rows below num_real only. A token without any key gets out 0 and lse -inf. out, lse
+        and workspace (uint8, at least _kvops.attend_workspace(...) bytes, used by one call at a
+        time) may be given; otherwise they are allocated for the call."""
+        squeeze = q.dim() == 3
+        if squeeze:
+            q = q.unsqueeze(1)
+        if q.dim() != 4 or q.shape[3] != KEY_DIM or q.stride(3) != 1:
+            raise ValueError("attend: q must be [B, heads, 576] or [B, tokens, heads, 576] with unit last stride")
+        B, T, H, _ = q.shape
+        dtype = dtype_name(q.dtype)
+        if B > self.max_num_reqs:
+            raise ValueError("attend: {} batch rows, max_num_reqs is {}".format(B, self.max_num_reqs))
+        if self._req_pool_indices is None or self._req_pool_indices.shape[0] < B:
+            raise RuntimeError("attend: call set_batch() with at least q's batch rows first")
+        slots = self.top_k_device_slots if topk_device_slots is None else topk_device_slots
+        if slots.dtype != torch.int32 or slots.dim() not in (2, 3) or slots.shape[0] < B or \
+                (slots.dim() == 3 and slots.shape[1] != T) or (slots.shape[-1] > 1 and slots.stride(-1) != 1):
+            raise ValueError("attend: topk_device_slots must be int32 [B, K] or [B, tokens, K] with unit last stride")
+        if row_format not in ROW_BYTES:
+            raise ValueError("attend: row_format must be 'raw', 'e4m3' or 'int8', got {!r}".format(row_format))
+        if hot_rows is None:
+            hot_rows = hot_req_stride_rows or self.device_buffer_size
+        D = 0
+        if draft_rows is not None:
+            if draft_rows.dim() != 3 or draft_rows.shape[0] < B or draft_rows.shape[2] != KEY_DIM or \
+                    draft_rows.dtype != q.dtype or draft_rows.stride(2) != 1:
+                raise ValueError("attend: draft_rows must be [B, drafts, 576] of q's type with unit last stride")
+            D = draft_rows.shape[1]
+        if tree is not None and (tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] < B or
+                                 tree.shape[1] != T or not tree.is_contiguous()):
+            raise ValueError("attend: tree must be a contiguous int64 [B, tokens]")
+        if isinstance(hot_row_base, torch.Tensor):
+            need = ((self.pool_size - 1) * hot_req_stride_rows + hot_rows) * ROW_BYTES[row_format]
+            if hot_row_base.numel() * hot_row_base.element_size() < need or not hot_row_base.is_contiguous():
+                raise ValueError("attend: hot rows must be contiguous and hold {} bytes".format(need))
+            hot = hot_row_base.data_ptr()
+        else:
+            hot = hot_row_base
+        for name, x, shape, want in (("out", out, (B, T, H, VALUE_DIM), q.dtype), ("lse", lse, (B, T, H), torch.float32)):
+            if x is not None and (x.dtype != want or not x.is_contiguous() or x.numel() != B * T * H * (
+                    VALUE_DIM if name == "out" else 1) or x.device != q.device):
+                raise ValueError("attend: {} must be a contiguous {} {}".format(name, want, shape))
+        for x in (q, slots, draft_rows, tree, workspace):
+            if x is not None and x.device != self.top_k_device_slots.device:
+                raise ValueError("attend: every tensor must be on {}".format(self.top_k_device_slots.device))
+        with self._on_device():
+            if stream is None:
+                return self._attend(q, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale, slots, draft_rows,
+                                    D, tree, out, lse, workspace, self._stream(), squeeze)
+            # what is allocated below belongs to the stream that uses it
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+                return self._attend(q, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale, slots, draft_rows,
+                                    D, tree, out, lse, workspace, stream, squeeze)
+
+    def _attend(self, q, hot, stride, hot_rows, row_format, dtype, scale, slots, draft, D, tree, out, lse, workspace,
+                stream, squeeze):
+        B, T, H, _ = q.shape
+        K = slots.shape[-1]
+
+        def step(x, d):  # the stride of a dimension of one entry is never used
+            return x.stride(d) if x.shape[d] > 1 else 0
+
+        if out is None:
+            out = torch.empty((B, H, VALUE_DIM) if squeeze else (B, T, H, VALUE_DIM), dtype=q.dtype, device=q.device)
+        if lse is None:
+            lse = torch.empty((B, H) if squeeze else (B, T, H), dtype=torch.float32, device=q.device)
+        if workspace is None:
+            need = self._k.attend_workspace(B, T, H, K, D, row_format, dtype)
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        self._k.attend_hot(
+            q.data_ptr(), step(q, 0), step(q, 1), step(q, 2), hot, stride, hot_rows,
+            self._req_pool_indices.data_ptr(), self.pool_size, slots.data_ptr(), step(slots, 0),
+            step(slots, 1) if slots.dim() == 3 else 0, self.num_real.data_ptr(),
+            draft.data_ptr() if D else 0, step(draft, 0) if D else 0, step(draft, 1) if D else 0,
+            tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
+            workspace.data_ptr() if workspace is not None else 0, workspace.numel() if workspace is not None else 0,
+            B, T, H, K, D, row_format, dtype, KEY_DIM ** -0.5 if scale is None else scale, stream)
+        return out, lse

@@ -16,7 +16,7 @@ from typing import List, Optional, Sequence
 from . import kvops as _kvops_module
 
 __all__ = ["DevicePool", "RowAllocator", "per_layer_seg_rows", "per_layer_seg_rows_injective", "node_of",
-           "seg_row_of", "device_view"]
+           "seg_row_of", "device_view", "dtype_name"]
 
 
 class _CudaArray:
@@ -143,17 +143,35 @@ class RowAllocator:
         return self.capacity - self._nfree
 
 
+def dtype_name(dtype):
+    """'fp16' or 'bf16' of a torch dtype or of such a name: the 16-bit type of a row's values."""
+    name = {"torch.float16": "fp16", "torch.bfloat16": "bf16"}.get(str(dtype), dtype)
+    if name not in ("fp16", "bf16"):
+        raise ValueError("rows must be float16 or bfloat16, got {}".format(dtype))
+    return name
+
+
 class DevicePool:
     """Pool of `node_num` segments, each on a device id (>= 0) or pinned host memory (-1).
 
     segment_devices[s] places segment s. Segments are allocated here unless
     `segment_addrs` gives existing UVA addresses (e.g. opened from other processes' IPC
     handles), in which case this object does not own them.
+
+    row_format "e4m3" or "int8" stores rows in 8 bits: `row_bytes` stays the size of the caller's
+    16-bit rows (of row_dtype, a torch dtype or 'fp16' / 'bf16'), their last plain_elems values
+    are kept as they are and the others are quantised in groups of 128 (a 1152-byte row takes 656
+    bytes, `seg_row_bytes`). batch_write_alllayers and batch_write then quantise as they write;
+    batch_read and sieve_and_read read the miss rows back into 16-bit hot rows. With
+    hot_quantized=True the hot rows are stored rows too (seg_row_bytes each): batch_read,
+    sieve_and_read and batch_write move them unchanged, `XdsOffloadCoordinator.attend` reads them
+    as they are, and only batch_write_alllayers quantises.
     """
 
     def __init__(self, device_id: int, layer_num: int, layer_rows: int, row_bytes: int, stripe_rows: int = 1,
                  segment_devices: Sequence[int] = (0,), segment_addrs: Optional[Sequence[int]] = None,
-                 injective: bool = False):
+                 injective: bool = False, *, row_format: str = "raw", row_dtype="fp16", plain_elems: int = 64,
+                 hot_quantized: bool = False):
         if layer_num < 1 or layer_rows < 1 or row_bytes <= 0 or row_bytes % 128 != 0:
             raise ValueError("invalid pool dims: L={} rows={} rowBytes={}".format(layer_num, layer_rows, row_bytes))
         n = len(segment_devices) if segment_addrs is None else len(segment_addrs)
@@ -166,6 +184,22 @@ class DevicePool:
         self.layer_num = layer_num
         self.layer_rows = layer_rows
         self.row_bytes = row_bytes
+        self.row_format = row_format
+        self.hot_quantized = hot_quantized
+        if row_format == "raw":
+            if hot_quantized:
+                raise ValueError("hot_quantized needs a row_format of 8 bits")
+            self._codec = None
+            self.seg_row_bytes = row_bytes
+        elif row_format in ("e4m3", "int8"):
+            self._codec = (row_format, dtype_name(row_dtype), row_bytes // 2 - plain_elems, plain_elems)
+            if not 0 <= plain_elems < row_bytes // 2:
+                raise ValueError("plain_elems must be in [0, {})".format(row_bytes // 2))
+            self.seg_row_bytes = self._k.quant_row_bytes(*self._codec)
+        else:
+            raise ValueError("row_format must be 'raw', 'e4m3' or 'int8', got {!r}".format(row_format))
+        # what the copies between hot rows and segment rows convert (None: they move rows unchanged)
+        self._hot_codec = None if hot_quantized else self._codec
         self.stripe_rows = stripe_rows
         self.injective = injective
         self.node_num = n
@@ -173,7 +207,7 @@ class DevicePool:
             self.per_layer_seg_rows = per_layer_seg_rows_injective(layer_rows, stripe_rows, n)
         else:
             self.per_layer_seg_rows = per_layer_seg_rows(layer_rows, n)
-        self.segment_bytes = layer_num * self.per_layer_seg_rows * row_bytes
+        self.segment_bytes = layer_num * self.per_layer_seg_rows * self.seg_row_bytes
         self.channels = [0] * n  # seg_base is directly dereferenceable (UVA)
         self._owned = []
         if segment_addrs is None:
@@ -204,7 +238,7 @@ class DevicePool:
     def seg_addr(self, node, layer, row):
         """Byte address of (layer, row) inside node's segment (test/kv_layout_ref.py:19-24)."""
         sr = seg_row_of(row, self.stripe_rows, self.node_num, self.injective)
-        return self.seg_bases[node] + (layer * self.per_layer_seg_rows + sr) * self.row_bytes
+        return self.seg_bases[node] + (layer * self.per_layer_seg_rows + sr) * self.seg_row_bytes
 
     def batch_read(self, layer_id, topk_indices, req_pool_indices, req_host_base, topk_device_slots, is_miss,
                    num_real, hot_row_base, max_num_reqs, top_k, stream=0, block_dim=1, *, fused=True,
@@ -212,18 +246,23 @@ class DevicePool:
         """Gather the miss rows of one layer from every segment (xds_ems_pool.py:204-217).
 
         fused=True issues one launch over all segments (import_multi); fused=False issues the
-        reference's one import_seg launch per segment. Both publish the same status pages."""
+        reference's one import_seg launch per segment. Both publish the same status pages. Rows
+        stored in 8 bits are read back by one launch over all segments either way."""
         status = self.next_status()
         off = layer_id * self.per_layer_seg_rows
         a = [_ptr(topk_indices), _ptr(req_pool_indices), _ptr(req_host_base), _ptr(topk_device_slots),
              _ptr(is_miss), _ptr(num_real), _ptr(hot_row_base)]
-        if fused:
-            self._k.import_multi(self.seg_bases, off, self.per_layer_seg_rows, self.row_bytes, *a, top_k, max_num_reqs,
+        if self._hot_codec is not None:
+            self._k.import_quant(self.seg_bases, off, self.per_layer_seg_rows, *self._hot_codec, *a, top_k,
+                                 max_num_reqs, self.stripe_rows, status, stream, block_dim,
+                                 hot_req_stride_rows=hot_req_stride_rows, injective=self.injective)
+        elif fused:
+            self._k.import_multi(self.seg_bases, off, self.per_layer_seg_rows, self.seg_row_bytes, *a, top_k, max_num_reqs,
                                  self.stripe_rows, status, stream, block_dim, hot_req_stride_rows=hot_req_stride_rows,
                                  injective=self.injective)
         else:
             for s in range(self.node_num):
-                self._k.import_seg(self.channels[s], self.seg_bases[s], off, self.per_layer_seg_rows, self.row_bytes,
+                self._k.import_seg(self.channels[s], self.seg_bases[s], off, self.per_layer_seg_rows, self.seg_row_bytes,
                                    *a, top_k, max_num_reqs, self.stripe_rows, self.node_num, s, status, stream,
                                    block_dim, hot_req_stride_rows=hot_req_stride_rows, injective=self.injective)
         return status
@@ -244,6 +283,9 @@ class DevicePool:
         import torch
         if topk_indices.dtype != torch.int32:
             raise ValueError("topk_indices must be int32")
+        if self._hot_codec is not None:
+            return self._sieve_and_read_quant(coord, layer_id, topk_indices, hot_row_base, stream, block_dim,
+                                              hot_req_stride_rows, path, publish, err_word)
         status = self.next_status() if publish else 0
         self._k.sieve_import(
             _ptr(topk_indices), _ptr(coord._req_pool_indices), _ptr(coord._seq_lens), _ptr(coord.prefill_lens),
@@ -251,9 +293,25 @@ class DevicePool:
             _ptr(coord.device_buffer_ht[layer_id]), _ptr(coord.sieve_hand[layer_id]), _ptr(coord.top_k_device_slots),
             _ptr(coord.is_miss), _ptr(coord.num_real), coord.top_k, coord.device_buffer_size,
             coord.padded_buffer_size, coord.visited_stride_b, coord.max_num_reqs, coord.pool_size, self.seg_bases,
-            layer_id * self.per_layer_seg_rows, self.per_layer_seg_rows, self.row_bytes, _ptr(coord.req_host_base),
+            layer_id * self.per_layer_seg_rows, self.per_layer_seg_rows, self.seg_row_bytes, _ptr(coord.req_host_base),
             _ptr(hot_row_base), self.stripe_rows, status, stream, block_dim, hot_req_stride_rows=hot_req_stride_rows,
             injective=self.injective, path=path, err_word=_ptr(err_word), copy_wait_polls=copy_wait_polls)
+        return status
+
+    def _sieve_and_read_quant(self, coord, layer_id, topk_indices, hot_row_base, stream, block_dim,
+                              hot_req_stride_rows, path, publish, err_word):
+        """The layer-step when the read converts rows: the SIEVE kernel, then the read launched as
+        its programmatic dependent (the one-kernel paths move rows unchanged)."""
+        if path not in ("auto", "split"):
+            raise ValueError("sieve_and_read: rows stored in 8 bits run path 'auto' or 'split', got {!r}".format(path))
+        status = self.next_status() if publish else 0
+        coord.sieve_update(layer_id, topk_indices, stream=stream)
+        self._k.import_quant(self.seg_bases, layer_id * self.per_layer_seg_rows, self.per_layer_seg_rows,
+                             *self._hot_codec, _ptr(topk_indices), _ptr(coord._req_pool_indices),
+                             _ptr(coord.req_host_base), _ptr(coord.top_k_device_slots), _ptr(coord.is_miss),
+                             _ptr(coord.num_real), _ptr(hot_row_base), coord.top_k, coord.max_num_reqs,
+                             self.stripe_rows, status, stream, block_dim, hot_req_stride_rows=hot_req_stride_rows,
+                             injective=self.injective, err_word=_ptr(err_word))
         return status
 
     def batch_write(self, layer_id, topk_indices, req_pool_indices, req_host_base, topk_device_slots, export_flags,
@@ -266,7 +324,13 @@ class DevicePool:
         a = [_ptr(topk_indices), _ptr(req_pool_indices), _ptr(req_host_base), _ptr(topk_device_slots),
              _ptr(export_flags), _ptr(num_real), _ptr(hot_row_base)]
         for s in range(self.node_num):
-            self._k.export_seg(self.channels[s], self.seg_bases[s], off, self.per_layer_seg_rows, self.row_bytes, *a,
+            if self._hot_codec is not None:
+                self._k.export_quant(self.channels[s], self.seg_bases[s], off, self.per_layer_seg_rows,
+                                     *self._hot_codec, *a, top_k, max_num_reqs, self.stripe_rows, self.node_num, s,
+                                     status, stream, block_dim, hot_req_stride_rows=hot_req_stride_rows,
+                                     injective=self.injective)
+                continue
+            self._k.export_seg(self.channels[s], self.seg_bases[s], off, self.per_layer_seg_rows, self.seg_row_bytes, *a,
                                top_k, max_num_reqs, self.stripe_rows, self.node_num, s, status, stream, block_dim,
                                hot_req_stride_rows=hot_req_stride_rows, injective=self.injective)
         return status
@@ -276,6 +340,12 @@ class DevicePool:
         (xds_ems_pool.py:220-230): one launch per segment, as in the reference."""
         status = self.next_status()
         for s in range(self.node_num):
+            if self._codec is not None:
+                self._k.export_quant_alllayer(self.channels[s], self.seg_bases[s], self.per_layer_seg_rows,
+                                              *self._codec, row_lo, row_cnt, self.layer_num, _ptr(src_layer0_base),
+                                              src_layer_stride, self.stripe_rows, self.node_num, s, status, stream,
+                                              block_dim, injective=self.injective)
+                continue
             self._k.export_seg_alllayer(self.channels[s], self.seg_bases[s], self.per_layer_seg_rows, self.row_bytes,
                                         row_lo, row_cnt, self.layer_num, _ptr(src_layer0_base), src_layer_stride,
                                         self.stripe_rows, self.node_num, s, status, stream, block_dim,
