@@ -54,6 +54,7 @@ extern "C" {
 #define KVOPS_ERR_SEG_NULL 0x101u  /* segment base is 0: nothing touched (0x1xx, init band) */
 #define KVOPS_ERR_ROW_BASE 0x200u  /* 0x200 + (index & 0xFF) + (1 << 16): row out of the segment */
 #define KVOPS_ERR_COPY_TIMEOUT 0x102u  /* kvops_sieve_import: a copy CTA stopped waiting for a walk list */
+#define KVOPS_ERR_ATTEND_TIMEOUT 0x103u  /* kvops_attend_hot: a wait inside the kernel gave up; outputs are not valid */
 
 /* Largest node count of one layout (common/kv_layout.h:45, KvLayoutValidate). */
 #define KVOPS_MAX_NODES 64
@@ -346,6 +347,7 @@ typedef struct KvopsAttend {
     uint64_t lse;                  /* fp32 [max_num_reqs, tokens, heads], 0: not wanted */
     uint64_t workspace;            /* kvops_attend_workspace bytes, 16-byte aligned; one launch at a time */
     uint64_t workspace_bytes;
+    uint64_t err_word;             /* as KvopsRowOpts.err_word: KVOPS_ERR_ATTEND_TIMEOUT; 0: none */
     uint32_t max_num_reqs, tokens, heads, top_k, drafts; /* tokens and drafts <= 64, heads <= 128 */
     uint32_t hot_rows;             /* rows per request that a slot may name */
     uint32_t pool_size;

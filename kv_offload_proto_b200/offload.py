@@ -160,7 +160,8 @@ class XdsOffloadCoordinator:
         return self.is_miss.sum()
 
     def attend(self, q, hot_row_base, *, hot_req_stride_rows=0, hot_rows=None, row_format="raw", scale=None,
-               topk_device_slots=None, draft_rows=None, tree=None, out=None, lse=None, workspace=None, stream=None):
+               topk_device_slots=None, draft_rows=None, tree=None, out=None, lse=None, workspace=None, stream=None,
+               err_word=0):
         """Attention of this step's tokens over one layer's hot rows (kvops_attend_hot).
 
         q: float16 or bfloat16 [B, heads, 576] (one token a request) or [B, tokens, heads, 576],
@@ -177,7 +178,8 @@ class XdsOffloadCoordinator:
         Returns (out, lse): [.., heads, 512] in q's type and fp32 [.., heads], written for the
         batch rows below num_real only. A token without any key gets out 0 and lse -inf. out, lse
         and workspace (uint8, at least _kvops.attend_workspace(...) bytes, used by one call at a
-        time) may be given; otherwise they are allocated for the call."""
+        time) may be given; otherwise they are allocated for the call. err_word: address (or int32
+        tensor) of a word that receives errCode 0x103 if a wait inside the kernel gave up."""
         squeeze = q.dim() == 3
         if squeeze:
             q = q.unsqueeze(1)
@@ -223,14 +225,14 @@ class XdsOffloadCoordinator:
         with self._on_device():
             if stream is None:
                 return self._attend(q, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale, slots, draft_rows,
-                                    D, tree, out, lse, workspace, self._stream(), squeeze)
+                                    D, tree, out, lse, workspace, self._stream(), squeeze, err_word)
             # what is allocated below belongs to the stream that uses it
             with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
                 return self._attend(q, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale, slots, draft_rows,
-                                    D, tree, out, lse, workspace, stream, squeeze)
+                                    D, tree, out, lse, workspace, stream, squeeze, err_word)
 
     def _attend(self, q, hot, stride, hot_rows, row_format, dtype, scale, slots, draft, D, tree, out, lse, workspace,
-                stream, squeeze):
+                stream, squeeze, err_word):
         B, T, H, _ = q.shape
         K = slots.shape[-1]
 
@@ -251,5 +253,6 @@ class XdsOffloadCoordinator:
             draft.data_ptr() if D else 0, step(draft, 0) if D else 0, step(draft, 1) if D else 0,
             tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
             workspace.data_ptr() if workspace is not None else 0, workspace.numel() if workspace is not None else 0,
-            B, T, H, K, D, row_format, dtype, KEY_DIM ** -0.5 if scale is None else scale, stream)
+            B, T, H, K, D, row_format, dtype, KEY_DIM ** -0.5 if scale is None else scale, stream,
+            err_word=err_word if isinstance(err_word, int) else err_word.data_ptr())
         return out, lse
