@@ -3,20 +3,28 @@
 // include/kvops_b200.h).
 //
 // A key row is read once for its score and its value, and every head and drafted token of a
-// request shares it, so both products are matrix products over tiles of 128 keys:
-//   S^T [128 keys x NQ queries] = K [128 x 576] Q^T,   O^T [512 x NQ] += V^T [512 x 128] P^T,
+// request shares it, so both products are matrix products over tiles of 64 keys:
+//   S^T [64 keys x NQ queries] = K [64 x 576] Q^T,   O^T [512 x NQ] += V^T [512 x 64] P^T,
 // with V the first 512 columns of K: one copy of the rows in shared memory serves both, K-major for
-// the first and MN-major for the second. The transposed form keeps the matrix unit's 128 rows full
-// (keys, then value dimensions) for any number of queries: with the queries as rows a tile of 64
-// would run at half rate, and 128 rows of 512 fp32 outputs would fill tensor memory and leave no
-// room for the scores. Measured on one SM: M = 64 takes 64 cycles for N = 128, 16 deep; M = 128, N = 64
-// takes 48 (the operands' 6 KB at 128 bytes a cycle).
+// the first and MN-major for the second. The transposed form keeps the matrix unit's 128 rows full of
+// value dimensions for any number of queries: with the queries as rows, a tile of 64 would run at half
+// rate, and 128 rows of 512 fp32 outputs would fill tensor memory and leave no room for the scores.
+// Operands come from shared memory at 128 bytes a cycle, which bounds both products: 48 cycles for
+// 16 dimensions (or keys) at NQ = 64, 36 + 16 of them a tile. Tiles of 128 keys would take 48 cycles
+// for twice the keys in the first product, but leave no room for a second tile beside the queries:
+// rows, products and softmax then take turns (12200 cycles for 128 keys, where this takes REPLACE).
 //
 // One CTA per SM takes a run of (query tile, key tile) pairs. Warps 0-7: the softmax, a thread per
-// key and half of the queries, and the outputs. Warps 8-15: the rows, by asynchronous 16-byte copies
-// or, from stored rows, through registers. Warp 16: one thread issues the matrix instructions.
-// Shared memory holds one key tile in five groups (four of 128 dimensions, one of the 64 rotary
-// ones) that are refilled one by one as the second product passes them.
+// key and half of the queries, and the outputs. Warps 8-15: the rows,
+// by asynchronous 16-byte copies, four rows of 128 bytes an instruction (38 bytes a cycle and SM; gathering
+// tensor copies of the same 512 bytes reach 48 alone, but cost the thread that issues them 190 cycles
+// each beside the other warps, which left 18). 16-bit rows land where the products read them; stored
+// rows' codes land in a warp's own place and are converted from there. Warps 16 and
+// 17 issue the two products: the first of the next tile goes ahead of the second of this one, whose
+// probabilities the softmax is still working out. Warp 18 finds the rows that the lists name, a few
+// tiles ahead. A key tile is four groups of 128 dimensions (16 KB)
+// and the 64 rotary dimensions (8 KB). The groups go through a ring of places that the second product
+// frees one by one, so rows travel while earlier ones are still in use.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stddef.h>
@@ -36,12 +44,15 @@ constexpr int kValueDim = 512;          // values of a row that the output sums
 constexpr int kKeyDim = 576;            // values of a row that the scores use
 constexpr uint32_t kStoredBytes = 656;  // of a stored row of 512 + 64 values
 constexpr uint32_t kStoredPlain = 528;  // where its 64 rotary values start
-constexpr int kTile = 128;              // keys per tile
-constexpr int kChunks = kKeyDim / 64;   // 128-byte columns of a tile
-constexpr uint32_t kChunkBytes = kTile * 128;
-constexpr int kGroups = 5;              // chunks 0-1, 2-3, 4-5, 6-7, 8
-constexpr int kSoftmaxWarps = 8, kLoadWarps = 8;
-constexpr int kThreads = (kSoftmaxWarps + kLoadWarps + 1) * 32;
+constexpr int kTile = 64;               // keys per tile
+constexpr uint32_t kChunkBytes = kTile * 128;  // 64 dimensions of a tile's keys, in 128-byte rows
+constexpr uint32_t kGroupBytes = 2 * kChunkBytes;
+constexpr int kSoftmaxWarps = 8;
+
+constexpr int kLoadWarps = 8;
+constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kWeighWarp = kScoreWarp + 1, kFindWarp = kScoreWarp + 2;
+constexpr int kThreads = (kFindWarp + 1) * 32;
+constexpr uint32_t kAhead = 4;  // tiles whose rows are known at a time
 
 // A running reference is kept this far (in powers of two) below the largest score seen, so that
 // the probabilities, up to 2^kLift, lose none of their small neighbours to fp16's subnormals, and it is
@@ -55,12 +66,22 @@ struct Plan {
     uint32_t lists;       // lists per request: 1, or tokens
     uint32_t group_rows;  // query rows that share a list
     uint32_t qtiles;      // query tiles per group
+    uint32_t list_end;    // top_k rounded up to four: where the drafted rows start among the keys
     uint32_t tiles;       // key tiles per unit
     uint32_t ctas;
     uint32_t whole;       // > 0: every CTA takes this many whole units; 0: an equal run of pairs
     float2 *part_ml;      // [2 * ctas][NQ] reference and sum of a unit's part
-    float *part_o;        // [2 * ctas][NQ][512] its weighted sums
+    float *part_o;        // [2 * ctas][NQ * 512] its weighted sums, in part_at's order
 };
+
+// Where (as float4) a part keeps the sums of dimension block * 128 + quarter * 32 + lane of the four
+// queries 4 i .. 4 i + 3 of a half: the order in which the softmax warps hold them.
+template <int NQ>
+__device__ __forceinline__ uint64_t part_at(uint32_t slot, uint32_t block, uint32_t quarter, uint32_t half, uint32_t i,
+                                            uint32_t lane)
+{
+    return ((((static_cast<uint64_t>(slot) * 4 + block) * 4 + quarter) * 2 + half) * (NQ / 8) + i) * 32 + lane;
+}
 
 __device__ __forceinline__ uint32_t real_units(const KvopsAttend &a, const Plan &p)
 {
@@ -85,7 +106,7 @@ struct Unit {
 };
 
 template <int NQ>
-__device__ __forceinline__ Unit unit_at(const KvopsAttend &a, const Plan &p, uint32_t unit)
+__device__ __forceinline__ Unit unit_at(const Plan &p, uint32_t unit)
 {
     Unit u;
     const uint32_t group = unit / p.qtiles;
@@ -103,22 +124,33 @@ __device__ __forceinline__ uint32_t token_of(const KvopsAttend &a, const Plan &p
     return p.lists > 1 ? u.token : row / a.heads;
 }
 
-template <int NQ>
+// Shared memory: a ring of groups, the rotary dimensions of two tiles, the queries, and for stored
+// rows the codes of a tile, 32 rows x 128 bytes of it each load warp's own. A tile's probabilities [64 keys]
+// [64 x 16 bit] take the place of its rotary dimensions, which only the scores need.
+template <int NQ, bool kStored>
 struct Layout {
-    static constexpr uint32_t q = kChunks * kChunkBytes;
-    // The probabilities [128 keys][64 x 16 bit] take the place of the rotary columns, which only the
-    // scores need, where the queries leave no room for them elsewhere.
-    static constexpr uint32_t p = NQ == 64 ? 8 * kChunkBytes : q + NQ * 2 * kKeyDim;
-    static constexpr uint32_t bytes = (NQ == 64 ? q + NQ * 2 * kKeyDim : p + kChunkBytes) + 1024;
+    // as many as fit beside the queries; a tile has four groups
+    static constexpr int places = kStored ? (NQ == 64 ? 6 : 8) : NQ == 64 ? 8 : NQ == 32 ? 10 : 11;
+    static constexpr uint32_t rope = places * kGroupBytes;
+    static constexpr uint32_t q = rope + 2 * kChunkBytes;
+    static constexpr uint32_t stage = q + NQ * 2 * kKeyDim;
+    static constexpr uint32_t bytes = stage + (kStored ? kTile * kValueDim : 0) + 1024;
+    static_assert(bytes + 6 * 1024 <= 227 * 1024, "with the static part");
 };
+constexpr int kMostPlaces = 11;
 
 struct Shared {
-    alignas(8) uint64_t q_full, full[kGroups], empty[kGroups], s_full, p_full, meta_full[2], meta_empty[2];
-    uint64_t tree[64];         // of the unit's query rows
-    float top[2][4][32];       // a tile's maxima by column, by half and lane quarter
     alignas(16) float per_warp[kSoftmaxWarps][32];  // read four at a time
-    uint8_t kind[2][kTile];    // of the tile's keys: kNone, kList, kDraft or kBadDraft
-    uint32_t any[2];           // whether the tile has a key
+    float top[2][4][32];       // a tile's maxima by column, by half and lane quarter
+    uint64_t tree[64];         // of the unit's query rows
+    // full: rows have landed; empty: the second product is done with them; done: with a tile; rope_*:
+    // a tile's rotary dimensions, then probabilities; out_free: a unit's outputs have left that place
+    uint64_t q_full, full[kMostPlaces], empty[kMostPlaces], rope_full[2], rope_empty[2], s_full[2], p_full[2], done,
+        out_free[2], meta_full[kAhead], meta_empty[kAhead];
+    uint64_t row[kAhead][kTile];  // where the tile's hot rows start, 0: no hot row
+    uint8_t kind[kAhead][kTile];  // of the tile's keys: kNone, kList, kDraft or kBadDraft
+    // 0 for a tile without any key, else 1 | lo << 8 | hi << 16: rows 4 lo .. 4 hi - 1 are drafted ones
+    uint32_t tile[kAhead];
     uint32_t tmem, stop;
 };
 enum : uint8_t { kNone = 0, kList = 1, kDraft = 2, kBadDraft = 3 };
@@ -171,6 +203,11 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool some)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16u : 0u) : "memory");
 }
+// An arrival of this thread once all its copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void copy_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
 __device__ __forceinline__ void copy_wait()
@@ -192,238 +229,424 @@ __device__ __forceinline__ bool not_finite(const uint4 &v)
 
 // ---- the rows ----------------------------------------------------------------------------------
 
-// This thread's share of a tile: unit `unit` (16 bytes) of the 128-byte columns of rows first + 32 j.
+// A place in the ring of groups and the parity of its use.
+template <int kPlaces>
+struct Ring {
+    uint32_t place = 0, turn = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++place == kPlaces) {
+            place = 0;
+            ++turn;
+        }
+    }
+};
+
+// The unit's queries, K-major in blocks of 64 dimensions, rows behind the last as zeros. Waits until
+// the scores of the last unit are done with their place; warp w takes rows w, w + 8, ...
+template <int NQ>
+__device__ __forceinline__ void load_queries(const KvopsAttend &a, const Plan &plan, Shared &sh, uint32_t q_at,
+                                             const Unit &u, uint32_t done, int warp, int lane)
+{
+    using namespace tc;
+    uint64_t from = 0;  // lane i: where row w + 8 i starts, 0: none
+    {
+        const uint32_t r = warp + kLoadWarps * lane, row = u.row0 + r;
+        if (r < u.rows) {
+            const uint32_t t = token_of(a, plan, u, row), h = plan.lists > 1 ? row : row - t * a.heads;
+            from = a.q + 2 * (u.req * a.q_stride_req + t * a.q_stride_token + h * a.q_stride_head);
+        }
+    }
+    if (done > 0) mbar_wait(smem_addr(&sh.s_full[(done - 1) & 1]), ((done - 1) >> 1) & 1, &sh.stop);
+#pragma unroll 4
+    for (int i = 0; i < NQ / kLoadWarps; ++i) {
+        const uint64_t row = __shfl_sync(0xFFFFFFFFu, from, i);
+        const uint32_t r = warp + kLoadWarps * i;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t c = k * 32 + lane;
+            if (c < 72)
+                copy16(q_at + (c >> 3) * (NQ * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                       reinterpret_cast<const uint8_t *>(row != 0 ? row + c * 16 : a.q), row != 0);
+        }
+    }
+    copies_arrive(smem_addr(&sh.q_full));
+}
+
+__device__ __forceinline__ const int32_t *list_of(const KvopsAttend &a, const Unit &u)
+{
+    return reinterpret_cast<const int32_t *>(a.topk_device_slots) + u.req * a.slots_stride_req +
+           u.token * a.slots_stride_token;
+}
+__device__ __forceinline__ const uint8_t *draft_row(const KvopsAttend &a, const Unit &u, uint32_t j)
+{
+    return reinterpret_cast<const uint8_t *>(a.draft_rows) + 2 * (u.req * a.draft_stride_req + j * a.draft_stride_row);
+}
+
+// 16 bytes of a drafted row. Not every query sees it: a value that is not finite would turn their
+// zero probability into NaN, so it is left out and the row marked.
+template <typename T>
+__device__ __forceinline__ uint4 draft_unit(const uint8_t *from, uint8_t *kind)
+{
+    uint4 v = *reinterpret_cast<const uint4 *>(from);
+    if (not_finite<T>(v)) {
+        v = make_uint4(0u, 0u, 0u, 0u);
+        *kind = kBadDraft;
+    }
+    return v;
+}
+
+// The rows of each tile, for the other warps: lane l looks at keys l and l + 32.
+template <int NQ, bool kStored>
+__device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan, Shared &sh, uint32_t begin, uint32_t end)
+{
+    using namespace tc;
+    constexpr uint32_t kRowBytes = kStored ? kStoredBytes : 2 * kKeyDim;
+    const int lane = threadIdx.x & 31;
+    uint32_t unit = begin / plan.tiles, tile = begin - unit * plan.tiles;  // the next to fetch
+    const int32_t *list = nullptr;
+    const int64_t *pool_at = nullptr;
+    const auto enter = [&]() {
+        const Unit u = unit_at<NQ>(plan, unit);
+        list = list_of(a, u);
+        pool_at = reinterpret_cast<const int64_t *>(a.req_pool_indices) + u.req;
+    };
+    // A tile on its way: its request's pool index and two slots, as they come from memory. Nothing is
+    // worked out of them before its turn: a warp stands still at the first use of a load.
+    struct Fetched {
+        int64_t pool;
+        int32_t slot[2];
+        uint32_t tile;
+    };
+    const auto fetch = [&]() {
+        Fetched f;
+        f.pool = -1;
+        if (a.top_k > 0) f.pool = *pool_at;
+        f.tile = tile;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t k = tile * kTile + lane + 32 * j;
+            f.slot[j] = -1;
+            if (k < a.top_k) f.slot[j] = list[k];
+        }
+        if (++tile == plan.tiles) {
+            tile = 0;
+            ++unit;
+            enter();
+        }
+        return f;
+    };
+    enter();
+    Fetched next[2];  // two tiles on their way
+    if (begin < end) next[0] = fetch();
+    if (begin + 1 < end) next[1] = fetch();
+    for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
+        const Fetched f = next[0];
+        next[0] = next[1];
+        if (at + 2 < end) next[1] = fetch();
+        const uint32_t buf = n % kAhead;
+        if (n >= kAhead) mbar_wait(smem_addr(&sh.meta_empty[buf]), (n / kAhead - 1) & 1, &sh.stop);
+        const bool in_pool = f.pool >= 0 && f.pool < static_cast<int64_t>(a.pool_size);
+        bool mine = false;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t k = f.tile * kTile + lane + 32 * j;
+            const bool listed = in_pool && f.slot[j] >= 0 && static_cast<uint32_t>(f.slot[j]) < a.hot_rows;
+            const bool drafted = k >= plan.list_end && k - plan.list_end < a.drafts;
+            sh.row[buf][lane + 32 * j] =
+                listed ? a.hot_row_base + (f.pool * a.hot_req_stride_rows + f.slot[j]) * kRowBytes : 0;
+            sh.kind[buf][lane + 32 * j] = listed ? kList : drafted ? kDraft : kNone;
+            mine |= listed || drafted;
+        }
+        const bool any = __any_sync(0xFFFFFFFFu, mine);
+        if (lane == 0) {
+            const uint32_t t0 = f.tile * kTile;
+            const uint32_t lo = plan.list_end <= t0 ? 0 : min(plan.list_end - t0, static_cast<uint32_t>(kTile));
+            const uint32_t till = plan.list_end + ((a.drafts + 3) & ~3u);
+            const uint32_t hi = a.drafts == 0 || till <= t0 ? lo : max(lo, min(till - t0, static_cast<uint32_t>(kTile)));
+            sh.tile[buf] = any ? 1u | (lo / 4) << 8 | (hi / 4) << 16 : 0u;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&sh.meta_full[buf]));
+    }
+}
+
+// The word of the n-th tile of the run, once it is known; and the end of its use.
+__device__ __forceinline__ uint32_t tile_word(Shared &sh, uint32_t n)
+{
+    tc::mbar_wait(tc::smem_addr(&sh.meta_full[n % kAhead]), (n / kAhead) & 1, &sh.stop);
+    return *const_cast<volatile uint32_t *>(&sh.tile[n % kAhead]);
+}
+__device__ __forceinline__ void tile_done(Shared &sh, uint32_t n, int lane)
+{
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(tc::smem_addr(&sh.meta_empty[n % kAhead]));
+}
+
+// Load warp w brings, of 16-bit rows, chunk w (64 dimensions) of all 64 rows; of stored rows, the codes
+// of group w / 2 of 32 rows, which it converts; and of either, the rotary dimensions of eight rows. Drafted rows,
+// whose first is at a multiple of four, come through registers.
 template <typename T, typename Code, bool kStored, int NQ>
 __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &plan, Shared &sh, uint32_t smem,
                                            uint32_t begin, uint32_t end)
 {
     using namespace tc;
-    const int tid = threadIdx.x - kSoftmaxWarps * 32, lane = tid & 31;
-    const uint32_t unit16 = tid & 7, first = tid >> 3;
-    const uint64_t row_bytes = kStored ? kStoredBytes : 2 * kKeyDim;
-    const uint32_t dst0 = smem + first * 128 + ((unit16 ^ (first & 7)) << 4);  // rows 32 apart swizzle alike
-    uint32_t done = 0, meta = 0;  // tiles with a key, tiles
-    uint32_t unit = begin / plan.tiles, tile = begin - unit * plan.tiles;
-    Unit u = unit_at<NQ>(a, plan, unit);
-
-    int32_t slot[4];
-    const uint8_t *hot = nullptr;
-    const auto fetch = [&]() {  // the slots of (u, tile), and where the request's hot rows are
-        const int32_t *list = reinterpret_cast<const int32_t *>(a.topk_device_slots) + u.req * a.slots_stride_req +
-                              u.token * a.slots_stride_token;
-        hot = nullptr;
-        if (a.top_k > 0) {
-            const int64_t pool = reinterpret_cast<const int64_t *>(a.req_pool_indices)[u.req];
-            if (pool >= 0 && pool < static_cast<int64_t>(a.pool_size))
-                hot = reinterpret_cast<const uint8_t *>(a.hot_row_base) + pool * a.hot_req_stride_rows * row_bytes;
-        }
+    using L = Layout<NQ, kStored>;
+    const int warp = (threadIdx.x >> 5) - kSoftmaxWarps, lane = threadIdx.x & 31;
+    const uint32_t group = warp >> 1, side = warp & 1, n16 = lane & 7, r4 = lane >> 3;
+    // Copies 128 bytes from byte `column` of kFours fours of rows (from `from` on, an even four) of tile n to
+    // `to`, four rows an instruction, leaving out the fours [lo, hi); rows that are none become zeros.
+    const auto copy = [&](auto fours, uint32_t n, int from, int lo, int hi, uint32_t to, uint32_t column) {
+        constexpr int kFours = decltype(fours)::value, kBatch = kFours < 8 ? kFours : 8;
+        const uint64_t *row = &sh.row[n % kAhead][4 * from + r4];
+        const uint64_t add = column + n16 * 16;
+        to += r4 * 128;
+        const uint32_t even = (n16 ^ r4) << 4, odd = (n16 ^ (r4 + 4)) << 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t k = tile * kTile + first + 32 * j;
-            slot[j] = k < a.top_k ? list[k] : -1;
+        for (int b = 0; b < kFours; b += kBatch) {
+            uint64_t at[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) at[i] = row[4 * (b + i)];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const bool some = at[i] != 0, skip = from + b + i >= lo && from + b + i < hi;
+                if (!skip)
+                    copy16(to + (b + i) * 512 + ((b + i) & 1 ? odd : even),
+                           reinterpret_cast<const uint8_t *>(some ? at[i] + add : a.q), some);
+            }
         }
     };
-    if (begin < end) fetch();
-    bool q_loaded = false;
-    for (uint32_t at = begin; at < end; ++at) {
-        const Unit now = u;
-        const uint32_t now_tile = tile;
-        const uint8_t *row[4];
-        uint8_t kind[4];
-        bool mine = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t k = now_tile * kTile + first + 32 * j;
-            row[j] = nullptr;
-            kind[j] = kNone;
-            if (k < a.top_k) {
-                if (hot != nullptr && slot[j] >= 0 && static_cast<uint32_t>(slot[j]) < a.hot_rows) {
-                    row[j] = hot + static_cast<uint32_t>(slot[j]) * row_bytes;
-                    kind[j] = kList;
-                }
-            } else if (k < a.top_k + a.drafts) {
-                row[j] = reinterpret_cast<const uint8_t *>(a.draft_rows) +
-                         2 * (now.req * a.draft_stride_req + (k - a.top_k) * a.draft_stride_row);
-                kind[j] = kDraft;
-            }
-            mine |= kind[j] != kNone;
-        }
-        const uint32_t buf = meta & 1;
-        if (meta >= 2) mbar_wait(smem_addr(&sh.meta_empty[buf]), ((meta >> 1) - 1) & 1, &sh.stop);
-        if (unit16 == 0) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sh.kind[buf][first + 32 * j] = kind[j];
-        }
-        const bool any = group_any(4, kLoadWarps * 32, mine);
-        if (tid == 0) {
-            sh.any[buf] = any;
-            mbar_arrive(smem_addr(&sh.meta_full[buf]));
-        }
-        ++meta;
-        // the next tile's slots travel while this tile's rows do
-        const bool last = at + 1 == end || tile + 1 == plan.tiles;
-        if (++tile == plan.tiles) {
-            tile = 0;
-            ++unit;
-            if (at + 1 < end) u = unit_at<NQ>(a, plan, unit);
-        }
-        if (at + 1 < end) fetch();
-        if (any) {
-            // Codes wait in registers for their place in shared memory: three groups of the four (a
-            // fourth would not fit), the last one following the first.
-            uint4 code[kStored ? 3 : 1][4];
-            float scale[kStored ? 3 : 1][4];
-            const auto stage = [&](int g) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    scale[g % 3][j] = 0.f;
-                    code[g % 3][j] = make_uint4(0u, 0u, 0u, 0u);
-                    if (kind[j] == kList) {
-                        scale[g % 3][j] = __ldg(reinterpret_cast<const float *>(row[j] + kValueDim) + g);
-                        code[g % 3][j] = __ldcs(reinterpret_cast<const uint4 *>(row[j] + g * 128) + unit16);
-                    }
-                }
-            };
-            if constexpr (kStored) {
-                stage(0);
-                stage(1);
-                stage(2);
-            }
-            const uint32_t freed = (done - 1) & 1;
-            if (!q_loaded) {
-                // the queries' place is free once the last unit's products are done
-                if (done > 0) mbar_wait(smem_addr(&sh.empty[kGroups - 1]), freed, &sh.stop);
-                for (uint32_t i = tid; i < NQ * 72; i += kLoadWarps * 32) {
-                    const uint32_t r = i / 72, c = i - r * 72;
-                    const uint32_t q_row = now.row0 + r;
-                    const uint32_t t = token_of(a, plan, now, q_row);
-                    const uint32_t h = plan.lists > 1 ? q_row : q_row - t * a.heads;
-                    const bool some = r < now.rows;
-                    const uint8_t *src = reinterpret_cast<const uint8_t *>(a.q);
-                    if (some)
-                        src += 2 * (now.req * a.q_stride_req + t * a.q_stride_token + h * a.q_stride_head) + c * 16;
-                    copy16(smem + Layout<NQ>::q + (c >> 3) * (NQ * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, some);
-                }
-            }
+    // Every lane's arrival, after its copies and (if any) the drafted rows that it stored itself.
+    const auto arrive = [&](uint64_t *bar, bool stored_some) {
+        if (stored_some) {
             copy_close();
+            copy_wait<0>();
+            fence_async_shared();
+            mbar_arrive(smem_addr(bar));
+        } else {
+            copies_arrive(smem_addr(bar));
+        }
+    };
+    const uint32_t stage = smem + L::stage + warp * (32 * 128);
+    float next_scale = 0.f;  // stored: of row 32 side + lane, group `group`, of the codes on their way
+    const auto send = [&](uint32_t n, int lo, int hi) {  // the codes of this warp's rows of tile n, and their scales
+        const uint64_t mine = sh.row[n % kAhead][side * 32 + lane];
+        next_scale = 0.f;
+        if (mine != 0) next_scale = __ldg(reinterpret_cast<const float *>(mine + kValueDim) + group);
+        copy(std::integral_constant<int, 8>(), n, side * 8, lo, hi, stage, group * 128);
+        copy_close();
+    };
+
+    uint32_t unit = begin / plan.tiles, tile = begin - unit * plan.tiles, done = 0;
+    Unit u = unit_at<NQ>(plan, unit);
+    Ring<L::places> ring;  // of group 0 of the tile
+    bool q_loaded = false, sent = false;  // sent: the tile's codes are on their way
+    uint32_t ends0 = 0, ends1 = 0;        // units that ended in a tile of an even number, of an odd one
+    for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
+        const uint32_t word = tile_word(sh, n);
+        if (word != 0) {
+            const int lo = word >> 8 & 0xFF, hi = word >> 16;
+            const bool first = !q_loaded;
+            q_loaded = true;
+            // Drafted rows' values from 64 * chunk on, of the fours from .. till; zeros behind the last row.
+            const auto bring_drafts = [&](uint32_t to, uint32_t chunk, uint32_t chunks, int from, int till) {
+                for (uint32_t i = 4 * from * chunks * 8 + lane; i < 4 * till * chunks * 8; i += 32) {
+                    const uint32_t c16 = i & 7, c = chunks == 2 ? i >> 3 & 1 : 0, r = chunks == 2 ? i >> 4 : i >> 3;
+                    const uint32_t j = tile * kTile + r - plan.list_end;
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (j < a.drafts)
+                        v = draft_unit<T>(draft_row(a, u, j) + (chunk + c) * 128 + c16 * 16, &sh.kind[n % kAhead][r]);
+                    store16(to + c * kChunkBytes + r * 128 + ((c16 ^ (r & 7)) << 4), v);
+                }
+            };
+            const auto bring_rope = [&]() {
+                // the place was the probabilities' of the tile before last, and perhaps its unit's outputs'
+                const uint32_t half = done & 1, rope = smem + L::rope + half * kChunkBytes;
+                if (done > 1) mbar_wait(smem_addr(&sh.rope_empty[half]), ((done >> 1) - 1) & 1, &sh.stop);
+                const uint32_t ends = half ? ends1 : ends0;
+                if (ends > 0) mbar_wait(smem_addr(&sh.out_free[half]), (ends - 1) & 1, &sh.stop);
+                copy(std::integral_constant<int, 2>(), n, 2 * warp, lo, hi, rope + warp * 1024,
+                     kStored ? kStoredPlain : 2 * kValueDim);
+                const int from = max(lo, 2 * warp), till = min(hi, 2 * warp + 2);
+                bring_drafts(rope, 8, 1, from, till);
+                arrive(&sh.rope_full[half], from < till);
+            };
+            // this warp's group and its place
+            uint32_t place = ring.place + group, turn = ring.turn;
+            if (place >= L::places) {
+                place -= L::places;
+                ++turn;
+            }
+            uint64_t *full = &sh.full[place];
+            if constexpr (kStored) {
+                if (!sent) send(n, lo, hi);
+                if (first) load_queries<NQ>(a, plan, sh, smem + L::q, u, done, warp, lane);
+                copy_wait<0>();
+                __syncwarp();
+                uint4 code[8];
+                const uint32_t r = side * 32 + lane;
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                if (done > 0) mbar_wait(smem_addr(&sh.empty[g]), freed, &sh.stop);
+                for (int i = 0; i < 8; ++i)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(code[i].x), "=r"(code[i].y), "=r"(code[i].z), "=r"(code[i].w)
+                                 : "r"(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) : "memory");
+                const float scale = next_scale;
+                __syncwarp();
+                bring_rope();  // ahead of the codes, whose landing its arrival would wait for as well
+                sent = false;
+                if (at + 1 < end) {  // the next tile's, into the place that was just read
+                    const uint32_t w = tile_word(sh, n + 1);
+                    sent = w != 0;
+                    if (sent) send(n + 1, w >> 8 & 0xFF, w >> 16);
+                }
+                if (turn > 0) mbar_wait(smem_addr(&sh.empty[place]), (turn - 1) & 1, &sh.stop);
+                const uint32_t to = smem + place * kGroupBytes;
+                const int from = max(lo, static_cast<int>(side) * 8), till = min(hi, static_cast<int>(side) * 8 + 8);
+                if (!(static_cast<int>(r >> 2) >= lo && static_cast<int>(r >> 2) < hi)) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t dst = dst0 + 2 * g * kChunkBytes + j * 32 * 128;
-                    if (kind[j] == kDraft) {
-                        // Rows that not every query sees: a value that is not finite would turn
-                        // their zero probability into NaN, so it is left out and the row marked.
-#pragma unroll
-                        for (int c = 0; c < (g < 4 ? 2 : 1); ++c) {
-                            uint4 v = *reinterpret_cast<const uint4 *>(row[j] + (2 * g + c) * 128 + unit16 * 16);
-                            if (not_finite<T>(v)) {
-                                v = make_uint4(0u, 0u, 0u, 0u);
-                                sh.kind[buf][first + 32 * j] = kBadDraft;
-                            }
-                            store16(dst + c * kChunkBytes, v);
-                        }
-                    } else if (!kStored || g == 4) {
-                        const uint8_t *src = kind[j] == kList ? row[j] : reinterpret_cast<const uint8_t *>(a.q);
-                        if (kind[j] == kList)
-                            src += (kStored ? kStoredPlain : 2 * g * 128) + unit16 * 16;
-                        copy16(dst, src, kind[j] == kList);
-                        if (g < 4) copy16(dst + kChunkBytes, src + (kind[j] == kList ? 128 : 0), kind[j] == kList);
-                    } else if constexpr (kStored) {
-                        // 16 codes: units 2 u and 2 u + 1 of the group's 16 (u = unit16)
-                        const float s = scale[g % 3][j];
-                        const uint4 c = code[g % 3][j];
-                        const uint32_t r = first + 32 * j, to = smem + (2 * g + (unit16 >> 2)) * kChunkBytes + r * 128;
-                        const uint32_t n = (unit16 & 3) * 2;
-                        store16(to + ((n ^ (r & 7)) << 4), decode_unit<T, Code>(make_uint2(c.x, c.y), s));
-                        store16(to + (((n + 1) ^ (r & 7)) << 4), decode_unit<T, Code>(make_uint2(c.z, c.w), s));
+                    for (int i = 0; i < 16; ++i) {
+                        const uint4 &w = code[i >> 1];
+                        store16(to + (i >> 3) * kChunkBytes + r * 128 + (((i & 7) ^ (r & 7)) << 4),
+                                decode_unit<T, Code>(i & 1 ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), scale));
                     }
                 }
-                copy_close();
-                if constexpr (kStored) {
-                    if (g == 0) stage(3);
-                }
-            }
-            const auto hand_over = [&](uint64_t *bar) {
+                bring_drafts(to, 2 * group, 2, from, till);
                 fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(bar));
-            };
-            copy_wait<5>();
-            if (!q_loaded) hand_over(&sh.q_full);
-            q_loaded = true;
-            copy_wait<4>();
-            hand_over(&sh.full[0]);
-            copy_wait<3>();
-            hand_over(&sh.full[1]);
-            copy_wait<2>();
-            hand_over(&sh.full[2]);
-            copy_wait<1>();
-            hand_over(&sh.full[3]);
-            copy_wait<0>();
-            hand_over(&sh.full[4]);
+                mbar_arrive(smem_addr(full));
+            } else {
+                if (first) load_queries<NQ>(a, plan, sh, smem + L::q, u, done, warp, lane);
+                if (turn > 0) mbar_wait(smem_addr(&sh.empty[place]), (turn - 1) & 1, &sh.stop);
+                const uint32_t to = smem + place * kGroupBytes + side * kChunkBytes;
+                copy(std::integral_constant<int, kTile / 4>(), n, 0, lo, hi, to, warp * 128);
+                bring_drafts(to, warp, 1, lo, hi);
+                arrive(full, lo < hi);
+                bring_rope();
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ring.next();
             ++done;
         }
-        if (last) q_loaded = false;
+        tile_done(sh, n, lane);
+        const bool wraps = tile + 1 == plan.tiles;
+        if (wraps || at + 1 == end) {
+            // a unit's outputs go through the place of its last tile's probabilities
+            if (q_loaded) ++(done & 1 ? ends0 : ends1);
+            q_loaded = false;
+        }
+        ++tile;
+        if (wraps) {
+            tile = 0;
+            u = unit_at<NQ>(plan, ++unit);
+        }
     }
+    copy_close();
+    copy_wait<0>();
 }
 
 // ---- the products ------------------------------------------------------------------------------
 
-template <typename T, int NQ>
-__device__ __forceinline__ void product_thread(const Plan &plan, Shared &sh, uint32_t smem, uint32_t begin, uint32_t end)
+// A product warp's walk over the tiles: body(starts) for each one with a key, `starts` telling whether
+// it is the first of its unit.
+template <typename Body>
+__device__ __forceinline__ void each_tile(const Plan &plan, Shared &sh, uint32_t begin, uint32_t end, const Body &body)
 {
     using namespace tc;
-    constexpr uint32_t type = std::is_same<T, Bf16>::value ? 1u : 0u;
-    constexpr uint32_t score = instruction(type, false, 128, NQ), weigh = instruction(type, true, 128, NQ);
-    const uint32_t s_at = sh.tmem, o_at = sh.tmem + NQ;
-    uint32_t done = 0, units = 0, tile = begin % plan.tiles;
-    bool started = false;  // this unit's part has outputs in tensor memory
-    for (uint32_t at = begin, meta = 0; at < end; ++at, ++meta) {
-        const uint32_t buf = meta & 1;
-        mbar_wait(smem_addr(&sh.meta_full[buf]), (meta >> 1) & 1, &sh.stop);
-        const bool any = *const_cast<volatile uint32_t *>(&sh.any[buf]) != 0;
-        mbar_arrive(smem_addr(&sh.meta_empty[buf]));
-        if (any) {
-            if (!started) mbar_wait(smem_addr(&sh.q_full), units++ & 1, &sh.stop);
-#pragma unroll 1
-            for (int g = 0; g < kGroups; ++g) {
-                mbar_wait(smem_addr(&sh.full[g]), done & 1, &sh.stop);
-                fence_after_sync();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (g == 4 && i >= 4) break;
-                    const int c = 2 * g + i / 4;
-                    mma(s_at, operand(smem + c * kChunkBytes + (i & 3) * 32, 16, 1024),
-                        operand(smem + Layout<NQ>::q + c * (NQ * 128) + (i & 3) * 32, 16, 1024), score, g > 0 || i > 0);
-                }
-            }
-            commit(smem_addr(&sh.s_full));
-            mbar_wait(smem_addr(&sh.p_full), done & 1, &sh.stop);
-            fence_after_sync();
-#pragma unroll 1
-            for (int b = 0; b < 4; ++b) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    mma(o_at + b * NQ, operand(smem + 2 * b * kChunkBytes + i * 2048, kChunkBytes, 1024),
-                        operand(smem + Layout<NQ>::p + i * 2048, 16, 1024), weigh, started || i > 0);
-                commit(smem_addr(&sh.empty[b]));
-            }
-            commit(smem_addr(&sh.empty[kGroups - 1]));
-            started = true;
-            ++done;
-        }
+    uint32_t tile = begin % plan.tiles;
+    bool starts = true;
+    const int lane = threadIdx.x & 31;
+    for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
+        const bool any = __shfl_sync(0xFFFFFFFFu, tile_word(sh, n), 0) != 0;
+        tile_done(sh, n, lane);
+        if (any) body(starts);
+        starts = !any && starts;
         if (++tile == plan.tiles) {
             tile = 0;
-            started = false;
+            starts = true;
         }
     }
 }
 
+template <typename T>
+constexpr uint32_t kType = std::is_same<T, Bf16>::value ? 1u : 0u;
+
+// The first product of each tile, as soon as its rows are there and the scores of the tile before
+// last have been read. (A warp of its own: one that issued both products would do the second only
+// after the next tile's rows, since a look at a barrier that is not there yet takes until it is.)
+template <typename T, bool kStored, int NQ>
+__device__ __forceinline__ void score_warp(const Plan &plan, Shared &sh, uint32_t smem, uint32_t begin, uint32_t end)
+{
+    using namespace tc;
+    using L = Layout<NQ, kStored>;
+    constexpr uint32_t inst = instruction(kType<T>, false, kTile, NQ);
+    const uint32_t elected = elect(), tmem = __shfl_sync(0xFFFFFFFFu, sh.tmem, 0);
+    // operands at their start; a descriptor counts addresses in units of 16 bytes
+    const uint64_t keys0 = operand(smem, 16, 1024), queries = operand(smem + L::q, 16, 1024);
+    const uint64_t rotary0 = operand(smem + L::rope, 16, 1024);
+    Ring<L::places> in;
+    uint32_t n = 0, units = 0;
+    each_tile(plan, sh, begin, end, [&](bool starts) {
+        const uint32_t buf = n & 1, s_at = tmem + buf * NQ;
+        if (starts) mbar_wait(smem_addr(&sh.q_full), units++ & 1, &sh.stop);
+        if (n > 1) mbar_wait(smem_addr(&sh.p_full[buf]), ((n >> 1) - 1) & 1, &sh.stop);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            mbar_wait(smem_addr(&sh.full[in.place]), in.turn & 1, &sh.stop);
+            fence_async_shared();  // what the copies wrote
+            fence_after_sync();
+            const uint64_t keys = keys0 + in.place * (kGroupBytes >> 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                mma(elected, s_at, keys + ((i / 4 * kChunkBytes + (i & 3) * 32) >> 4),
+                    queries + (((2 * g + i / 4) * (NQ * 128) + (i & 3) * 32) >> 4), inst, g > 0 || i > 0);
+            in.next();
+        }
+        mbar_wait(smem_addr(&sh.rope_full[buf]), (n >> 1) & 1, &sh.stop);
+        fence_async_shared();
+        fence_after_sync();
+        const uint64_t rotary = rotary0 + buf * (kChunkBytes >> 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            mma(elected, s_at, rotary + ((i * 32) >> 4), queries + ((8 * (NQ * 128) + i * 32) >> 4), inst, true);
+        commit(elected, smem_addr(&sh.s_full[buf]));
+        ++n;
+    });
+}
+
+// The second product of each tile, as soon as its probabilities are there.
+template <typename T, bool kStored, int NQ>
+__device__ __forceinline__ void weigh_warp(const Plan &plan, Shared &sh, uint32_t smem, uint32_t begin, uint32_t end)
+{
+    using namespace tc;
+    using L = Layout<NQ, kStored>;
+    constexpr uint32_t inst = instruction(kType<T>, true, 128, NQ);
+    const uint32_t elected = elect(), o_at = __shfl_sync(0xFFFFFFFFu, sh.tmem, 0) + 2 * NQ;
+    const uint64_t values0 = operand(smem, kChunkBytes, 1024), probs0 = operand(smem + L::rope, 16, 1024);
+    Ring<L::places> out;
+    uint32_t n = 0;
+    each_tile(plan, sh, begin, end, [&](bool starts) {
+        const uint32_t buf = n & 1;
+        mbar_wait(smem_addr(&sh.p_full[buf]), (n >> 1) & 1, &sh.stop);
+        fence_async_shared();
+        fence_after_sync();
+        const uint64_t probs = probs0 + buf * (kChunkBytes >> 4);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const uint64_t values = values0 + out.place * (kGroupBytes >> 4);
+#pragma unroll
+            for (int i = 0; i < kTile / 16; ++i)
+                mma(elected, o_at + b * NQ, values + ((i * 2048) >> 4), probs + ((i * 2048) >> 4), inst, !starts || i > 0);
+            commit(elected, smem_addr(&sh.empty[out.place]));
+            out.next();
+        }
+        commit(elected, smem_addr(&sh.rope_empty[buf]));
+        commit(elected, smem_addr(&sh.done));
+        ++n;
+    });
+}
+
 // ---- the softmax and the outputs ---------------------------------------------------------------
 
-template <typename T, int NQ>
+template <typename T, bool kStored, int NQ>
 __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &plan, Shared &sh, uint32_t smem,
                                               uint32_t begin, uint32_t end)
 {
@@ -431,9 +654,12 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
     constexpr int NH = NQ / 2;  // queries of a thread
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quarter = warp & 3, half = warp >> 2;
-    const int key = quarter * 32 + lane;  // this thread's row of the tile
+    // The scores of 64 keys lie in lanes 0-15 of each quarter: lanes 16-31 have no key, but their share of
+    // the outputs' dimensions.
+    const int key = quarter * 16 + (lane & 15), dim = quarter * 32 + lane;
+    const bool keyed = lane < 16;
     const uint32_t lanes = static_cast<uint32_t>(quarter) << 21;
-    const uint32_t s_at = sh.tmem + lanes + half * NH, o_at = sh.tmem + lanes + NQ + half * NH;
+    const uint32_t s_at = sh.tmem + lanes + half * NH, o_at = s_at + 2 * NQ;
     const float factor = a.scale * 1.4426950408889634f;  // scores as powers of two
     float *mine = sh.per_warp[warp];
     const auto spread = [&](float x) {  // column c's x, held by lane c, to be read by every lane
@@ -449,7 +675,7 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
         return f;
     };
     uint32_t done = 0, unit = begin / plan.tiles, tile = begin - unit * plan.tiles, start_tile = tile;
-    bool fresh = true, started = false;
+    bool fresh = true, started = false, open = false;
     Unit u{};
     float ref = -INFINITY;  // of column `lane` of this half
     float sum[NH];          // of this thread's keys, by column
@@ -457,7 +683,7 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
         if (fresh) {
             fresh = started = false;
             start_tile = tile;
-            u = unit_at<NQ>(a, plan, unit);
+            u = unit_at<NQ>(plan, unit);
             ref = -INFINITY;
 #pragma unroll
             for (int i = 0; i < NH; ++i) sum[i] = 0.f;
@@ -471,49 +697,86 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 group_barrier(3, kSoftmaxWarps * 32);
             }
         }
-        const uint32_t buf = meta & 1;
-        mbar_wait(smem_addr(&sh.meta_full[buf]), (meta >> 1) & 1, &sh.stop);
+        const uint32_t word = tile_word(sh, meta);
         // (through a barrier: after a wait has given up, too, the warps of a half must agree)
-        const bool any = group_any(1 + half, 128, *const_cast<volatile uint32_t *>(&sh.any[buf]) != 0);
+        const bool any = group_any(1 + half, 128, word != 0);
         if (any) {
-            mbar_wait(smem_addr(&sh.s_full), done & 1, &sh.stop);
+            mbar_wait(smem_addr(&sh.s_full[done & 1]), (done >> 1) & 1, &sh.stop);
             fence_after_sync();
         }
-        const uint8_t kind = *const_cast<volatile uint8_t *>(&sh.kind[buf][key]);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&sh.meta_empty[buf]));
+        const uint8_t kind = keyed ? *const_cast<volatile uint8_t *>(&sh.kind[meta % kAhead][key]) : kNone;
+        tile_done(sh, meta, lane);
         if (any) {
-            float x[NH];
-            tmem_load<NH>(s_at, x);
+            float y[NH];  // the scores in powers of two, then less their references, then probabilities
+            const auto scores = [&]() {
+                tmem_load<NH>(s_at + (done & 1) * NQ, y);
 #pragma unroll
-            for (int i = 0; i < NH; ++i) x[i] = kind == kNone ? -INFINITY : x[i] * factor;
-            if (kind >= kDraft) {
-                const uint32_t j = tile * kTile + key - a.top_k;
+                for (int i = 0; i < NH; ++i) y[i] = kind == kNone ? -INFINITY : y[i] * factor;
+                if (kind >= kDraft) {
+                    const uint32_t j = tile * kTile + key - plan.list_end;
+#pragma unroll
+                    for (int i = 0; i < NH; ++i) {
+                        const bool sees = (sh.tree[half * NH + i] >> j) & 1;
+                        if (!sees) y[i] = -INFINITY;
+                        else if (kind == kBadDraft) y[i] = NAN;
+                    }
+                }
+            };
+            const auto lower = [&]() {  // by the references, which the warp keeps spread; their largest excess
+                float excess = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NH; i += 4) {
+                    const float4 r = spread4(i);
+                    y[i] -= r.x, y[i + 1] -= r.y, y[i + 2] -= r.z, y[i + 3] -= r.w;
+                    excess = fmaxf(excess, fmaxf(fmaxf(y[i], y[i + 1]), fmaxf(y[i + 2], y[i + 3])));
+                }
+                return excess;
+            };
+            const auto write = [&]() {  // the probabilities, to where the second product reads them
+                const uint32_t to = smem + Layout<NQ, kStored>::rope + (done & 1) * kChunkBytes + key * 128;
+#pragma unroll
+                for (int i = 0; i < NH; i += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int c = i + 2 * k;
+                        y[c] = exp2_fast(y[c]);
+                        y[c + 1] = exp2_fast(y[c + 1]);
+                        w[k] = T::pack(y[c], y[c + 1]);
+                    }
+                    if (keyed)
+                        store16(to + ((((half * NH + i) >> 3) ^ (key & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                }
+            };
+            scores();
+            bool move_all = !started;
+            if (started) {
+                // The references only have to move when a score passes one by kLift + kSlack, which each
+                // thread's largest excess tells. The probabilities are worked out as if none had, so that
+                // the warps need not wait for one another before, and again in the rare tile where one has.
+                const float excess = lower();
+                write();
+                move_all = group_any(1 + half, 128, excess > kLift + kSlack || (open && excess > -INFINITY));
+                if (move_all) scores();
+            }
+            if (move_all) {
+                float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < NH; ++i) {
-                    const bool sees = (sh.tree[half * NH + i] >> j) & 1;
-                    if (!sees) x[i] = -INFINITY;
-                    else if (kind == kBadDraft) x[i] = NAN;
+                    const float m = warp_max(y[i]);
+                    if (lane == i) top = m;
                 }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < NH; ++i) {
-                const float m = warp_max(x[i]);
-                if (lane == i) top = m;
-            }
-            sh.top[half][quarter][lane] = top;
-            group_barrier(1 + half, 128);
-            top = fmaxf(fmaxf(sh.top[half][0][lane], sh.top[half][1][lane]),
-                        fmaxf(sh.top[half][2][lane], sh.top[half][3][lane]));
-            // the same decision in the four warps of this half
-            const bool move = top > ref + (kLift + kSlack) || (ref == -INFINITY && top > -INFINITY);
-            if (__any_sync(0xFFFFFFFFu, move)) {
+                sh.top[half][quarter][lane] = top;
+                group_barrier(1 + half, 128);
+                // the same decision in the four warps of this half
+                top = fmaxf(fmaxf(sh.top[half][0][lane], sh.top[half][1][lane]),
+                            fmaxf(sh.top[half][2][lane], sh.top[half][3][lane]));
+                const bool move = top > ref + (kLift + kSlack) || (ref == -INFINITY && top > -INFINITY);
                 const float was = ref;
                 if (move) ref = top - kLift;
-                if (started) {
+                if (started && __any_sync(0xFFFFFFFFu, move)) {
                     spread(move ? exp2_fast(was - ref) : 1.f);
-                    mbar_wait(smem_addr(&sh.empty[kGroups - 1]), (done - 1) & 1, &sh.stop);
+                    mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
                     fence_after_sync();
 #pragma unroll
                     for (int i = 0; i < NH; i += 4) {
@@ -532,28 +795,21 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                         tmem_store<8>(o, v);
                     }
                 }
+                spread(ref == -INFINITY ? 0.f : ref);
+                // a column without any key so far: its first finite score moves its reference
+                open = __any_sync(0xFFFFFFFFu, lane < NH && ref == -INFINITY);
+                lower();
+                write();
             }
-            spread(ref == -INFINITY ? 0.f : ref);
-            const uint32_t to = smem + Layout<NQ>::p + key * 128;
 #pragma unroll
-            for (int i = 0; i < NH; i += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int k = 0; k < 4; k += 2) {
-                    const int c = i + 2 * k;
-                    const float4 r = spread4(c);
-                    const float p0 = exp2_fast(x[c] - r.x), p1 = exp2_fast(x[c + 1] - r.y);
-                    const float p2 = exp2_fast(x[c + 2] - r.z), p3 = exp2_fast(x[c + 3] - r.w);
-                    sum[c] += p0, sum[c + 1] += p1, sum[c + 2] += p2, sum[c + 3] += p3;
-                    w[k] = T::pack(p0, p1);
-                    w[k + 1] = T::pack(p2, p3);
-                }
-                store16(to + ((((half * NH + i) >> 3) ^ (key & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
-            }
+            for (int i = 0; i < NH; ++i) sum[i] += y[i];
+            // Every tile's end is waited for in its turn, since a parity only tells a phase from its
+            // neighbours. This one was reached before the next tile's first product, as a rule.
+            if (done > 0) mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
             fence_async_shared();
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&sh.p_full));
+            if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[done & 1]));
             started = true;
             ++done;
         }
@@ -568,7 +824,6 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
             // every warp adds the quarters in the same order
             total = (sh.top[half][0][lane & (NH - 1)] + sh.top[half][1][lane & (NH - 1)]) +
                     (sh.top[half][2][lane & (NH - 1)] + sh.top[half][3][lane & (NH - 1)]);
-            group_barrier(1 + half, 128);
             const uint32_t col = half * NH + lane;
             if (lane < NH && quarter == 0 && col < u.rows) {
                 if (!complete)
@@ -577,31 +832,72 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                     reinterpret_cast<float *>(a.lse)[u.out_row + col] =
                         total == 0.f ? -INFINITY : (ref + log2f(total)) * 0.6931471805599453f;
             }
-            spread(complete ? (total == 0.f ? 0.f : 1.f / total) : 1.f);
+            spread(total == 0.f ? 0.f : 1.f / total);
             if (started) {
-                mbar_wait(smem_addr(&sh.empty[kGroups - 1]), (done - 1) & 1, &sh.stop);
+                mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
                 fence_after_sync();
             }
+            // 16 queries of 128 dimensions at a time (8, where a half has no more).
+            constexpr int kRows = NH < 16 ? NH : 16;
+            // The last probabilities' place turns [dimension][query] into rows of 128 dimensions (256
+            // bytes; odd rows with their halves swapped in each 128 bytes, to keep the two rows that a
+            // pair of lanes writes in different banks).
+            const uint32_t place = (done - 1) & 1;
+            const uint32_t rows = smem + Layout<NQ, kStored>::rope + place * kChunkBytes + half * kRows * 256;
 #pragma unroll 1
-            for (int b = 0; b < 4 * NH / 8; ++b) {
-                const int i = b % (NH / 8) * 8;
-                const uint32_t dim = b / (NH / 8) * 128 + key, c = half * NH + i;
-                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (started) tmem_load<8>(o_at + b / (NH / 8) * NQ + i, v);
-                const float4 f = spread4(i), g = spread4(i + 4);
-                v[0] *= f.x, v[1] *= f.y, v[2] *= f.z, v[3] *= f.w;
-                v[4] *= g.x, v[5] *= g.y, v[6] *= g.z, v[7] *= g.w;
+            for (int b = 0; b < 4 * NH / kRows; ++b) {
+                const uint32_t block = b / (NH / kRows), first = b % (NH / kRows) * kRows;  // of the half's queries
+                float v[kRows];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    if (c + k >= u.rows) break;
-                    if (complete)
-                        reinterpret_cast<uint16_t *>(a.out)[(u.out_row + c + k) * kValueDim + dim] =
-                            static_cast<uint16_t>(T::pack(v[k], 0.f));
-                    else
-                        plan.part_o[(static_cast<uint64_t>(slot) * NQ + c + k) * kValueDim + dim] = v[k];
+                for (int i = 0; i < kRows; ++i) v[i] = 0.f;
+                if (started) tmem_load<kRows>(o_at + block * NQ + first, v);
+                if (!complete) {
+                    float4 *to = reinterpret_cast<float4 *>(plan.part_o);
+#pragma unroll
+                    for (int i = 0; i < kRows; i += 4)
+                        to[part_at<NQ>(slot, block, quarter, half, (first + i) / 4, lane)] =
+                            make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    continue;
+                }
+                const uint32_t r0 = half * NH + first;
+                if (!started) {  // no keys at all
+                    for (int i = 0; i < kRows; ++i)
+                        if (r0 + i < u.rows)
+                            reinterpret_cast<uint16_t *>(a.out)[(u.out_row + r0 + i) * kValueDim + block * 128 + dim] = 0;
+                    continue;
+                }
+                group_barrier(1 + half, 128);
+#pragma unroll
+                for (int i = 0; i < kRows; i += 4) {
+                    const float4 f = spread4(first + i);
+                    v[i] *= f.x, v[i + 1] *= f.y, v[i + 2] *= f.z, v[i + 3] *= f.w;
+#pragma unroll
+                    for (int c = i; c < i + 4; c += 2) {
+                        // an even lane takes query c of its dimension and the next, an odd one c + 1
+                        const bool odd = lane & 1;
+                        const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[c] : v[c + 1], 1);
+                        const uint32_t w = odd ? T::pack(other, v[c + 1]) : T::pack(v[c], other);
+                        const uint32_t r = c + odd, word = dim >> 1;
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows + r * 256 + ((word ^ (odd ? 16 : 0)) << 2)), "r"(w)
+                                     : "memory");
+                    }
+                }
+                group_barrier(1 + half, 128);
+#pragma unroll
+                for (int i = 0; i < kRows / 8; ++i) {
+                    const uint32_t n = i * 128 + dim, r = n >> 4, q = n & 15;
+                    uint4 w;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                 : "r"(rows + r * 256 + ((q ^ ((r & 1) << 2)) << 4)) : "memory");
+                    if (r0 + r < u.rows)
+                        reinterpret_cast<uint4 *>(a.out)[(u.out_row + r0 + r) * (kValueDim / 8) + block * 16 + q] = w;
                 }
             }
+            group_barrier(1 + half, 128);
             fence_before_sync();
+            fence_async_shared();
+            __syncwarp();
+            if (started && lane == 0) mbar_arrive(smem_addr(&sh.out_free[place]));
             fresh = true;
         }
         if (++tile == plan.tiles) {
@@ -612,29 +908,37 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
 }
 
 template <typename T, typename Code, bool kStored, int NQ>
-__global__ void __launch_bounds__(kThreads, 1) attend_kernel(const KvopsAttend a, const Plan plan)
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(const KvopsAttend a, const Plan plan)
 {
     using namespace tc;
     extern __shared__ uint8_t dynamic[];
     __shared__ Shared sh;
     const uint32_t smem = (smem_addr(dynamic) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // join_kernel may take its seats and wait
     if (threadIdx.x == 0) {
         sh.stop = 0;
-        mbar_init(smem_addr(&sh.q_full), kLoadWarps);
-        for (int g = 0; g < kGroups; ++g) {
-            mbar_init(smem_addr(&sh.full[g]), kLoadWarps);
+        mbar_init(smem_addr(&sh.q_full), kLoadWarps * 32);
+        for (int g = 0; g < kMostPlaces; ++g) {
+            mbar_init(smem_addr(&sh.full[g]), 2 * 32);
             mbar_init(smem_addr(&sh.empty[g]), 1);
         }
-        mbar_init(smem_addr(&sh.s_full), 1);
-        mbar_init(smem_addr(&sh.p_full), kSoftmaxWarps);
+        mbar_init(smem_addr(&sh.done), 1);
         for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_addr(&sh.rope_full[b]), kLoadWarps * 32);
+            mbar_init(smem_addr(&sh.rope_empty[b]), 1);
+            mbar_init(smem_addr(&sh.s_full[b]), 1);
+            mbar_init(smem_addr(&sh.p_full[b]), kSoftmaxWarps);
+            mbar_init(smem_addr(&sh.out_free[b]), kSoftmaxWarps);
+        }
+        for (uint32_t b = 0; b < kAhead; ++b) {
             mbar_init(smem_addr(&sh.meta_full[b]), 1);
-            mbar_init(smem_addr(&sh.meta_empty[b]), kSoftmaxWarps + 1);
+            mbar_init(smem_addr(&sh.meta_empty[b]), kSoftmaxWarps + kLoadWarps + 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kSoftmaxWarps + kLoadWarps) tmem_alloc<512>(&sh.tmem);
+    if (warp == kScoreWarp) tmem_alloc<512>(&sh.tmem);
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
@@ -643,70 +947,92 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const KvopsAttend a
     // A wait that gives up sets sh.stop and every role goes on to its end without waiting again, so
     // that no thread is left at a barrier.
     if (warp < kSoftmaxWarps) {
-        softmax_warps<T, NQ>(a, plan, sh, smem, begin, end);
+        softmax_warps<T, kStored, NQ>(a, plan, sh, smem, begin, end);
     } else if (warp < kSoftmaxWarps + kLoadWarps) {
         load_warps<T, Code, kStored, NQ>(a, plan, sh, smem, begin, end);
-    } else if ((threadIdx.x & 31) == 0) {
-        product_thread<T, NQ>(plan, sh, smem, begin, end);
+    } else if (warp == kScoreWarp) {
+        score_warp<T, kStored, NQ>(plan, sh, smem, begin, end);
+    } else if (warp == kWeighWarp) {
+        weigh_warp<T, kStored, NQ>(plan, sh, smem, begin, end);
+    } else {
+        find_warp<NQ, kStored>(a, plan, sh, begin, end);
     }
     __syncwarp();
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-    if (warp == kSoftmaxWarps + kLoadWarps) tmem_free<512>(sh.tmem);
+    if (warp == kScoreWarp) tmem_free<512>(sh.tmem);
     if (threadIdx.x == 0 && sh.stop != 0 && a.err_word != 0)
         atomicCAS_system(reinterpret_cast<uint32_t *>(a.err_word), 0u, KVOPS_ERR_ATTEND_TIMEOUT);
 }
 
+static_assert(sizeof(Shared) <= 6 * 1024, "as Layout counts it");
 static_assert(offsetof(Shared, per_warp) % 16 == 0 && alignof(Shared) % 16 == 0, "read as float4");
 
 // Joins the parts of the units that a CTA's run cuts. Block x is the cut between CTAs x and x + 1, and
-// does its unit if it is the first cut in it; eight query rows per block, one per warp. The parts are
-// added in their order.
+// does its unit if it is the first cut in it; block y takes four query rows, a thread one dimension of
+// them. The parts are added in their order.
 template <typename T, int NQ>
-__global__ void __launch_bounds__(256) join_kernel(const KvopsAttend a, const Plan plan)
+__global__ void __launch_bounds__(kValueDim) join_kernel(const KvopsAttend a, const Plan plan)
 {
+    __shared__ alignas(16) uint16_t rows[4][kValueDim];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t units = real_units(a, plan);
     const uint32_t cut = run_start(plan, units, blockIdx.x + 1);
     if (cut % plan.tiles == 0) return;
     const uint32_t unit = cut / plan.tiles, begin = unit * plan.tiles, end = begin + plan.tiles;
     if (run_start(plan, units, blockIdx.x) > begin) return;
-    const Unit u = unit_at<NQ>(a, plan, unit);
-    const uint32_t row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const Unit u = unit_at<NQ>(plan, unit);
+    const uint32_t row = blockIdx.y * 4, dim = threadIdx.x, lane = dim & 31;
     if (row >= u.rows) return;
-    float top = -INFINITY;
-    for (uint32_t c = blockIdx.x; c < plan.ctas && run_start(plan, units, c) < end; ++c) {
-        const uint32_t from = run_start(plan, units, c);
-        if (run_start(plan, units, c + 1) == from) continue;
-        top = fmaxf(top, plan.part_ml[static_cast<uint64_t>(2 * c + (from < begin ? 1 : 0)) * NQ + row].x);
-    }
-    float total = 0.f;
-    float4 acc[4];
-    for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t c = blockIdx.x; c < plan.ctas && run_start(plan, units, c) < end; ++c) {
-        const uint32_t from = run_start(plan, units, c);
-        if (run_start(plan, units, c + 1) == from) continue;
-        const uint64_t part = static_cast<uint64_t>(2 * c + (from < begin ? 1 : 0)) * NQ + row;
-        const float2 ml = plan.part_ml[part];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float w = exp2_fast(ml.x - top);
-        total += ml.y * w;
-        const float4 *o = reinterpret_cast<const float4 *>(plan.part_o + part * kValueDim);
+    const uint32_t block = dim >> 7, quarter = (dim >> 5) & 3, half = row / (NQ / 2), i = row % (NQ / 2) / 4;
+    // parts of CTA c: slot 2 c, or 2 c + 1 where its run started in an earlier unit
+    const auto part_of = [&](uint32_t c) { return 2 * c + (run_start(plan, units, c) < begin ? 1 : 0); };
+    uint32_t stop = blockIdx.x + 1;
+    while (stop < plan.ctas && run_start(plan, units, stop) < end) ++stop;
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, total[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c = blockIdx.x; c < stop; ++c) {
+        if (run_start(plan, units, c + 1) == run_start(plan, units, c)) continue;
+        const float2 *ml = plan.part_ml + static_cast<uint64_t>(part_of(c)) * NQ + row;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 v = o[i * 32 + lane];
-            acc[i].x += v.x * w, acc[i].y += v.y * w, acc[i].z += v.z * w, acc[i].w += v.w * w;
+        for (int k = 0; k < 4; ++k)
+            if (row + k < u.rows) top[k] = fmaxf(top[k], ml[k].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t c = blockIdx.x; c < stop; ++c) {
+        if (run_start(plan, units, c + 1) == run_start(plan, units, c)) continue;
+        const uint32_t part = part_of(c);
+        const float2 *ml = plan.part_ml + static_cast<uint64_t>(part) * NQ + row;
+        float w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            w[k] = 0.f;
+            if (row + k < u.rows && (ml[k].x != -INFINITY || ml[k].y != 0.f)) {
+                w[k] = exp2_fast(ml[k].x - top[k]);
+                total[k] += ml[k].y * w[k];
+            }
         }
+        const float4 v = reinterpret_cast<const float4 *>(plan.part_o)[part_at<NQ>(part, block, quarter, half, i, lane)];
+        acc.x += v.x * w[0], acc.y += v.y * w[1], acc.z += v.z * w[2], acc.w += v.w * w[3];
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    uint2 *out = reinterpret_cast<uint2 *>(a.out) + (u.out_row + row) * (kValueDim / 4);
+    const float v[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        out[i * 32 + lane] = make_uint2(T::pack(acc[i].x * inv, acc[i].y * inv), T::pack(acc[i].z * inv, acc[i].w * inv));
-    if (lane == 0 && a.lse != 0)
-        reinterpret_cast<float *>(a.lse)[u.out_row + row] =
-            total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
+    for (int k = 0; k < 4; ++k)
+        rows[k][dim] = static_cast<uint16_t>(T::pack(total[k] == 0.f ? 0.f : v[k] * (1.f / total[k]), 0.f));
+    __syncthreads();
+    if (dim < 256) {
+        const uint32_t k = dim >> 6, q = dim & 63;
+        if (row + k < u.rows)
+            reinterpret_cast<uint4 *>(a.out)[(u.out_row + row + k) * (kValueDim / 8) + q] =
+                *reinterpret_cast<const uint4 *>(&rows[k][q * 8]);
+    }
+    if (dim == 0 && a.lse != 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (row + k < u.rows)
+                reinterpret_cast<float *>(a.lse)[u.out_row + row + k] =
+                    total[k] == 0.f ? -INFINITY : (top[k] + log2f(total[k])) * 0.6931471805599453f;
+    }
 }
 
 // ---- the host ----------------------------------------------------------------------------------
@@ -739,9 +1065,17 @@ int sm_count()
     return n;
 }
 
-// Queries per tile and how the work is dealt out, for `lists` lists per request. The number of
-// pairs must stay below 2^32 (check_pairs).
-uint32_t queries_per_tile(uint32_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// Queries per tile. A pair costs about the same for any number up to 64 (the rows' way into shared
+// memory), so a tile takes as many as there are, unless smaller tiles keep more SMs busy.
+uint32_t queries_per_tile(const KvopsAttend &a, uint32_t lists, int sms)
+{
+    const uint32_t rows = a.heads * (lists > 1 ? 1 : a.tokens);
+    uint32_t nq = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    const uint64_t lists_all = static_cast<uint64_t>(a.max_num_reqs) * lists;
+    const uint64_t tiles = (a.top_k + a.drafts + kTile - 1) / kTile;
+    while (nq > 16 && lists_all * ((rows + nq / 2 - 1) / (nq / 2)) * tiles <= static_cast<uint64_t>(sms)) nq /= 2;
+    return nq;
+}
 
 Plan make_plan(const KvopsAttend &a, uint32_t lists, uint32_t nq, int sms)
 {
@@ -749,7 +1083,8 @@ Plan make_plan(const KvopsAttend &a, uint32_t lists, uint32_t nq, int sms)
     p.lists = lists;
     p.group_rows = a.heads * (lists > 1 ? 1 : a.tokens);
     p.qtiles = (p.group_rows + nq - 1) / nq;
-    p.tiles = (a.top_k + a.drafts + kTile - 1) / kTile;
+    p.list_end = (a.top_k + 3) & ~3u;
+    p.tiles = (p.list_end + a.drafts + kTile - 1) / kTile;
     if (p.tiles == 0) p.tiles = 1;  // no keys at all: outputs of zero
     const uint64_t units = static_cast<uint64_t>(a.max_num_reqs) * lists * p.qtiles, pairs = units * p.tiles;
     // Whole units need no joining, equal runs of pairs leave no SM idle. In tiles' times: a unit costs
@@ -775,14 +1110,14 @@ template <typename T, typename Code, bool kStored, int NQ>
 cudaError_t launch_as(const KvopsAttend &a, const Plan &p, cudaStream_t s)
 {
     const auto kernel = attend_kernel<T, Code, kStored, NQ>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<NQ>::bytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<NQ, kStored>::bytes);
     if (e != cudaSuccess) return e;
-    kernel<<<p.ctas, kThreads, Layout<NQ>::bytes, s>>>(a, p);
+    kernel<<<p.ctas, kThreads, Layout<NQ, kStored>::bytes, s>>>(a, p);
     e = cudaGetLastError();
     if (e != cudaSuccess || p.whole > 0 || p.ctas < 2) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.ctas - 1, NQ / 8);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(p.ctas - 1, (p.group_rows < NQ ? p.group_rows + 3 : NQ) / 4);
+    cfg.blockDim = dim3(kValueDim);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -796,9 +1131,9 @@ template <typename T, int NQ>
 cudaError_t launch_format(const KvopsAttend &a, const Plan &p, cudaStream_t s)
 {
     switch (a.row_format) {
+        case KVOPS_ROW_RAW: return launch_as<T, Int8, false, NQ>(a, p, s);
         case KVOPS_ROW_E4M3: return launch_as<T, E4m3, true, NQ>(a, p, s);
-        case KVOPS_ROW_INT8: return launch_as<T, Int8, true, NQ>(a, p, s);
-        default: return launch_as<T, Int8, false, NQ>(a, p, s);
+        default: return launch_as<T, Int8, true, NQ>(a, p, s);
     }
 }
 
@@ -825,7 +1160,7 @@ extern "C" int kvops_attend_workspace(const KvopsAttend *a, uint64_t *out_bytes)
     // enough for one list per request and for one per token
     uint64_t most = 0;
     for (uint32_t lists : {1u, a->tokens}) {
-        const uint32_t nq = kvb::queries_per_tile(a->heads * (lists > 1 ? 1 : a->tokens));
+        const uint32_t nq = kvb::queries_per_tile(*a, lists, sms);
         const uint64_t n = a->max_num_reqs == 0 ? 0 : kvb::workspace_of(kvb::make_plan(*a, lists, nq, sms), nq);
         most = n > most ? n : most;
     }
@@ -854,7 +1189,7 @@ extern "C" int kvops_attend_hot(const KvopsAttend *a, uint64_t stream)
     const int sms = kvb::sm_count();
     if (sms <= 0) return kvb::set_last_error(KVOPS_E_CUDA, "attend_hot: no current device");
     const uint32_t lists = a->tokens > 1 && a->slots_stride_token != 0 && a->top_k > 0 ? a->tokens : 1;
-    const uint32_t nq = kvb::queries_per_tile(a->heads * (lists > 1 ? 1 : a->tokens));
+    const uint32_t nq = kvb::queries_per_tile(*a, lists, sms);
     kvb::Plan p = kvb::make_plan(*a, lists, nq, sms);
     if (static_cast<uint64_t>(a->max_num_reqs) * lists * p.qtiles * p.tiles >= (1ull << 32))
         return invalid("attend_hot: requests x lists x keys out of range");

@@ -29,17 +29,24 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Waits for the phase of this parity, or until another wait of the CTA has given up (*stop). Gives
-// up itself, and says so in *stop, after kWaitTries tries (over a second).
-constexpr uint32_t kWaitTries = 1u << 22;
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *stop)
+// The whole warp waits for the phase of this parity, or until another wait of the CTA has given up
+// (*stop). Gives up itself, and says so in *stop, after kWaitClocks (half a second or more; the SM's own
+// clock, since reading the global timer takes microseconds). The warp leaves together: a lane left
+// behind could find the barrier two phases on, where the parity is its own again, and wait for good.
+constexpr long long kWaitClocks = 1ll << 30;
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *stop)
 {
-    for (uint32_t i = 0; i < kWaitTries; ++i) {
-        if (mbar_try(bar, parity)) return true;
-        if ((i & 63u) == 63u && *stop != 0) return false;
+    if (!mbar_try(bar, parity)) {
+        const long long start = clock64();
+        while (!mbar_try(bar, parity)) {
+            if (*stop != 0) break;
+            if (clock64() - start > kWaitClocks) {
+                *stop = 1u;
+                break;
+            }
+        }
     }
-    *stop = 1u;
-    return false;
+    __syncwarp();
 }
 
 // What generic stores wrote to shared memory becomes visible to the matrix instructions.
@@ -68,17 +75,30 @@ __host__ __device__ constexpr uint32_t instruction(uint32_t type, bool mn, uint3
            ((m / 16) << 24);
 }
 
-// acc (in tensor memory) = a * b + (accumulate ? acc : 0), 16 deep; issued by one thread.
-__device__ __forceinline__ void mma(uint32_t acc, uint64_t a, uint64_t b, uint32_t inst, bool accumulate)
+// acc (in tensor memory) = a * b + (accumulate ? acc : 0), 16 deep. The whole warp comes here and the
+// one lane with `elected` issues: the operands are then uniform over the warp and stay in uniform
+// registers (issued from a branch of one lane, each took some 90 cycles to move there).
+__device__ __forceinline__ void mma(uint32_t elected, uint32_t acc, uint64_t a, uint64_t b, uint32_t inst, bool accumulate)
 {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(acc),
-        "l"(a), "l"(b), "r"(inst), "r"(accumulate ? 1u : 0u) : "memory");
+        "{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; "
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(acc),
+        "l"(a), "l"(b), "r"(inst), "r"(accumulate ? 1u : 0u), "r"(elected) : "memory");
 }
-// The barrier gets an arrival once every matrix instruction issued so far has ended.
-__device__ __forceinline__ void commit(uint32_t bar)
+// The barrier gets an arrival once every matrix instruction that the lane issued so far has ended.
+__device__ __forceinline__ void commit(uint32_t elected, uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "{ .reg .pred q; setp.ne.b32 q, %1, 0; "
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar), "r"(elected)
+        : "memory");
+}
+// 1 in one lane of the converged warp.
+__device__ __forceinline__ uint32_t elect()
+{
+    uint32_t e;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(e));
+    return e;
 }
 
 template <uint32_t kCols>
