@@ -173,30 +173,22 @@ __device__ __forceinline__ float exp2_fast(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float warp_max(float x)
+// Of the threads of a warp with the same columns (those whose lanes differ in bits 2-4), the largest
+// values or the sums; returns the one of the thread's own column, number `own`.
+template <bool kMax, int kN>
+__device__ __forceinline__ float join_columns(float (&v)[kN], int own)
 {
-    float y;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Lane l's sum over the warp of column l % kN.
-template <int kN>
-__device__ __forceinline__ float column_sum(float (&v)[kN], int lane)
-{
+    float mine = 0.f;
 #pragma unroll
-    for (int w = kN / 2; w > 0; w /= 2) {
+    for (int i = 0; i < kN; ++i) {
 #pragma unroll
-        for (int i = 0; i < w; ++i) {
-            const bool up = (lane & w) != 0;
-            const float give = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
-            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, w);
+        for (int w = 4; w < 32; w *= 2) {
+            const float other = __shfl_xor_sync(0xFFFFFFFFu, v[i], w);
+            v[i] = kMax ? fmaxf(v[i], other) : v[i] + other;
         }
+        if (own == i) mine = v[i];
     }
-    float s = v[0];
-#pragma unroll
-    for (int w = kN; w < 32; w *= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, w);
-    return s;
+    return mine;
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool some)
@@ -651,24 +643,30 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                                               uint32_t begin, uint32_t end)
 {
     using namespace tc;
-    constexpr int NH = NQ / 2;  // queries of a thread
+    constexpr int NH = NQ / 2, kBlocks = NH / 8;  // a half's queries
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int quarter = warp & 3, half = warp >> 2;
-    // The scores of 64 keys lie in lanes 0-15 of each quarter: lanes 16-31 have no key, but their share of
-    // the outputs' dimensions.
-    const int key = quarter * 16 + (lane & 15), dim = quarter * 32 + lane;
-    const bool keyed = lane < 16;
+    // The scores of 64 keys lie in lanes 0-15 of each quarter of tensor memory. A thread takes two keys,
+    // key and key + 8, and of each eight columns of its half two: 8 b + pair, 8 b + pair + 1.
+    const int key = quarter * 16 + (lane >> 2), pair = 2 * (lane & 3), dim = quarter * 32 + lane;
+    // The column whose reference the thread keeps (the four warps of a half, and more than one thread
+    // where a half has fewer than 32 columns, keep the same).
+    const int slot_of = (lane >> 2) & (2 * kBlocks - 1), column = 8 * (slot_of >> 1) + pair + (slot_of & 1);
     const uint32_t lanes = static_cast<uint32_t>(quarter) << 21;
     const uint32_t s_at = sh.tmem + lanes + half * NH, o_at = s_at + 2 * NQ;
     const float factor = a.scale * 1.4426950408889634f;  // scores as powers of two
     float *mine = sh.per_warp[warp];
-    const auto spread = [&](float x) {  // column c's x, held by lane c, to be read by every lane
+    const auto spread = [&](float x) {  // x of the thread's column, to be read by every lane
         __syncwarp();
-        mine[lane] = x;
+        mine[column] = x;
         __syncwarp();
     };
-    // of columns i .. i + 3; volatile: read where it is used, not kept in registers
-    const auto spread4 = [&](int i) {
+    const auto spread2 = [&](int b) {  // of columns 8 b + pair and the next
+        float2 f;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(smem_addr(mine + 8 * b + pair)) : "memory");
+        return f;
+    };
+    const auto spread4 = [&](int i) {  // of columns i .. i + 3
         float4 f;
         asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                      : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(smem_addr(mine + i)) : "memory");
@@ -677,8 +675,8 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
     uint32_t done = 0, unit = begin / plan.tiles, tile = begin - unit * plan.tiles, start_tile = tile;
     bool fresh = true, started = false, open = false;
     Unit u{};
-    float ref = -INFINITY;  // of column `lane` of this half
-    float sum[NH];          // of this thread's keys, by column
+    float ref = -INFINITY;   // of `column`
+    float sum[2 * kBlocks];  // of this thread's keys, by its columns
     for (uint32_t at = begin, meta = 0; at < end; ++at, ++meta) {
         if (fresh) {
             fresh = started = false;
@@ -686,7 +684,7 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
             u = unit_at<NQ>(plan, unit);
             ref = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NH; ++i) sum[i] = 0.f;
+            for (int i = 0; i < 2 * kBlocks; ++i) sum[i] = 0.f;
             if (a.drafts > 0) {
                 group_barrier(3, kSoftmaxWarps * 32);
                 if (threadIdx.x < NQ && threadIdx.x < u.rows) {
@@ -704,48 +702,47 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
             mbar_wait(smem_addr(&sh.s_full[done & 1]), (done >> 1) & 1, &sh.stop);
             fence_after_sync();
         }
-        const uint8_t kind = keyed ? *const_cast<volatile uint8_t *>(&sh.kind[meta % kAhead][key]) : kNone;
+        const uint8_t kind[2] = {*const_cast<volatile uint8_t *>(&sh.kind[meta % kAhead][key]),
+                                 *const_cast<volatile uint8_t *>(&sh.kind[meta % kAhead][key + 8])};
         tile_done(sh, meta, lane);
         if (any) {
-            float y[NH];  // the scores in powers of two, then less their references, then probabilities
+            // The scores in powers of two, then less their references, then probabilities.
+            float y[4 * kBlocks];
             const auto scores = [&]() {
-                tmem_load<NH>(s_at + (done & 1) * NQ, y);
+                tmem_load_spread<kBlocks>(s_at + (done & 1) * NQ, y);
 #pragma unroll
-                for (int i = 0; i < NH; ++i) y[i] = kind == kNone ? -INFINITY : y[i] * factor;
-                if (kind >= kDraft) {
-                    const uint32_t j = tile * kTile + key - plan.list_end;
+                for (int i = 0; i < 4 * kBlocks; ++i) y[i] = kind[i >> 1 & 1] == kNone ? -INFINITY : y[i] * factor;
 #pragma unroll
-                    for (int i = 0; i < NH; ++i) {
-                        const bool sees = (sh.tree[half * NH + i] >> j) & 1;
-                        if (!sees) y[i] = -INFINITY;
-                        else if (kind == kBadDraft) y[i] = NAN;
+                for (int r = 0; r < 2; ++r) {
+                    if (kind[r] < kDraft) continue;
+                    const uint32_t j = tile * kTile + key + 8 * r - plan.list_end;
+#pragma unroll
+                    for (int i = 0; i < 2 * kBlocks; ++i) {
+                        float &x = y[4 * (i >> 1) + 2 * r + (i & 1)];
+                        if (!(sh.tree[half * NH + 8 * (i >> 1) + pair + (i & 1)] >> j & 1)) x = -INFINITY;
+                        else if (kind[r] == kBadDraft) x = NAN;
                     }
                 }
             };
             const auto lower = [&]() {  // by the references, which the warp keeps spread; their largest excess
                 float excess = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < NH; i += 4) {
-                    const float4 r = spread4(i);
-                    y[i] -= r.x, y[i + 1] -= r.y, y[i + 2] -= r.z, y[i + 3] -= r.w;
-                    excess = fmaxf(excess, fmaxf(fmaxf(y[i], y[i + 1]), fmaxf(y[i + 2], y[i + 3])));
+                for (int b = 0; b < kBlocks; ++b) {
+                    const float2 r = spread2(b);
+                    y[4 * b] -= r.x, y[4 * b + 1] -= r.y, y[4 * b + 2] -= r.x, y[4 * b + 3] -= r.y;
+                    excess = fmaxf(excess, fmaxf(fmaxf(y[4 * b], y[4 * b + 1]), fmaxf(y[4 * b + 2], y[4 * b + 3])));
                 }
                 return excess;
             };
             const auto write = [&]() {  // the probabilities, to where the second product reads them
-                const uint32_t to = smem + Layout<NQ, kStored>::rope + (done & 1) * kChunkBytes + key * 128;
+                const uint32_t to = smem + Layout<NQ, kStored>::rope + (done & 1) * kChunkBytes + key * 128 + pair * 2;
 #pragma unroll
-                for (int i = 0; i < NH; i += 8) {
-                    uint32_t w[4];
+                for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int c = i + 2 * k;
-                        y[c] = exp2_fast(y[c]);
-                        y[c + 1] = exp2_fast(y[c + 1]);
-                        w[k] = T::pack(y[c], y[c + 1]);
-                    }
-                    if (keyed)
-                        store16(to + ((((half * NH + i) >> 3) ^ (key & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                    for (int i = 4 * b; i < 4 * b + 4; ++i) y[i] = exp2_fast(y[i]);
+                    const uint32_t at = to + (((half * kBlocks + b) ^ (key & 7)) << 4);
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(T::pack(y[4 * b], y[4 * b + 1])) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 1024), "r"(T::pack(y[4 * b + 2], y[4 * b + 3])) : "memory");
                 }
             };
             scores();
@@ -760,17 +757,15 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 if (move_all) scores();
             }
             if (move_all) {
-                float top = -INFINITY;
+                float m[2 * kBlocks];
 #pragma unroll
-                for (int i = 0; i < NH; ++i) {
-                    const float m = warp_max(y[i]);
-                    if (lane == i) top = m;
-                }
-                sh.top[half][quarter][lane] = top;
+                for (int i = 0; i < 2 * kBlocks; ++i) m[i] = fmaxf(y[4 * (i >> 1) + (i & 1)], y[4 * (i >> 1) + 2 + (i & 1)]);
+                float top = join_columns<true>(m, slot_of);
+                sh.top[half][quarter][column] = top;
                 group_barrier(1 + half, 128);
                 // the same decision in the four warps of this half
-                top = fmaxf(fmaxf(sh.top[half][0][lane], sh.top[half][1][lane]),
-                            fmaxf(sh.top[half][2][lane], sh.top[half][3][lane]));
+                top = fmaxf(fmaxf(sh.top[half][0][column], sh.top[half][1][column]),
+                            fmaxf(sh.top[half][2][column], sh.top[half][3][column]));
                 const bool move = top > ref + (kLift + kSlack) || (ref == -INFINITY && top > -INFINITY);
                 const float was = ref;
                 if (move) ref = top - kLift;
@@ -779,9 +774,9 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                     mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
                     fence_after_sync();
 #pragma unroll
-                    for (int i = 0; i < NH; i += 4) {
-                        const float4 f = spread4(i);
-                        sum[i] *= f.x, sum[i + 1] *= f.y, sum[i + 2] *= f.z, sum[i + 3] *= f.w;
+                    for (int b = 0; b < kBlocks; ++b) {
+                        const float2 f = spread2(b);
+                        sum[2 * b] *= f.x, sum[2 * b + 1] *= f.y;
                     }
 #pragma unroll 1
                     for (int b = 0; b < 4 * NH / 8; ++b) {
@@ -797,12 +792,12 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 }
                 spread(ref == -INFINITY ? 0.f : ref);
                 // a column without any key so far: its first finite score moves its reference
-                open = __any_sync(0xFFFFFFFFu, lane < NH && ref == -INFINITY);
+                open = __any_sync(0xFFFFFFFFu, ref == -INFINITY);
                 lower();
                 write();
             }
 #pragma unroll
-            for (int i = 0; i < NH; ++i) sum[i] += y[i];
+            for (int i = 0; i < 2 * kBlocks; ++i) sum[i] += y[4 * (i >> 1) + (i & 1)] + y[4 * (i >> 1) + 2 + (i & 1)];
             // Every tile's end is waited for in its turn, since a parity only tells a phase from its
             // neighbours. This one was reached before the next tile's first product, as a rule.
             if (done > 0) mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
@@ -817,22 +812,25 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
         if (ends || at + 1 == end) {
             const bool complete = ends && start_tile == 0;
             const uint32_t slot = 2 * blockIdx.x + (at - tile + start_tile > begin ? 1 : 0);
-            float total = column_sum<NH>(sum, lane);
+            const float part = join_columns<false>(sum, slot_of);
             group_barrier(1 + half, 128);
-            sh.top[half][quarter][lane] = total;
+            sh.top[half][quarter][column] = part;
             group_barrier(1 + half, 128);
-            // every warp adds the quarters in the same order
-            total = (sh.top[half][0][lane & (NH - 1)] + sh.top[half][1][lane & (NH - 1)]) +
-                    (sh.top[half][2][lane & (NH - 1)] + sh.top[half][3][lane & (NH - 1)]);
+            // From here on lane l has column l. Every warp adds the quarters in the same order.
+            const int c = lane & (NH - 1);
+            const float total = (sh.top[half][0][c] + sh.top[half][1][c]) + (sh.top[half][2][c] + sh.top[half][3][c]);
+            const float at_ref = started ? mine[c] : 0.f;
+            __syncwarp();
             const uint32_t col = half * NH + lane;
             if (lane < NH && quarter == 0 && col < u.rows) {
                 if (!complete)
-                    plan.part_ml[static_cast<uint64_t>(slot) * NQ + col] = make_float2(ref, total);
+                    plan.part_ml[static_cast<uint64_t>(slot) * NQ + col] = make_float2(total == 0.f ? -INFINITY : at_ref, total);
                 else if (a.lse != 0)
                     reinterpret_cast<float *>(a.lse)[u.out_row + col] =
-                        total == 0.f ? -INFINITY : (ref + log2f(total)) * 0.6931471805599453f;
+                        total == 0.f ? -INFINITY : (at_ref + log2f(total)) * 0.6931471805599453f;
             }
-            spread(total == 0.f ? 0.f : 1.f / total);
+            if (lane < NH) mine[lane] = total == 0.f ? 0.f : 1.f / total;
+            __syncwarp();
             if (started) {
                 mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
                 fence_after_sync();

@@ -153,6 +153,37 @@ __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[kN])
 #pragma unroll
     for (int i = 0; i < kN; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Lanes 0-15 of the calling warp's quarter, 8 kBlocks columns from `at`, spread over all its threads:
+// v[4 b + 2 r + e] of thread t is lane t / 4 + 8 r, column 8 b + 2 (t % 4) + e.
+template <int kBlocks>
+__device__ __forceinline__ void tmem_load_spread(uint32_t at, float (&v)[4 * kBlocks])
+{
+    static_assert(kBlocks == 1 || kBlocks == 2 || kBlocks == 4, "blocks");
+    uint32_t r[4 * kBlocks];
+    if constexpr (kBlocks == 1) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4]; "
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+            : "r"(at) : "memory");
+    } else if constexpr (kBlocks == 2) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8]; "
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+            : "r"(at) : "memory");
+    } else {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16]; "
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+              "=r"(r[15])
+            : "r"(at) : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * kBlocks; ++i) v[i] = __uint_as_float(r[i]);
+}
 template <int kN>
 __device__ __forceinline__ void tmem_store(uint32_t at, const float (&v)[kN])
 {
