@@ -69,7 +69,7 @@ struct Plan {
     uint32_t list_end;    // top_k rounded up to four: where the drafted rows start among the keys
     uint32_t tiles;       // key tiles per unit
     uint32_t ctas;
-    uint32_t whole;       // > 0: every CTA takes this many whole units; 0: an equal run of pairs
+    uint32_t whole;       // > 0: every CTA takes this many whole units; 0: runs of pairs of one length
     float2 *part_ml;      // [2 * ctas][NQ] reference and sum of a unit's part
     float *part_o;        // [2 * ctas][NQ * 512] its weighted sums, in part_at's order
 };
@@ -90,11 +90,10 @@ __device__ __forceinline__ uint32_t real_units(const KvopsAttend &a, const Plan 
     return reqs * p.lists * p.qtiles;
 }
 
-// The first pair of CTA c.
-__device__ __forceinline__ uint32_t run_start(const Plan &p, uint32_t units, uint32_t c)
+// Pairs of a CTA's run; CTA c has those from c * run_length on.
+__device__ __forceinline__ uint32_t run_length(const Plan &p, uint32_t units)
 {
-    if (p.whole > 0) return min(c * p.whole, units) * p.tiles;
-    return static_cast<uint32_t>(static_cast<uint64_t>(units) * p.tiles * c / p.ctas);
+    return p.whole > 0 ? p.whole * p.tiles : (units * p.tiles + p.ctas - 1) / p.ctas;
 }
 
 struct Unit {
@@ -941,7 +940,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     fence_after_sync();
     const uint32_t units = real_units(a, plan);
-    const uint32_t begin = run_start(plan, units, blockIdx.x), end = run_start(plan, units, blockIdx.x + 1);
+    const uint32_t run = run_length(plan, units), pairs = units * plan.tiles;
+    const uint32_t begin = min(blockIdx.x * run, pairs), end = min(begin + run, pairs);
     // A wait that gives up sets sh.stop and every role goes on to its end without waiting again, so
     // that no thread is left at a barrier.
     if (warp < kSoftmaxWarps) {
@@ -967,64 +967,89 @@ __global__ void __launch_bounds__(kThreads, 1)
 static_assert(sizeof(Shared) <= 6 * 1024, "as Layout counts it");
 static_assert(offsetof(Shared, per_warp) % 16 == 0 && alignof(Shared) % 16 == 0, "read as float4");
 
-// Joins the parts of the units that a CTA's run cuts. Block x is the cut between CTAs x and x + 1, and
-// does its unit if it is the first cut in it; block y takes four query rows, a thread one dimension of
-// them. The parts are added in their order.
+// Joins the parts of the units that the ends of runs cut. Block x is the cut behind CTA x's run, and does
+// its unit if it is the first cut in it; block y takes four query rows, block z 128 dimensions, a thread
+// one of them. The parts are added in their order.
+constexpr int kJoinThreads = 128;
 template <typename T, int NQ>
-__global__ void __launch_bounds__(kValueDim) join_kernel(const KvopsAttend a, const Plan plan)
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const KvopsAttend a, const Plan plan)
 {
-    __shared__ alignas(16) uint16_t rows[4][kValueDim];
+    __shared__ alignas(16) uint16_t rows[4][kJoinThreads];
+    __shared__ float4 weight[kJoinThreads];  // of a part, by row
+    __shared__ float top_of[4][4], sum_of[4][4];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t units = real_units(a, plan);
-    const uint32_t cut = run_start(plan, units, blockIdx.x + 1);
-    if (cut % plan.tiles == 0) return;
+    const uint32_t units = real_units(a, plan), run = run_length(plan, units), cut = (blockIdx.x + 1) * run;
+    if (cut >= units * plan.tiles || cut % plan.tiles == 0) return;
     const uint32_t unit = cut / plan.tiles, begin = unit * plan.tiles, end = begin + plan.tiles;
-    if (run_start(plan, units, blockIdx.x) > begin) return;
+    const uint32_t first = begin / run, parts = (end - 1) / run - first + 1;
+    if (first != blockIdx.x) return;
     const Unit u = unit_at<NQ>(plan, unit);
-    const uint32_t row = blockIdx.y * 4, dim = threadIdx.x, lane = dim & 31;
+    const uint32_t row = blockIdx.y * 4, thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
     if (row >= u.rows) return;
-    const uint32_t block = dim >> 7, quarter = (dim >> 5) & 3, half = row / (NQ / 2), i = row % (NQ / 2) / 4;
-    // parts of CTA c: slot 2 c, or 2 c + 1 where its run started in an earlier unit
-    const auto part_of = [&](uint32_t c) { return 2 * c + (run_start(plan, units, c) < begin ? 1 : 0); };
-    uint32_t stop = blockIdx.x + 1;
-    while (stop < plan.ctas && run_start(plan, units, stop) < end) ++stop;
+    const uint32_t half = row / (NQ / 2), i = row % (NQ / 2) / 4;
+    // the part of CTA c: slot 2 c, or 2 c + 1 where its run started in an earlier unit (the first's may have)
+    const auto slot_of = [&](uint32_t n) { return 2 * (first + n) + (n == 0 && first * run < begin ? 1 : 0); };
+    const auto at_most = [&](float x, float (&of)[4][4], int k) {  // over the block's threads
+        for (int w = 16; w > 0; w /= 2) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, w));
+        if (lane == 0) of[k][warp] = x;
+    };
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, total[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t c = blockIdx.x; c < stop; ++c) {
-        if (run_start(plan, units, c + 1) == run_start(plan, units, c)) continue;
-        const float2 *ml = plan.part_ml + static_cast<uint64_t>(part_of(c)) * NQ + row;
+    for (uint32_t n = thread; n < parts; n += kJoinThreads) {
+        const float2 *ml = plan.part_ml + static_cast<uint64_t>(slot_of(n)) * NQ + row;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (row + k < u.rows) top[k] = fmaxf(top[k], ml[k].x);
     }
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t c = blockIdx.x; c < stop; ++c) {
-        if (run_start(plan, units, c + 1) == run_start(plan, units, c)) continue;
-        const uint32_t part = part_of(c);
-        const float2 *ml = plan.part_ml + static_cast<uint64_t>(part) * NQ + row;
-        float w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            w[k] = 0.f;
-            if (row + k < u.rows && (ml[k].x != -INFINITY || ml[k].y != 0.f)) {
-                w[k] = exp2_fast(ml[k].x - top[k]);
-                total[k] += ml[k].y * w[k];
+    for (int k = 0; k < 4; ++k) at_most(top[k], top_of, k);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top[k] = fmaxf(fmaxf(top_of[k][0], top_of[k][1]), fmaxf(top_of[k][2], top_of[k][3]));
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t n0 = 0; n0 < parts; n0 += kJoinThreads) {
+        const uint32_t some = min(parts - n0, static_cast<uint32_t>(kJoinThreads));
+        if (thread < some) {
+            const float2 *ml = plan.part_ml + static_cast<uint64_t>(slot_of(n0 + thread)) * NQ + row;
+            float w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                w[k] = 0.f;
+                if (row + k < u.rows && (ml[k].x != -INFINITY || ml[k].y != 0.f)) {
+                    w[k] = exp2_fast(ml[k].x - top[k]);
+                    total[k] += ml[k].y * w[k];
+                }
             }
+            weight[thread] = make_float4(w[0], w[1], w[2], w[3]);
         }
-        const float4 v = reinterpret_cast<const float4 *>(plan.part_o)[part_at<NQ>(part, block, quarter, half, i, lane)];
-        acc.x += v.x * w[0], acc.y += v.y * w[1], acc.z += v.z * w[2], acc.w += v.w * w[3];
+        __syncthreads();
+        const float4 *o = reinterpret_cast<const float4 *>(plan.part_o);
+#pragma unroll 8
+        for (uint32_t n = 0; n < some; ++n) {
+            const float4 v = o[part_at<NQ>(slot_of(n0 + n), blockIdx.z, warp, half, i, lane)], w = weight[n];
+            acc.x += v.x * w.x, acc.y += v.y * w.y, acc.z += v.z * w.z, acc.w += v.w * w.w;
+        }
+        __syncthreads();
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        for (int w = 16; w > 0; w /= 2) total[k] += __shfl_xor_sync(0xFFFFFFFFu, total[k], w);
+        if (lane == 0) sum_of[k][warp] = total[k];
+    }
+    __syncthreads();
     const float v[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        rows[k][dim] = static_cast<uint16_t>(T::pack(total[k] == 0.f ? 0.f : v[k] * (1.f / total[k]), 0.f));
+    for (int k = 0; k < 4; ++k) {
+        total[k] = (sum_of[k][0] + sum_of[k][1]) + (sum_of[k][2] + sum_of[k][3]);
+        rows[k][thread] = static_cast<uint16_t>(T::pack(total[k] == 0.f ? 0.f : v[k] * (1.f / total[k]), 0.f));
+    }
     __syncthreads();
-    if (dim < 256) {
-        const uint32_t k = dim >> 6, q = dim & 63;
+    if (thread < 64) {
+        const uint32_t k = thread >> 4, q = thread & 15;
         if (row + k < u.rows)
-            reinterpret_cast<uint4 *>(a.out)[(u.out_row + row + k) * (kValueDim / 8) + q] =
+            reinterpret_cast<uint4 *>(a.out)[(u.out_row + row + k) * (kValueDim / 8) + blockIdx.z * 16 + q] =
                 *reinterpret_cast<const uint4 *>(&rows[k][q * 8]);
     }
-    if (dim == 0 && a.lse != 0) {
+    if (thread == 0 && blockIdx.z == 0 && a.lse != 0) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (row + k < u.rows)
@@ -1114,8 +1139,8 @@ cudaError_t launch_as(const KvopsAttend &a, const Plan &p, cudaStream_t s)
     e = cudaGetLastError();
     if (e != cudaSuccess || p.whole > 0 || p.ctas < 2) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.ctas - 1, (p.group_rows < NQ ? p.group_rows + 3 : NQ) / 4);
-    cfg.blockDim = dim3(kValueDim);
+    cfg.gridDim = dim3(p.ctas - 1, (p.group_rows < NQ ? p.group_rows + 3 : NQ) / 4, kValueDim / kJoinThreads);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
