@@ -290,23 +290,24 @@ int kvops_import_multi_noalloc(uint32_t node_num, const uint64_t *seg_bases, uin
 int kvops_quant_row_bytes(uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
                           uint32_t *out_bytes);
 
-/* kvops_export_seg_alllayer_ex that quantises: the source rows have 2 * (quant_elems +
- * plain_elems) bytes, the segment's rows are stored rows. */
-int kvops_export_quant_alllayer(uint64_t channel, uint64_t seg_base, uint32_t per_layer_seg_rows,
+/* kvops_export_seg_alllayer_ex that quantises, over all segments in one launch: the source rows have
+ * 2 * (quant_elems + plain_elems) bytes, the segments' rows are stored rows. Writes the status pages of
+ * every node. */
+int kvops_export_quant_alllayer(uint32_t node_num, const uint64_t *seg_bases, uint32_t per_layer_seg_rows,
                                 uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
                                 uint32_t row_lo, uint32_t row_cnt, uint32_t layer_num, uint64_t src_layer0_base,
-                                uint64_t src_layer_stride, uint32_t stripe_rows, uint32_t node_num, uint32_t my_node,
-                                uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts);
+                                uint64_t src_layer_stride, uint32_t stripe_rows, uint64_t status, uint64_t stream,
+                                uint32_t block_dim, const KvopsRowOpts *opts);
 
-/* kvops_export_seg that quantises: the flagged hot rows are 16-bit rows, the segment's rows are
- * stored rows. The form for single tokens. */
-int kvops_export_quant(uint64_t channel, uint64_t seg_base, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
-                       uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
-                       uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
-                       uint64_t topk_device_slots, uint64_t export_flags, uint64_t num_real, uint64_t hot_row_base,
-                       uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint32_t node_num,
-                       uint32_t my_node, uint64_t status, uint64_t stream, uint32_t block_dim,
-                       const KvopsRowOpts *opts);
+/* kvops_export_seg that quantises, over all segments in one launch: the flagged hot rows are 16-bit
+ * rows, the segments' rows are stored rows. The form for single tokens. Positions that name the same
+ * segment row race. */
+int kvops_export_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows,
+                       uint32_t per_layer_seg_rows, uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems,
+                       uint32_t plain_elems, uint64_t topk_indices, uint64_t req_pool_indices,
+                       uint64_t req_host_base, uint64_t topk_device_slots, uint64_t export_flags, uint64_t num_real,
+                       uint64_t hot_row_base, uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows,
+                       uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts);
 
 /* kvops_import_multi that reads stored rows back into 16-bit hot rows. */
 int kvops_import_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows,

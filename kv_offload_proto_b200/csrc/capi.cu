@@ -229,7 +229,7 @@ int import_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t node_lo
 int export_common(uint64_t seg_base, uint32_t plsr, uint32_t row_bytes, uint32_t row_lo, uint32_t row_cnt,
                   uint32_t layer_num, uint64_t src_layer0_base, uint64_t src_layer_stride, uint32_t stripe_rows,
                   uint32_t node_num, uint32_t my_node, uint64_t status, uint64_t stream, uint32_t block_dim,
-                  const KvopsRowOpts *opts, const kvb::RowCodec *codec = nullptr)
+                  const KvopsRowOpts *opts)
 {
     KV_REQUIRE_INIT();
     if (block_dim > 8) return fail(KVOPS_E_INVALID, "export blockDim must be <= 8 (status slot layout)");
@@ -282,9 +282,7 @@ int export_common(uint64_t seg_base, uint32_t plsr, uint32_t row_bytes, uint32_t
         p.units_per_layer = 0;
         p.seg_null = 1;
     }
-    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = codec != nullptr ? kvb::launch_export_quant(p, *codec, s, ds->sm_count)
-                                     : kvb::launch_export(p, s, ds->sm_count);
+    cudaError_t e = kvb::launch_export(p, reinterpret_cast<cudaStream_t>(stream), ds->sm_count);
     if (e != cudaSuccess) return cuda_fail(e, "launch kvc_scatter_rows_alllayer");
     return KVOPS_OK;
 }
@@ -307,8 +305,8 @@ int make_codec(uint32_t format, uint32_t dtype, uint32_t quant, uint32_t plain, 
 
 // The gather of 16-bit hot rows from stored segment rows (or the scatter into them): build_gather
 // with the stored row's size, the hot rows' stride in 16-bit rows, and the codec's alignment.
-int gather_quant_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t node_lo, uint32_t node_hi,
-                        uint32_t my_node, uint32_t layer_offset_rows, uint32_t plsr, uint32_t row_format,
+int gather_quant_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows, uint32_t plsr,
+                        uint32_t row_format,
                         uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems, uint64_t topk_indices,
                         uint64_t req_pool_indices, uint64_t req_host_base, uint64_t topk_device_slots, uint64_t flags,
                         uint64_t num_real, uint64_t hot_row_base, uint32_t top_k, uint32_t max_num_reqs,
@@ -316,6 +314,10 @@ int gather_quant_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t n
                         const KvopsRowOpts *opts, bool write)
 {
     const char *what = write ? "export_quant" : "import_quant";
+    KV_REQUIRE_INIT();
+    if (node_num == 0 || node_num > KVOPS_MAX_NODES)
+        return fail(KVOPS_E_INVALID, std::string(what) + " node_num must be in [1, 64]");
+    if (seg_bases == nullptr) return fail(KVOPS_E_INVALID, std::string(what) + ": seg_bases is NULL");
     kvb::RowCodec c{};
     int rc = make_codec(row_format, row_dtype, quant_elems, plain_elems, what, &c);
     if (rc != KVOPS_OK) return rc;
@@ -325,7 +327,7 @@ int gather_quant_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t n
         return fail(KVOPS_E_INVALID, std::string(what) + ": hot rows and segments must be 16-byte aligned");
     kvb::GatherParams p{};
     DeviceState *ds = nullptr;
-    rc = build_gather(node_num, seg_bases, node_lo, node_hi, my_node, layer_offset_rows, plsr,
+    rc = build_gather(node_num, seg_bases, 0, node_num, kvb::kAllNodes, layer_offset_rows, plsr,
                       kvb::codec_stored_bytes(c), topk_indices, req_pool_indices, req_host_base, topk_device_slots,
                       flags, num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream, block_dim, opts,
                       &p, &ds, what);
@@ -749,45 +751,67 @@ int kvops_quant_row_bytes(uint32_t row_format, uint32_t row_dtype, uint32_t quan
     return KVOPS_OK;
 }
 
-int kvops_export_quant_alllayer(uint64_t channel, uint64_t seg_base, uint32_t per_layer_seg_rows,
+int kvops_export_quant_alllayer(uint32_t node_num, const uint64_t *seg_bases, uint32_t per_layer_seg_rows,
                                 uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
                                 uint32_t row_lo, uint32_t row_cnt, uint32_t layer_num, uint64_t src_layer0_base,
-                                uint64_t src_layer_stride, uint32_t stripe_rows, uint32_t node_num, uint32_t my_node,
-                                uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts)
+                                uint64_t src_layer_stride, uint32_t stripe_rows, uint64_t status, uint64_t stream,
+                                uint32_t block_dim, const KvopsRowOpts *opts)
 {
-    (void)channel;
     KV_REQUIRE_INIT();
-    kvb::RowCodec c{};
-    const int rc = make_codec(row_format, row_dtype, quant_elems, plain_elems, "export_quant_alllayer", &c);
+    if (node_num == 0 || node_num > KVOPS_MAX_NODES)
+        return fail(KVOPS_E_INVALID, "export_quant_alllayer node_num must be in [1, 64]");
+    if (seg_bases == nullptr) return fail(KVOPS_E_INVALID, "export_quant_alllayer: seg_bases is NULL");
+    if (block_dim == 0 || block_dim > 8)
+        return fail(KVOPS_E_INVALID, "export_quant_alllayer blockDim must be in [1, 8] (status slot layout)");
+    kvb::ExportQuantParams p{};
+    int rc = make_codec(row_format, row_dtype, quant_elems, plain_elems, "export_quant_alllayer", &p.codec);
     if (rc != KVOPS_OK) return rc;
-    if ((seg_base | src_layer0_base | src_layer_stride) % 16 != 0)
+    uint64_t bases = src_layer0_base | src_layer_stride;
+    for (uint32_t n = 0; n < node_num; ++n) bases |= seg_bases[n];
+    if (bases % 16 != 0)
         return fail(KVOPS_E_INVALID, "export_quant_alllayer: bases and strides must be 16-byte aligned");
     if (row_cnt > 0 && layer_num > 0 && src_layer0_base == 0)
         return fail(KVOPS_E_INVALID, "export_quant_alllayer: a tensor address is 0");
-    return export_common(seg_base, per_layer_seg_rows, kvb::codec_stored_bytes(c), row_lo, row_cnt, layer_num,
-                         src_layer0_base, src_layer_stride, stripe_rows, node_num, my_node, status, stream, block_dim,
-                         opts, &c);
+    if (static_cast<uint64_t>(row_lo) + row_cnt > (1ull << 32))
+        return fail(KVOPS_E_INVALID, "export_quant_alllayer row_lo + row_cnt exceeds the 32-bit row space");
+    const KvopsRowOpts o = opts ? *opts : KvopsRowOpts{};
+    if (o.injective > 1) return fail(KVOPS_E_INVALID, "export_quant_alllayer: injective must be 0 or 1");
+    if ((o.err_word & 3) != 0) return fail(KVOPS_E_INVALID, "export_quant_alllayer: err_word must be 4-byte aligned");
+    DeviceState *ds = nullptr;
+    rc = current_device_state(&ds);
+    if (rc != KVOPS_OK) return rc;
+    p.src0 = reinterpret_cast<const uint8_t *>(src_layer0_base);
+    p.src_layer_stride = src_layer_stride;
+    p.plsr = per_layer_seg_rows;
+    p.row_lo = row_lo;
+    p.row_cnt = row_cnt;
+    p.layer_num = layer_num;
+    p.stripe = stripe_rows;
+    p.nodes = node_num;
+    p.injective = o.injective;
+    p.units_per_layer = row_cnt;
+    if (stripe_rows > 0 && o.injective == 0 && row_cnt > 0)
+        p.units_per_layer = (static_cast<uint64_t>(row_lo) + row_cnt - 1) / stripe_rows - row_lo / stripe_rows + 1;
+    for (uint32_t n = 0; n < node_num; ++n) p.seg[n] = reinterpret_cast<uint8_t *>(seg_bases[n]);
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    rc = make_status_target(status, 0, node_num, block_dim, ds, o.err_word, s, &p.st);
+    if (rc != KVOPS_OK) return rc;
+    const cudaError_t e = kvb::launch_export_quant(p, s, ds->sm_count);
+    if (e != cudaSuccess) return cuda_fail(e, "launch export_quant_alllayer");
+    return KVOPS_OK;
 }
 
-int kvops_export_quant(uint64_t channel, uint64_t seg_base, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
-                       uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
-                       uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
-                       uint64_t topk_device_slots, uint64_t export_flags, uint64_t num_real, uint64_t hot_row_base,
-                       uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint32_t node_num,
-                       uint32_t my_node, uint64_t status, uint64_t stream, uint32_t block_dim,
-                       const KvopsRowOpts *opts)
+int kvops_export_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows,
+                       uint32_t per_layer_seg_rows, uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems,
+                       uint32_t plain_elems, uint64_t topk_indices, uint64_t req_pool_indices,
+                       uint64_t req_host_base, uint64_t topk_device_slots, uint64_t export_flags, uint64_t num_real,
+                       uint64_t hot_row_base, uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows,
+                       uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts)
 {
-    (void)channel;
-    KV_REQUIRE_INIT();
-    if (node_num == 0 || node_num > KVOPS_MAX_NODES)
-        return fail(KVOPS_E_INVALID, "export_quant node_num must be in [1, 64]");
-    if (my_node >= node_num) return fail(KVOPS_E_INVALID, "export_quant my_node must be < node_num");
-    uint64_t segs[KVOPS_MAX_NODES] = {0};
-    segs[my_node] = seg_base;
-    return gather_quant_common(node_num, segs, my_node, my_node + 1, my_node, layer_offset_rows, per_layer_seg_rows,
-                               row_format, row_dtype, quant_elems, plain_elems, topk_indices, req_pool_indices,
-                               req_host_base, topk_device_slots, export_flags, num_real, hot_row_base, top_k,
-                               max_num_reqs, stripe_rows, status, stream, block_dim, opts, true);
+    return gather_quant_common(node_num, seg_bases, layer_offset_rows, per_layer_seg_rows, row_format, row_dtype,
+                               quant_elems, plain_elems, topk_indices, req_pool_indices, req_host_base,
+                               topk_device_slots, export_flags, num_real, hot_row_base, top_k, max_num_reqs,
+                               stripe_rows, status, stream, block_dim, opts, true);
 }
 
 int kvops_import_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows,
@@ -797,14 +821,10 @@ int kvops_import_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t la
                        uint64_t hot_row_base, uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows,
                        uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts)
 {
-    KV_REQUIRE_INIT();
-    if (node_num == 0 || node_num > KVOPS_MAX_NODES)
-        return fail(KVOPS_E_INVALID, "import_quant node_num must be in [1, 64]");
-    if (seg_bases == nullptr) return fail(KVOPS_E_INVALID, "import_quant: seg_bases is NULL");
-    return gather_quant_common(node_num, seg_bases, 0, node_num, kvb::kAllNodes, layer_offset_rows,
-                               per_layer_seg_rows, row_format, row_dtype, quant_elems, plain_elems, topk_indices,
-                               req_pool_indices, req_host_base, topk_device_slots, is_miss, num_real, hot_row_base,
-                               top_k, max_num_reqs, stripe_rows, status, stream, block_dim, opts, false);
+    return gather_quant_common(node_num, seg_bases, layer_offset_rows, per_layer_seg_rows, row_format, row_dtype,
+                               quant_elems, plain_elems, topk_indices, req_pool_indices, req_host_base,
+                               topk_device_slots, is_miss, num_real, hot_row_base, top_k, max_num_reqs, stripe_rows,
+                               status, stream, block_dim, opts, false);
 }
 
 int kvops_sieve_update(uint64_t topk_indices, uint64_t req_pool_indices, uint64_t seq_lens, uint64_t prefill_lens,

@@ -111,6 +111,17 @@ struct RowCodec {
     uint32_t plain_elems;  // a multiple of 8
 };
 
+// Export of 16-bit rows of every layer to the stored rows of all segments in one launch.
+struct ExportQuantParams {
+    const uint8_t *src0;
+    uint64_t src_layer_stride;
+    uint64_t units_per_layer;        // rows written per layer: all, or one per stripe (reference map)
+    uint32_t plsr, row_lo, row_cnt, layer_num, stripe, nodes, injective;
+    RowCodec codec;
+    StatusTarget st;
+    uint8_t *seg[kMaxNodes];
+};
+
 // Values that share one scale.
 constexpr uint32_t kQuantGroup = 128;
 
@@ -203,11 +214,11 @@ cudaError_t launch_gather(const GatherParams &p, cudaStream_t s, int sm_count);
 // every position whose flag (p.is_miss) is set.
 cudaError_t launch_scatter(const GatherParams &p, cudaStream_t s, int sm_count);
 cudaError_t launch_export(const ExportParams &p, cudaStream_t s, int sm_count);
-// The same three copies between 16-bit rows and stored rows (quant.cu). p.row_bytes is the
-// stored row's size (the segments' rows); the hot or source rows have codec_row_bytes(c).
+// The copies between 16-bit rows and stored rows (quant.cu). p.row_bytes is the stored row's size (the
+// segments' rows); the hot or source rows have codec_row_bytes(c).
 cudaError_t launch_gather_quant(const GatherParams &p, const RowCodec &c, cudaStream_t s, int sm_count);
 cudaError_t launch_scatter_quant(const GatherParams &p, const RowCodec &c, cudaStream_t s, int sm_count);
-cudaError_t launch_export_quant(const ExportParams &p, const RowCodec &c, cudaStream_t s, int sm_count);
+cudaError_t launch_export_quant(const ExportQuantParams &p, cudaStream_t s, int sm_count);
 // Fused SIEVE step + miss-row gather (one CTA per request). Sets *launched = false, launching
 // nothing, when the request's state and the copy ring do not fit shared memory; the caller
 // then runs launch_sieve_update and launch_gather instead.

@@ -152,33 +152,32 @@ uint32_t quant_row_bytes(const std::string &row_format, const std::string &row_d
     return n;
 }
 
-void export_quant_alllayer(uint64_t channel, uint64_t seg_base, uint32_t per_layer_seg_rows,
+void export_quant_alllayer(const std::vector<uint64_t> &seg_bases, uint32_t per_layer_seg_rows,
                            const std::string &row_format, const std::string &row_dtype, uint32_t quant_elems,
                            uint32_t plain_elems, uint32_t row_lo, uint32_t row_cnt, uint32_t layer_num,
                            uint64_t src_layer0_base, uint64_t src_layer_stride, uint32_t stripe_rows,
-                           uint32_t node_num, uint32_t my_node, uint64_t status, uint64_t stream, uint32_t block_dim,
-                           bool injective, uint64_t err_word)
+                           uint64_t status, uint64_t stream, uint32_t block_dim, bool injective, uint64_t err_word)
 {
     const KvopsRowOpts o = row_opts(0, injective, err_word);
-    check(kvops_export_quant_alllayer(channel, seg_base, per_layer_seg_rows, row_format_of(row_format),
-                                      row_dtype_of(row_dtype), quant_elems, plain_elems, row_lo, row_cnt, layer_num,
-                                      src_layer0_base, src_layer_stride, stripe_rows, node_num, my_node, status,
-                                      stream, block_dim, &o));
+    check(kvops_export_quant_alllayer(static_cast<uint32_t>(seg_bases.size()), seg_bases.data(), per_layer_seg_rows,
+                                      row_format_of(row_format), row_dtype_of(row_dtype), quant_elems, plain_elems,
+                                      row_lo, row_cnt, layer_num, src_layer0_base, src_layer_stride, stripe_rows,
+                                      status, stream, block_dim, &o));
 }
 
-void export_quant(uint64_t channel, uint64_t seg_base, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
+void export_quant(const std::vector<uint64_t> &seg_bases, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
                   const std::string &row_format, const std::string &row_dtype, uint32_t quant_elems,
                   uint32_t plain_elems, uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
                   uint64_t topk_device_slots, uint64_t export_flags, uint64_t num_real, uint64_t hot_row_base,
-                  uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint32_t node_num, uint32_t my_node,
-                  uint64_t status, uint64_t stream, uint32_t block_dim, uint64_t hot_req_stride_rows, bool injective,
-                  uint64_t err_word)
+                  uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint64_t status, uint64_t stream,
+                  uint32_t block_dim, uint64_t hot_req_stride_rows, bool injective, uint64_t err_word)
 {
     const KvopsRowOpts o = row_opts(hot_req_stride_rows, injective, err_word);
-    check(kvops_export_quant(channel, seg_base, layer_offset_rows, per_layer_seg_rows, row_format_of(row_format),
-                             row_dtype_of(row_dtype), quant_elems, plain_elems, topk_indices, req_pool_indices,
-                             req_host_base, topk_device_slots, export_flags, num_real, hot_row_base, top_k,
-                             max_num_reqs, stripe_rows, node_num, my_node, status, stream, block_dim, &o));
+    check(kvops_export_quant(static_cast<uint32_t>(seg_bases.size()), seg_bases.data(), layer_offset_rows,
+                             per_layer_seg_rows, row_format_of(row_format), row_dtype_of(row_dtype), quant_elems,
+                             plain_elems, topk_indices, req_pool_indices, req_host_base, topk_device_slots,
+                             export_flags, num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream,
+                             block_dim, &o));
 }
 
 void import_quant(const std::vector<uint64_t> &seg_bases, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
@@ -335,19 +334,18 @@ PYBIND11_MODULE(_kvops, m)
     // 8-bit stored rows and the attention over the hot rows (not in the reference module).
     m.def("quant_row_bytes", &quant_row_bytes, py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems") = 512,
           py::arg("plain_elems") = 64);
-    m.def("export_quant_alllayer", &export_quant_alllayer, py::arg("channel"), py::arg("seg_base"),
-          py::arg("per_layer_seg_rows"), py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"),
-          py::arg("plain_elems"), py::arg("row_lo"), py::arg("row_cnt"), py::arg("layer_num"),
-          py::arg("src_layer0_base"), py::arg("src_layer_stride"), py::arg("stripe_rows"), py::arg("node_num"),
-          py::arg("my_node"), py::arg("status"), py::arg("stream") = 0, py::arg("block_dim") = 1, py::kw_only(),
-          py::arg("injective") = false, py::arg("err_word") = 0);
-    m.def("export_quant", &export_quant, py::arg("channel"), py::arg("seg_base"), py::arg("layer_offset_rows"),
+    m.def("export_quant_alllayer", &export_quant_alllayer, py::arg("seg_bases"), py::arg("per_layer_seg_rows"),
+          py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"), py::arg("plain_elems"),
+          py::arg("row_lo"), py::arg("row_cnt"), py::arg("layer_num"), py::arg("src_layer0_base"),
+          py::arg("src_layer_stride"), py::arg("stripe_rows"), py::arg("status"), py::arg("stream") = 0,
+          py::arg("block_dim") = 1, py::kw_only(), py::arg("injective") = false, py::arg("err_word") = 0);
+    m.def("export_quant", &export_quant, py::arg("seg_bases"), py::arg("layer_offset_rows"),
           py::arg("per_layer_seg_rows"), py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"),
           py::arg("plain_elems"), py::arg("topk_indices"), py::arg("req_pool_indices"), py::arg("req_host_base"),
           py::arg("topk_device_slots"), py::arg("export_flags"), py::arg("num_real"), py::arg("hot_row_base"),
-          py::arg("top_k"), py::arg("max_num_reqs"), py::arg("stripe_rows"), py::arg("node_num"), py::arg("my_node"),
-          py::arg("status"), py::arg("stream") = 0, py::arg("block_dim") = 1, py::kw_only(),
-          py::arg("hot_req_stride_rows") = 0, py::arg("injective") = false, py::arg("err_word") = 0);
+          py::arg("top_k"), py::arg("max_num_reqs"), py::arg("stripe_rows"), py::arg("status"), py::arg("stream") = 0,
+          py::arg("block_dim") = 1, py::kw_only(), py::arg("hot_req_stride_rows") = 0, py::arg("injective") = false,
+          py::arg("err_word") = 0);
     m.def("import_quant", &import_quant, py::arg("seg_bases"), py::arg("layer_offset_rows"),
           py::arg("per_layer_seg_rows"), py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"),
           py::arg("plain_elems"), py::arg("topk_indices"), py::arg("req_pool_indices"), py::arg("req_host_base"),

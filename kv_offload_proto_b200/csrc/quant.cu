@@ -4,9 +4,9 @@
 //
 // A 1152-byte row and its 656 stored bytes cross memory once, whichever way: the bound is HBM (or
 // the link to the segment). A CTA evaluates a tile of positions, one per thread, into a shared
-// list as rows.cu does, and then takes the listed rows as one flat array of 16-byte units of
-// eight values. A group of 128 values is 16 units, so it always lies in the 16 lanes of a
-// half-warp, whose maximum four shuffles give: the values are read once, from registers to codes.
+// list as rows.cu does, and then takes the listed rows as one flat array of groups of 128 values. A
+// group is 16 units of 16 bytes, one for each lane of a half-warp, which takes eight groups at a
+// time: the values are read once, from registers to codes.
 #include <stdint.h>
 
 #include "kvops_internal.cuh"
@@ -17,7 +17,7 @@ namespace kvb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // units in flight per thread
+constexpr int kUnroll = 4;  // 16-code units in flight per thread, reading
 
 // i / d for the unit indexes of a tile: multiply-high with ceil(2^32 / d), exact while the
 // product of index and divisor is below 2^32 (host-checked), else a division (magic 0).
@@ -38,41 +38,44 @@ __device__ __forceinline__ void cta_copy_plain(const uint8_t *const *src, uint8_
     }
 }
 
-// Quantises n 16-bit rows src[i] into the stored rows dst[i]. Every thread of the CTA calls it.
+// Quantises n 16-bit rows src[i] into the stored rows dst[i]. Every thread of the CTA calls it. magic:
+// of the groups per row.
 template <typename T, typename Code>
 __device__ __forceinline__ void cta_encode_rows(const RowCodec &c, const uint8_t *const *src, uint8_t *const *dst,
                                                 int n, uint32_t magic)
 {
-    const uint32_t units = c.quant_elems / 8;
-    const uint32_t total = static_cast<uint32_t>(n) * units;
-    const uint32_t rounds = (total + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-    for (uint32_t it = 0; it < rounds; ++it) {
-        uint4 v[kUnroll];
-        uint32_t row[kUnroll], unit[kUnroll];
+    const uint32_t per_row = c.quant_elems / kQuantGroup, total = static_cast<uint32_t>(n) * per_row;
+    const int lane = threadIdx.x & 15;
+    for (uint32_t g0 = threadIdx.x / 32 * 16; g0 < total; g0 += kThreads / 16 * 8) {  // (uniform over the warp)
+        const uint32_t mine = g0 + (threadIdx.x >> 4 & 1) * 8;
+        uint4 v[8];
+        uint32_t row[8], group[8];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            const uint32_t i = (it * kUnroll + k) * kThreads + threadIdx.x;
-            row[k] = div_magic(i, units, magic);
-            unit[k] = i - row[k] * units;
+        for (int k = 0; k < 8; ++k) {
+            row[k] = div_magic(mine + k, per_row, magic);
+            group[k] = mine + k - row[k] * per_row;
             v[k] = make_uint4(0u, 0u, 0u, 0u);
-            if (i < total) v[k] = load_stream(reinterpret_cast<const uint4 *>(src[row[k]]) + unit[k]);
+            if (mine + k < total) v[k] = load_stream(reinterpret_cast<const uint4 *>(src[row[k]]) + group[k] * 16 + lane);
         }
+        uint2 codes[8];
+        float scale;
+        encode_groups<T, Code>(v, lane, codes, &scale);
+        uint8_t *at = nullptr;  // this lane's group's scale
+        uint32_t at_group = 0;
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            // total is a multiple of 16: a half-warp's lanes are all inside or all outside, and
-            // every lane takes part in the shuffles.
-            float scale;
-            const uint2 codes = encode_unit<T, Code>(v[k], &scale);
-            if ((it * kUnroll + k) * kThreads + threadIdx.x < total) {
-                uint8_t *d = dst[row[k]];
-                reinterpret_cast<uint2 *>(d)[unit[k]] = codes;
-                if ((unit[k] & 15u) == 0) {
-                    float *scales = reinterpret_cast<float *>(d + c.quant_elems);
-                    scales[unit[k] / 16] = scale;
-                    if (unit[k] + 16 == units)  // the padding, as zeros
-                        for (uint32_t g = units / 16; g < codec_scale_bytes(c) / 4; ++g) scales[g] = 0.f;
-                }
+        for (int k = 0; k < 8; ++k) {
+            if (mine + k >= total) continue;
+            uint8_t *d = dst[row[k]];
+            reinterpret_cast<uint2 *>(d)[group[k] * 16 + lane] = codes[k];
+            if (scale_group(lane) == k && (lane & 1) == 0) {
+                at = d + c.quant_elems;
+                at_group = group[k];
             }
+        }
+        if (at != nullptr) {
+            reinterpret_cast<float *>(at)[at_group] = scale;
+            if (at_group + 1 == per_row)  // the padding, as zeros
+                for (uint32_t g = per_row; g < codec_scale_bytes(c) / 4; ++g) reinterpret_cast<float *>(at)[g] = 0.f;
         }
     }
     cta_copy_plain(src, dst, n, c.plain_elems / 8, 2 * c.quant_elems, c.quant_elems + codec_scale_bytes(c));
@@ -83,10 +86,11 @@ template <typename T, typename Code>
 __device__ __forceinline__ void cta_decode_rows(const RowCodec &c, const uint8_t *const *src, uint8_t *const *dst,
                                                 int n, uint32_t magic)
 {
-    const uint32_t units = c.quant_elems / 8;
+    // units of 16 codes, eight to a group
+    const uint32_t units = c.quant_elems / 16;
     const uint32_t total = static_cast<uint32_t>(n) * units;
     for (uint32_t i0 = threadIdx.x; i0 < total; i0 += kThreads * kUnroll) {
-        uint2 v[kUnroll];
+        uint4 v[kUnroll];
         float scale[kUnroll];
         uint32_t row[kUnroll], unit[kUnroll];
 #pragma unroll
@@ -96,14 +100,17 @@ __device__ __forceinline__ void cta_decode_rows(const RowCodec &c, const uint8_t
             unit[k] = i - row[k] * units;
             if (i < total) {
                 const uint8_t *s = src[row[k]];
-                v[k] = load_stream(reinterpret_cast<const uint2 *>(s) + unit[k]);
-                scale[k] = *reinterpret_cast<const volatile float *>(s + c.quant_elems + unit[k] / 16 * 4);
+                v[k] = load_stream(reinterpret_cast<const uint4 *>(s) + unit[k]);
+                scale[k] = *reinterpret_cast<const volatile float *>(s + c.quant_elems + unit[k] / 8 * 4);
             }
         }
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k) {
-            if (i0 + k * kThreads < total)
-                reinterpret_cast<uint4 *>(dst[row[k]])[unit[k]] = decode_unit<T, Code>(v[k], scale[k]);
+            if (i0 + k * kThreads < total) {
+                uint4 *d = reinterpret_cast<uint4 *>(dst[row[k]]) + 2 * unit[k];
+                d[0] = decode_unit<T, Code>(make_uint2(v[k].x, v[k].y), scale[k]);
+                d[1] = decode_unit<T, Code>(make_uint2(v[k].z, v[k].w), scale[k]);
+            }
         }
     }
     cta_copy_plain(src, dst, n, c.plain_elems / 8, c.quant_elems + codec_scale_bytes(c), 2 * c.quant_elems);
@@ -154,14 +161,12 @@ __global__ void __launch_bounds__(kThreads, 4) gather_quant_kernel(const GatherP
 }
 
 template <typename T, typename Code>
-__global__ void __launch_bounds__(kThreads, 4) export_quant_kernel(const ExportParams p, const RowCodec c,
-                                                                   uint32_t tile, uint32_t magic)
+__global__ void __launch_bounds__(kThreads, 4) export_quant_kernel(const ExportQuantParams p, uint32_t tile, uint32_t magic)
 {
     __shared__ const uint8_t *s_src[kThreads];
     __shared__ uint8_t *s_dst[kThreads];
     __shared__ int s_n;
     const uint64_t total = p.units_per_layer * p.layer_num;
-    if (p.seg_null && blockIdx.x == 0 && threadIdx.x == 0) record_error(p.st, KVOPS_ERR_SEG_NULL);
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
     for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * tile; base < total;
@@ -171,23 +176,30 @@ __global__ void __launch_bounds__(kThreads, 4) export_quant_kernel(const ExportP
         const uint8_t *src = nullptr;
         uint8_t *dst = nullptr;
         if (threadIdx.x < tile && u < total) {
-            const uint64_t l = u / p.units_per_layer;
-            const uint64_t k = u - l * p.units_per_layer;
-            uint32_t src_row, seg_row;
-            if (export_unit(p, k, &src_row, &seg_row)) {
-                if (seg_row >= p.plsr) {
-                    const uint64_t idx = l * p.row_cnt + (src_row - p.row_lo);
-                    record_error(p.st, KVOPS_ERR_ROW_BASE + static_cast<uint32_t>(idx & 0xFFu) + (1u << 16));
-                } else {
-                    src = p.src0 + l * p.src_layer_stride + static_cast<uint64_t>(src_row) * codec_row_bytes(c);
-                    dst = p.seg + (l * p.plsr + seg_row) * static_cast<uint64_t>(p.row_bytes);
-                    ok = true;
-                }
+            const uint64_t l = u / p.units_per_layer, k = u - l * p.units_per_layer;
+            // Unit k is the k-th row, or (reference map) the last row in range of the k-th stripe, the
+            // one that the reference's ascending per-row writes leave in the shared segment row.
+            uint64_t row = p.row_lo + k;
+            if (p.stripe > 0 && !p.injective) {
+                const uint64_t end = (p.row_lo / p.stripe + k + 1) * p.stripe, hi = static_cast<uint64_t>(p.row_lo) + p.row_cnt;
+                row = (end < hi ? end : hi) - 1;
+            }
+            const uint32_t r = static_cast<uint32_t>(row);
+            const uint32_t node = node_of(r, p.stripe, p.nodes), seg_row = seg_row_of(r, p.stripe, p.nodes, p.injective != 0);
+            if (p.seg[node] == nullptr) {
+                record_error(p.st, KVOPS_ERR_SEG_NULL);
+            } else if (seg_row >= p.plsr) {
+                record_error(p.st, KVOPS_ERR_ROW_BASE + static_cast<uint32_t>((l * p.row_cnt + (row - p.row_lo)) & 0xFFu) +
+                                       (1u << 16));
+            } else {
+                src = p.src0 + l * p.src_layer_stride + row * codec_row_bytes(p.codec);
+                dst = p.seg[node] + (l * p.plsr + seg_row) * static_cast<uint64_t>(codec_stored_bytes(p.codec));
+                ok = true;
             }
         }
         list_append(ok, src, dst, s_src, s_dst, &s_n);
         __syncthreads();
-        cta_encode_rows<T, Code>(c, s_src, s_dst, s_n, magic);
+        cta_encode_rows<T, Code>(p.codec, s_src, s_dst, s_n, magic);
         __syncthreads();
         if (threadIdx.x == 0) s_n = 0;
         __syncthreads();
@@ -196,31 +208,35 @@ __global__ void __launch_bounds__(kThreads, 4) export_quant_kernel(const ExportP
     if (threadIdx.x == 0) arrive_and_publish(p.st);
 }
 
-// Positions per tile (at most one per thread), grid and division constant of a launch.
+// Positions per tile (at most one per thread) and grid of a launch: tiles of `most` positions, or smaller
+// ones where those leave CTAs without any.
 struct Shape {
-    uint32_t tile, magic;
+    uint32_t tile;
     int grid;
 };
 
-Shape shape_of(uint64_t positions, const RowCodec &c, int sm_count)
+Shape shape_of(uint64_t positions, uint32_t most, int sm_count)
 {
     Shape s;
     const uint64_t cap = static_cast<uint64_t>(sm_count > 0 ? sm_count : 148) * 4;
-    s.tile = kThreads;
-    while (s.tile > 32 && positions < cap * s.tile * 4) s.tile /= 2;
+    s.tile = most;
+    while (s.tile > 16 && positions <= cap * (s.tile / 2)) s.tile /= 2;
     const uint64_t tiles = (positions + s.tile - 1) / s.tile;
     s.grid = static_cast<int>(tiles < 1 ? 1 : (tiles < cap ? tiles : cap));
-    const uint64_t units = c.quant_elems / 8;
-    // indexes run up to one round past the last unit of a tile
-    s.magic = units * (s.tile * units + kThreads * kUnroll) < (1ull << 32)
-                  ? static_cast<uint32_t>(((1ull << 32) + units - 1) / units) : 0u;
     return s;
+}
+
+// The multiplier of div_magic for indexes up to one round past a tile's last, or 0.
+uint32_t magic_of(uint64_t d)
+{
+    return d * (kThreads * d + kThreads * 8) < (1ull << 32) ? static_cast<uint32_t>(((1ull << 32) + d - 1) / d) : 0u;
 }
 
 template <typename T, typename Code>
 cudaError_t launch_gather_as(const GatherParams &p, const RowCodec &c, bool write, cudaStream_t s, int sm_count)
 {
-    const Shape sh = shape_of(static_cast<uint64_t>(p.max_num_reqs) * p.top_k, c, sm_count);
+    const Shape sh = shape_of(static_cast<uint64_t>(p.max_num_reqs) * p.top_k, kThreads, sm_count);
+    const uint32_t magic = magic_of(write ? c.quant_elems / kQuantGroup : c.quant_elems / 16);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(sh.grid);
     cfg.blockDim = dim3(kThreads);
@@ -230,15 +246,15 @@ cudaError_t launch_gather_as(const GatherParams &p, const RowCodec &c, bool writ
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return write ? cudaLaunchKernelEx(&cfg, gather_quant_kernel<T, Code, true>, p, c, sh.tile, sh.magic)
-                 : cudaLaunchKernelEx(&cfg, gather_quant_kernel<T, Code, false>, p, c, sh.tile, sh.magic);
+    return write ? cudaLaunchKernelEx(&cfg, gather_quant_kernel<T, Code, true>, p, c, sh.tile, magic)
+                 : cudaLaunchKernelEx(&cfg, gather_quant_kernel<T, Code, false>, p, c, sh.tile, magic);
 }
 
 template <typename T, typename Code>
-cudaError_t launch_export_as(const ExportParams &p, const RowCodec &c, cudaStream_t s, int sm_count)
+cudaError_t launch_export_as(const ExportQuantParams &p, cudaStream_t s, int sm_count)
 {
-    const Shape sh = shape_of(p.units_per_layer * p.layer_num, c, sm_count);
-    export_quant_kernel<T, Code><<<sh.grid, kThreads, 0, s>>>(p, c, sh.tile, sh.magic);
+    const Shape sh = shape_of(p.units_per_layer * p.layer_num, kThreads / 2, sm_count);
+    export_quant_kernel<T, Code><<<sh.grid, kThreads, 0, s>>>(p, sh.tile, magic_of(p.codec.quant_elems / kQuantGroup));
     return cudaGetLastError();
 }
 
@@ -264,12 +280,12 @@ cudaError_t launch_scatter_quant(const GatherParams &p, const RowCodec &c, cudaS
     return launch_gather_any(p, c, true, s, sm_count);
 }
 
-cudaError_t launch_export_quant(const ExportParams &p, const RowCodec &c, cudaStream_t s, int sm_count)
+cudaError_t launch_export_quant(const ExportQuantParams &p, cudaStream_t s, int sm_count)
 {
-    const bool e4m3 = c.format == KVOPS_ROW_E4M3;
-    if (c.dtype == KVOPS_DTYPE_FP16)
-        return e4m3 ? launch_export_as<Fp16, E4m3>(p, c, s, sm_count) : launch_export_as<Fp16, Int8>(p, c, s, sm_count);
-    return e4m3 ? launch_export_as<Bf16, E4m3>(p, c, s, sm_count) : launch_export_as<Bf16, Int8>(p, c, s, sm_count);
+    const bool e4m3 = p.codec.format == KVOPS_ROW_E4M3;
+    if (p.codec.dtype == KVOPS_DTYPE_FP16)
+        return e4m3 ? launch_export_as<Fp16, E4m3>(p, s, sm_count) : launch_export_as<Fp16, Int8>(p, s, sm_count);
+    return e4m3 ? launch_export_as<Bf16, E4m3>(p, s, sm_count) : launch_export_as<Bf16, Int8>(p, s, sm_count);
 }
 
 }  // namespace kvb

@@ -85,39 +85,56 @@ struct Int8 {
     }
 };
 
-// Eight 16-bit values (one 16-byte unit) -> eight codes and, in every lane of the 16 that hold the
-// group, its scale. Lanes of a half-warp hold the 16 units of one group in order.
+// Eight groups of 128 values at once, by the 16 lanes of a half-warp: lane l has unit l (16 bytes, eight
+// values) of each group in v[0..7], and gets its codes; scale is that of group scale_group(l).
+// The eight maxima are reduced together, each step halving what a lane still holds, so that one lane
+// (of two) ends up with one group's maximum and the two divisions are done once for eight groups: they
+// and 32 shuffles a lane would otherwise cost more than the rest.
+__device__ __forceinline__ int scale_group(int lane) { return (lane >> 1) & 7; }
 template <typename T, typename Code>
-__device__ __forceinline__ uint2 encode_unit(const uint4 &v, float *scale)
+__device__ __forceinline__ void encode_groups(const uint4 (&v)[8], int lane, uint2 (&codes)[8], float *scale)
 {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    // The largest magnitude by its bits, which order like the values and put inf and NaN on top.
-    uint32_t m = 0;
+    // The largest magnitudes by their bits, which order like the values and put inf and NaN on top.
+    uint32_t m[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t p = __vmaxu2(__vmaxu2(v[k].x & 0x7FFF7FFFu, v[k].y & 0x7FFF7FFFu),
+                                    __vmaxu2(v[k].z & 0x7FFF7FFFu, v[k].w & 0x7FFF7FFFu));
+        m[k] = max(p & 0xFFFFu, p >> 16);
+    }
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    const uint32_t top = max(m & 0xFFFFu, m >> 16);
+    for (int w = 4; w > 0; w /= 2) {  // bit 2 w of the lane takes the upper half of the groups
+#pragma unroll
+        for (int k = 0; k < w; ++k) {
+            const bool up = (lane & (2 * w)) != 0;
+            const uint32_t give = up ? m[k] : m[k + w], keep = up ? m[k + w] : m[k];
+            m[k] = max(keep, __shfl_xor_sync(0xFFFFFFFFu, give, 2 * w));
+        }
+    }
+    const uint32_t top = max(m[0], __shfl_xor_sync(0xFFFFFFFFu, m[0], 1));
     const float a = T::unpack(top).x;
     float inv = 0.f;
+    *scale = 0.f;
     if (top >= T::kInf) {
         *scale = __int_as_float(0x7FC00000);
-        return make_uint2(0u, 0u);
+    } else if (a >= 0x1p-100f) {
+        inv = __fdiv_rn(Code::kMax, a);
+        *scale = __fdiv_rn(a, Code::kMax);
     }
-    if (a < 0x1p-100f) {
-        *scale = 0.f;
-        return make_uint2(0u, 0u);
-    }
-    inv = __fdiv_rn(Code::kMax, a);
-    *scale = __fdiv_rn(a, Code::kMax);
-    float x[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = T::unpack(w[i]);
-        x[2 * i] = __fmul_rn(f.x, inv);
-        x[2 * i + 1] = __fmul_rn(f.y, inv);
+    for (int k = 0; k < 8; ++k) {
+        const float f = __shfl_sync(0xFFFFFFFFu, inv, 2 * k, 16);
+        const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = T::unpack(w[i]);
+            x[2 * i] = __fmul_rn(p.x, f);
+            x[2 * i + 1] = __fmul_rn(p.y, f);
+        }
+        codes[k] = make_uint2(Code::encode4(x[0], x[1], x[2], x[3]), Code::encode4(x[4], x[5], x[6], x[7]));
+        if (f == 0.f) codes[k] = make_uint2(0u, 0u);  // (no product of 0 and inf or NaN, no negative zeros)
     }
-    return make_uint2(Code::encode4(x[0], x[1], x[2], x[3]), Code::encode4(x[4], x[5], x[6], x[7]));
 }
 
 // Eight codes -> the eight 16-bit values they stand for.

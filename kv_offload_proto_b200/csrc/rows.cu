@@ -48,6 +48,34 @@ __global__ void __launch_bounds__(kRowThreads, 4) gather_kernel(const GatherPara
     if (threadIdx.x == 0) arrive_and_publish(p.st);
 }
 
+// Destination unit k of one layer -> (source row, segment row); false if outside the range.
+// Reference map with S > 1: unit k is the k-th owned stripe and only its last row in range is
+// copied, because the reference's ascending per-row writes leave exactly that row in the
+// shared segment row (kvc_scatter_rows_alllayer.cpp:34-53).
+__device__ __forceinline__ bool export_unit(const ExportParams &p, uint64_t k, uint32_t *src_row, uint32_t *seg_row)
+{
+    const uint64_t lo = p.row_lo, hi = static_cast<uint64_t>(p.row_lo) + p.row_cnt - 1;
+    if (p.stripe == 0) {
+        *src_row = static_cast<uint32_t>(lo + k);
+        *seg_row = *src_row;
+        return true;
+    }
+    const uint64_t S = p.stripe;
+    if (!p.injective) {
+        const uint64_t g = p.g_first + k * p.nodes;
+        const uint64_t last = (g + 1) * S - 1;
+        *src_row = static_cast<uint32_t>(last < hi ? last : hi);
+        *seg_row = static_cast<uint32_t>(g / p.nodes);
+        return true;
+    }
+    const uint64_t g = p.g_first + (k / S) * p.nodes;
+    const uint64_t r = g * S + k % S;
+    if (r < lo || r > hi) return false;
+    *src_row = static_cast<uint32_t>(r);
+    *seg_row = static_cast<uint32_t>((g / p.nodes) * S + k % S);
+    return true;
+}
+
 template <typename V>
 __global__ void __launch_bounds__(kRowThreads, 4) export_kernel(const ExportParams p, uint32_t magic)
 {

@@ -318,18 +318,18 @@ class DevicePool:
                     num_real, hot_row_base, max_num_reqs, top_k, stream=0, block_dim=1, *, hot_req_stride_rows=0) -> int:
         """Export one layer's flagged hot rows to their pool rows (kvc_scatter_rows, the single-layer
         decode-increment export of doc/kv_offload_design.md:394-396): batch_read's arguments and
-        rules in the opposite direction, one launch per segment. Returns the status address."""
+        rules in the opposite direction, one launch per segment (one for all, where rows are
+        quantised on the way). Returns the status address."""
         status = self.next_status()
         off = layer_id * self.per_layer_seg_rows
         a = [_ptr(topk_indices), _ptr(req_pool_indices), _ptr(req_host_base), _ptr(topk_device_slots),
              _ptr(export_flags), _ptr(num_real), _ptr(hot_row_base)]
+        if self._hot_codec is not None:
+            self._k.export_quant(self.seg_bases, off, self.per_layer_seg_rows, *self._hot_codec, *a, top_k,
+                                 max_num_reqs, self.stripe_rows, status, stream, block_dim,
+                                 hot_req_stride_rows=hot_req_stride_rows, injective=self.injective)
+            return status
         for s in range(self.node_num):
-            if self._hot_codec is not None:
-                self._k.export_quant(self.channels[s], self.seg_bases[s], off, self.per_layer_seg_rows,
-                                     *self._hot_codec, *a, top_k, max_num_reqs, self.stripe_rows, self.node_num, s,
-                                     status, stream, block_dim, hot_req_stride_rows=hot_req_stride_rows,
-                                     injective=self.injective)
-                continue
             self._k.export_seg(self.channels[s], self.seg_bases[s], off, self.per_layer_seg_rows, self.seg_row_bytes, *a,
                                top_k, max_num_reqs, self.stripe_rows, self.node_num, s, status, stream, block_dim,
                                hot_req_stride_rows=hot_req_stride_rows, injective=self.injective)
@@ -337,15 +337,15 @@ class DevicePool:
 
     def batch_write_alllayers(self, row_lo, row_cnt, src_layer0_base, src_layer_stride, stream=0, block_dim=1) -> int:
         """Export rows [row_lo, row_lo+row_cnt) of every layer to their segments
-        (xds_ems_pool.py:220-230): one launch per segment, as in the reference."""
+        (xds_ems_pool.py:220-230): one launch per segment, as in the reference (one for all segments
+        where rows are stored in 8 bits)."""
         status = self.next_status()
+        if self._codec is not None:
+            self._k.export_quant_alllayer(self.seg_bases, self.per_layer_seg_rows, *self._codec, row_lo, row_cnt,
+                                          self.layer_num, _ptr(src_layer0_base), src_layer_stride, self.stripe_rows,
+                                          status, stream, block_dim, injective=self.injective)
+            return status
         for s in range(self.node_num):
-            if self._codec is not None:
-                self._k.export_quant_alllayer(self.channels[s], self.seg_bases[s], self.per_layer_seg_rows,
-                                              *self._codec, row_lo, row_cnt, self.layer_num, _ptr(src_layer0_base),
-                                              src_layer_stride, self.stripe_rows, self.node_num, s, status, stream,
-                                              block_dim, injective=self.injective)
-                continue
             self._k.export_seg_alllayer(self.channels[s], self.seg_bases[s], self.per_layer_seg_rows, self.row_bytes,
                                         row_lo, row_cnt, self.layer_num, _ptr(src_layer0_base), src_layer_stride,
                                         self.stripe_rows, self.node_num, s, status, stream, block_dim,

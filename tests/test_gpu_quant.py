@@ -48,9 +48,8 @@ def test_export_alllayer_bytes(fmt, dtype, quant, plain, N, S, injective, lo, cn
     segs = [dev(w) for w in want]
     src = rows.cuda()
     status = mod.alloc_status(8 * N)
-    for n in range(N):
-        mod.export_quant_alllayer(0, segs[n].data_ptr(), plsr, fmt, dtype, quant, plain, lo, cnt, layers,
-                                  src.data_ptr(), src.stride(0) * 2, S, N, n, status, 0, 1, injective=injective)
+    mod.export_quant_alllayer([s.data_ptr() for s in segs], plsr, fmt, dtype, quant, plain, lo, cnt, layers,
+                              src.data_ptr(), src.stride(0) * 2, S, status, 0, 1, injective=injective)
     for n in range(N):
         assert mod.poll_status(status + 64 * n, 10_000_000) == 0
     torch.cuda.synchronize()
@@ -91,9 +90,9 @@ def test_single_rows_written_and_read_back(fmt, dtype, quant, plain, N, S, R, K,
     a = [dev(x) for x in (topk, req, base, slots, flags, np.array([num_real], np.int32))]
     ptrs = [x.data_ptr() for x in a]
     status = mod.alloc_status(8 * N)
+    mod.export_quant([s.data_ptr() for s in segs], plsr, plsr, fmt, dtype, quant, plain, *ptrs, hot.data_ptr(), K, R, S,
+                     status, 0, 1, hot_req_stride_rows=dbs, injective=True)
     for n in range(N):
-        mod.export_quant(0, segs[n].data_ptr(), plsr, plsr, fmt, dtype, quant, plain, *ptrs, hot.data_ptr(), K, R, S, N,
-                         n, status, 0, 1, hot_req_stride_rows=dbs, injective=True)
         assert mod.poll_status(status + 64 * n, 10_000_000) == 0
     err = torch.zeros(1, dtype=torch.int32, device="cuda")
     mod.import_quant([s.data_ptr() for s in segs], plsr, plsr, fmt, dtype, quant, plain, *ptrs, back.data_ptr(), K, R,
@@ -125,8 +124,7 @@ def test_nonfinite_groups_read_back_as_nan():
     rows[1, 511] = float("nan")
     src, seg = rows.cuda(), torch.zeros(3 * 656, dtype=torch.uint8, device="cuda")
     status = mod.alloc_status(8)
-    mod.export_quant_alllayer(0, seg.data_ptr(), 3, "int8", "fp16", 512, 64, 0, 3, 1, src.data_ptr(), 3 * 1152, 1, 1, 0,
-                              status)
+    mod.export_quant_alllayer([seg.data_ptr()], 3, "int8", "fp16", 512, 64, 0, 3, 1, src.data_ptr(), 3 * 1152, 1, status)
     assert mod.poll_status(status, 10_000_000) == 0
     a = [dev(x) for x in (np.arange(3, dtype=np.int32)[None], np.zeros(1, np.int64), np.zeros(1, np.int64),
                           np.arange(3, dtype=np.int32)[None], np.ones((1, 3), np.int8), np.ones(1, np.int32))]
@@ -153,11 +151,11 @@ def test_errcodes_and_refusals():
     assert mod.poll_status(status, 10_000_000) == 0x101
     mod.import_quant([seg.data_ptr()], 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, status)
     assert mod.poll_status(status, 10_000_000) & 0xFF00 == 0x200
-    mod.export_quant(0, seg.data_ptr(), 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, 1, 0, status)
+    mod.export_quant([seg.data_ptr()], 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, status)
     assert mod.poll_status(status, 10_000_000) & 0xFF00 == 0x200
-    mod.export_quant_alllayer(0, 0, 2, *codec, 0, 2, 1, hot.data_ptr(), 0, 1, 1, 0, status)
+    mod.export_quant_alllayer([0], 2, *codec, 0, 2, 1, hot.data_ptr(), 0, 1, status)
     assert mod.poll_status(status, 10_000_000) == 0x101
-    mod.export_quant_alllayer(0, seg.data_ptr(), 2, *codec, 0, 4, 1, hot.data_ptr(), 0, 1, 1, 0, status)
+    mod.export_quant_alllayer([seg.data_ptr()], 2, *codec, 0, 4, 1, hot.data_ptr(), 0, 1, status)
     assert mod.poll_status(status, 10_000_000) & 0xFF00 == 0x200
     for call, message in [
         (lambda: mod.import_quant([seg.data_ptr() + 8], 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, 0), "16-byte"),
@@ -166,14 +164,14 @@ def test_errcodes_and_refusals():
          "quant_elems"),
         (lambda: mod.import_quant([], 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, 0), "node_num"),
         (lambda: mod.import_quant([seg.data_ptr()], 0, 2, *codec, 0, *p[1:], hot.data_ptr(), 4, 1, 1, 0), "address is 0"),
-        (lambda: mod.export_quant(0, seg.data_ptr(), 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, 1, 1, 0), "my_node"),
-        (lambda: mod.export_quant(0, seg.data_ptr(), 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, 1, 0, 0, 0, 9),
-         "blockDim"),
-        (lambda: mod.export_quant_alllayer(0, seg.data_ptr(), 2, *codec, 0, 2, 1, hot.data_ptr() + 2, 0, 1, 1, 0, 0),
-         "16-byte"),
-        (lambda: mod.export_quant_alllayer(0, seg.data_ptr(), 2, *codec, 0, 2, 2, hot.data_ptr(), 1160, 1, 1, 0, 0),
-         "16-byte"),
-        (lambda: mod.export_quant_alllayer(0, seg.data_ptr(), 2, *codec, 0, 2, 1, 0, 0, 1, 1, 0, 0), "address is 0"),
+        (lambda: mod.export_quant([0] * 65, 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, 0), "node_num"),
+        (lambda: mod.export_quant([seg.data_ptr()], 0, 2, *codec, *p, hot.data_ptr(), 4, 1, 1, 0, 0, 9), "blockDim"),
+        (lambda: mod.export_quant_alllayer([], 2, *codec, 0, 2, 1, hot.data_ptr(), 0, 1, 0), "node_num"),
+        (lambda: mod.export_quant_alllayer([seg.data_ptr()], 2, *codec, 0, 2, 1, hot.data_ptr(), 0, 1, 0, 0, 9), "blockDim"),
+        (lambda: mod.export_quant_alllayer([seg.data_ptr()], 2, *codec, 0, 2, 1, hot.data_ptr() + 2, 0, 1, 0), "16-byte"),
+        (lambda: mod.export_quant_alllayer([seg.data_ptr()], 2, *codec, 0, 2, 2, hot.data_ptr(), 1160, 1, 0), "16-byte"),
+        (lambda: mod.export_quant_alllayer([seg.data_ptr()], 2, *codec, 0, 2, 1, 0, 0, 1, 0), "address is 0"),
+        (lambda: mod.export_quant_alllayer([seg.data_ptr()], 2, *codec, 2 ** 32 - 1, 2, 1, hot.data_ptr(), 0, 1, 0), "32-bit"),
     ]:
         with pytest.raises(RuntimeError, match=message):
             call()
@@ -252,7 +250,7 @@ def test_rows_beyond_four_gigabytes():
                           np.ones((2, 1), np.int8), np.array([2], np.int32))]
     p = [x.data_ptr() for x in a]
     status = mod.alloc_status(8)
-    mod.export_quant(0, seg.data_ptr(), 0, 6_700_001, "e4m3", "bf16", 512, 64, *p, hot.data_ptr(), 1, 2, 1, 1, 0, status,
+    mod.export_quant([seg.data_ptr()], 0, 6_700_001, "e4m3", "bf16", 512, 64, *p, hot.data_ptr(), 1, 2, 1, status,
                      hot_req_stride_rows=1_000_000)
     assert mod.poll_status(status, 10_000_000) == 0
     enc = quant_model.encode(rows, "e4m3", 512)

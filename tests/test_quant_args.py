@@ -37,9 +37,9 @@ def test_codec_refusals(args, message):
 def test_calls_before_init_raise():
     mod = kp.kvops()
     with pytest.raises(RuntimeError, match="kvops not inited"):
-        mod.export_quant_alllayer(0, 0, 0, "e4m3", "fp16", 512, 64, *([0] * 9))
+        mod.export_quant_alllayer([0], 0, "e4m3", "fp16", 512, 64, *([0] * 7))
     with pytest.raises(RuntimeError, match="kvops not inited"):
-        mod.export_quant(0, 0, 0, 0, "e4m3", "fp16", 512, 64, *([0] * 13))
+        mod.export_quant([0], 0, 0, "e4m3", "fp16", 512, 64, *([0] * 11))
     with pytest.raises(RuntimeError, match="kvops not inited"):
         mod.import_quant([0], 0, 0, "e4m3", "fp16", 512, 64, *([0] * 11))
     with pytest.raises(RuntimeError, match="kvops not inited"):
