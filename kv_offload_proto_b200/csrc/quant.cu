@@ -3,10 +3,16 @@
 // segments, kvops_import_quant reads the miss rows back into 16-bit hot rows.
 //
 // A 1152-byte row and its 656 stored bytes cross memory once, whichever way: the bound is HBM (or
-// the link to the segment). A CTA evaluates a tile of positions, one per thread, into a shared
-// list as rows.cu does, and then takes the listed rows as one flat array of groups of 128 values. A
-// group is 16 units of 16 bytes, one for each lane of a half-warp, which takes eight groups at a
-// time: the values are read once, from registers to codes.
+// the link to the segment).
+// Writing, a warp takes a tile of positions, one per lane, lists the rows it found in shared memory, and
+// takes them as one flat array of groups of 128 values: 16 units of 16 bytes, one for each lane of a
+// half-warp, which takes eight groups at a time, so that values are read once, from registers to codes.
+// No two warps wait for each other. 8192 rows of 61 layers, 903 MB: 189 us, 4.8 TB/s. The instructions
+// were 63% of the issue slots with an address for each group; hence four groups to an address.
+// Reading, a CTA takes a tile, as rows.cu does, since few positions may be misses, and 16 codes (32
+// bytes) a thread at a time. 262,144 of 524,288 positions, 479 MB: 127 us, 3.8 TB/s; copying as many rows
+// of these sizes from and to random places, without any rule or arithmetic, takes 98 us. (A warp a tile:
+// 136 us; the next tile's positions loaded ahead: 136 us; the memory is the limit, not the waits.)
 #include <stdint.h>
 
 #include "kvops_internal.cuh"
@@ -17,7 +23,8 @@ namespace kvb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;  // 16-code units in flight per thread, reading
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;  // 16-byte units in flight per thread
 
 // i / d for the unit indexes of a tile: multiply-high with ceil(2^32 / d), exact while the
 // product of index and divisor is below 2^32 (host-checked), else a division (magic 0).
@@ -26,156 +33,213 @@ __device__ __forceinline__ uint32_t div_magic(uint32_t i, uint32_t d, uint32_t m
     return magic ? __umulhi(i, magic) : i / d;
 }
 
-// Copies the 16-byte units [0, units) of n rows (src[i] + src_off -> dst[i] + dst_off).
-__device__ __forceinline__ void cta_copy_plain(const uint8_t *const *src, uint8_t *const *dst, int n, uint32_t units,
-                                               uint32_t src_off, uint32_t dst_off)
+// The multipliers for a row's groups (writing) or units of 16 codes (reading), and for its plain units.
+struct Magics {
+    uint32_t quant, plain;
+};
+
+// The rows that a group of kGroup threads (a warp, or the CTA) takes: src[i] -> dst[i].
+template <int kGroup>
+struct List {
+    const uint8_t *src[kGroup];
+    uint8_t *dst[kGroup];
+};
+
+// Lists the accepted rows of the lanes; returns how many.
+__device__ __forceinline__ int list_rows(List<32> &list, bool ok, const uint8_t *src, uint8_t *dst, int lane)
 {
-    const uint32_t total = static_cast<uint32_t>(n) * units;
-    for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
-        const uint32_t r = i / units, u = i - r * units;
-        const uint4 v = load_stream(reinterpret_cast<const uint4 *>(src[r] + src_off) + u);
-        reinterpret_cast<uint4 *>(dst[r] + dst_off)[u] = v;
+    const unsigned mask = __ballot_sync(0xFFFFFFFFu, ok);
+    const int at = __popc(mask & ((1u << lane) - 1u));
+    __syncwarp();  // the rows listed before have been read
+    if (ok) {
+        list.src[at] = src;
+        list.dst[at] = dst;
+    }
+    __syncwarp();
+    return __popc(mask);
+}
+
+// Copies the rows' plain parts, `units` of 16 bytes each.
+template <int kGroup>
+__device__ __forceinline__ void copy_plain(const List<kGroup> &list, int n, uint32_t units, uint32_t magic,
+                                           uint32_t src_at, uint32_t dst_at, int thread)
+{
+    const uint32_t total = n * units;
+    for (uint32_t i0 = thread; i0 < total; i0 += kGroup * kUnroll) {
+        uint4 v[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const uint32_t i = i0 + k * kGroup, row = div_magic(i, units, magic);
+            if (i < total) v[k] = load_stream(reinterpret_cast<const uint4 *>(list.src[row] + src_at) + (i - row * units));
+        }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const uint32_t i = i0 + k * kGroup, row = div_magic(i, units, magic);
+            if (i < total) reinterpret_cast<uint4 *>(list.dst[row] + dst_at)[i - row * units] = v[k];
+        }
     }
 }
 
-// Quantises n 16-bit rows src[i] into the stored rows dst[i]. Every thread of the CTA calls it. magic:
-// of the groups per row.
-template <typename T, typename Code>
-__device__ __forceinline__ void cta_encode_rows(const RowCodec &c, const uint8_t *const *src, uint8_t *const *dst,
-                                                int n, uint32_t magic)
+// Quantises n listed 16-bit rows into stored rows. kRun groups of a row share its addresses.
+template <typename T, typename Code, int kRun>
+__device__ __forceinline__ void encode_rows(const RowCodec &c, const List<32> &list, int n, Magics m, int lane)
 {
-    const uint32_t per_row = c.quant_elems / kQuantGroup, total = static_cast<uint32_t>(n) * per_row;
-    const int lane = threadIdx.x & 15;
-    for (uint32_t g0 = threadIdx.x / 32 * 16; g0 < total; g0 += kThreads / 16 * 8) {  // (uniform over the warp)
-        const uint32_t mine = g0 + (threadIdx.x >> 4 & 1) * 8;
+    copy_plain<32>(list, n, c.plain_elems / 8, m.plain, 2 * c.quant_elems, c.quant_elems + codec_scale_bytes(c), lane);
+    const uint32_t per_row = c.quant_elems / (kQuantGroup * kRun), total = static_cast<uint32_t>(n) * per_row;  // runs
+    constexpr int kRuns = 8 / kRun;
+    const int half = lane >> 4, unit = lane & 15;
+    for (uint32_t r0 = 0; r0 < total; r0 += 2 * kRuns) {
+        const uint32_t mine = r0 + half * kRuns;
         uint4 v[8];
-        uint32_t row[8], group[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            row[k] = div_magic(mine + k, per_row, magic);
-            group[k] = mine + k - row[k] * per_row;
-            v[k] = make_uint4(0u, 0u, 0u, 0u);
-            if (mine + k < total) v[k] = load_stream(reinterpret_cast<const uint4 *>(src[row[k]]) + group[k] * 16 + lane);
+        for (int j = 0; j < kRuns; ++j) {
+            const uint32_t row = div_magic(mine + j, per_row, m.quant), run = mine + j - row * per_row;
+            const bool any = mine + j < total;
+            const uint4 *at = any ? reinterpret_cast<const uint4 *>(list.src[row]) + run * (16 * kRun) + unit : nullptr;
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                v[j * kRun + k] = make_uint4(0u, 0u, 0u, 0u);
+                if (any) v[j * kRun + k] = load_stream(at + 16 * k);
+            }
         }
         uint2 codes[8];
         float scale;
-        encode_groups<T, Code>(v, lane, codes, &scale);
-        uint8_t *at = nullptr;  // this lane's group's scale
-        uint32_t at_group = 0;
+        encode_groups<T, Code>(v, unit, codes, &scale);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (mine + k >= total) continue;
-            uint8_t *d = dst[row[k]];
-            reinterpret_cast<uint2 *>(d)[group[k] * 16 + lane] = codes[k];
-            if (scale_group(lane) == k && (lane & 1) == 0) {
-                at = d + c.quant_elems;
-                at_group = group[k];
+        for (int j = 0; j < kRuns; ++j) {
+            const uint32_t row = div_magic(mine + j, per_row, m.quant), run = mine + j - row * per_row;
+            if (mine + j < total) {
+                uint2 *at = reinterpret_cast<uint2 *>(list.dst[row]) + run * (16 * kRun) + unit;
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) at[16 * k] = codes[j * kRun + k];
             }
         }
-        if (at != nullptr) {
-            reinterpret_cast<float *>(at)[at_group] = scale;
-            if (at_group + 1 == per_row)  // the padding, as zeros
-                for (uint32_t g = per_row; g < codec_scale_bytes(c) / 4; ++g) reinterpret_cast<float *>(at)[g] = 0.f;
+        const uint32_t own = mine + scale_group(unit) / kRun;  // the run of the group whose scale this lane has
+        if (own < total && (unit & 1) == 0) {
+            const uint32_t row = div_magic(own, per_row, m.quant);
+            const uint32_t group = (own - row * per_row) * kRun + scale_group(unit) % kRun;
+            float *scales = reinterpret_cast<float *>(list.dst[row] + c.quant_elems);
+            scales[group] = scale;
+            if (kRun == 1 && group + 1 == per_row)  // the padding, as zeros (no run of four leaves any)
+                for (uint32_t g = per_row; g < codec_scale_bytes(c) / 4; ++g) scales[g] = 0.f;
         }
     }
-    cta_copy_plain(src, dst, n, c.plain_elems / 8, 2 * c.quant_elems, c.quant_elems + codec_scale_bytes(c));
 }
 
-// Reads n stored rows src[i] back into the 16-bit rows dst[i].
+// Reads n listed stored rows back into 16-bit rows, with the whole CTA.
 template <typename T, typename Code>
-__device__ __forceinline__ void cta_decode_rows(const RowCodec &c, const uint8_t *const *src, uint8_t *const *dst,
-                                                int n, uint32_t magic)
+__device__ __forceinline__ void decode_rows(const RowCodec &c, const List<kThreads> &list, int n, Magics m)
 {
-    // units of 16 codes, eight to a group
-    const uint32_t units = c.quant_elems / 16;
-    const uint32_t total = static_cast<uint32_t>(n) * units;
+    const uint32_t units = c.quant_elems / 16, total = static_cast<uint32_t>(n) * units;  // (eight to a group)
     for (uint32_t i0 = threadIdx.x; i0 < total; i0 += kThreads * kUnroll) {
         uint4 v[kUnroll];
         float scale[kUnroll];
-        uint32_t row[kUnroll], unit[kUnroll];
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k) {
-            const uint32_t i = i0 + k * kThreads;
-            row[k] = div_magic(i, units, magic);
-            unit[k] = i - row[k] * units;
+            const uint32_t i = i0 + k * kThreads, row = div_magic(i, units, m.quant), unit = i - row * units;
             if (i < total) {
-                const uint8_t *s = src[row[k]];
-                v[k] = load_stream(reinterpret_cast<const uint4 *>(s) + unit[k]);
-                scale[k] = *reinterpret_cast<const volatile float *>(s + c.quant_elems + unit[k] / 8 * 4);
+                const uint8_t *s = list.src[row];
+                v[k] = load_stream(reinterpret_cast<const uint4 *>(s) + unit);
+                scale[k] = *reinterpret_cast<const volatile float *>(s + c.quant_elems + unit / 8 * 4);
             }
         }
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k) {
-            if (i0 + k * kThreads < total) {
-                uint4 *d = reinterpret_cast<uint4 *>(dst[row[k]]) + 2 * unit[k];
+            const uint32_t i = i0 + k * kThreads, row = div_magic(i, units, m.quant), unit = i - row * units;
+            if (i < total) {
+                uint4 *d = reinterpret_cast<uint4 *>(list.dst[row]) + 2 * unit;
                 d[0] = decode_unit<T, Code>(make_uint2(v[k].x, v[k].y), scale[k]);
                 d[1] = decode_unit<T, Code>(make_uint2(v[k].z, v[k].w), scale[k]);
             }
         }
     }
-    cta_copy_plain(src, dst, n, c.plain_elems / 8, c.quant_elems + codec_scale_bytes(c), 2 * c.quant_elems);
+    copy_plain<kThreads>(list, n, c.plain_elems / 8, m.plain, c.quant_elems + codec_scale_bytes(c), 2 * c.quant_elems,
+                         threadIdx.x);
 }
 
-// Miss rows read back (kWrite false) or flagged hot rows written (true) under the gather's rules.
-template <typename T, typename Code, bool kWrite>
-__global__ void __launch_bounds__(kThreads, 4) gather_quant_kernel(const GatherParams p, const RowCodec c,
-                                                                   uint32_t tile, uint32_t magic)
+// The number of positions of the launch's real batch rows. Launched as programmatic dependents, like
+// gather_kernel (rows.cu): wait for the kernel before (the SIEVE step) to end before its outputs are read.
+__device__ __forceinline__ int64_t real_positions(const GatherParams &p)
 {
-    __shared__ const uint8_t *s_src[kThreads];
-    __shared__ uint8_t *s_dst[kThreads];
-    __shared__ int s_n;
-    // Launched as a programmatic dependent, like gather_kernel (rows.cu): wait for the kernel
-    // before (the SIEVE step) to end before its outputs are read.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
     int32_t num_real = p.num_real != nullptr ? *p.num_real : 0;
     if (num_real > static_cast<int32_t>(p.max_num_reqs)) num_real = static_cast<int32_t>(p.max_num_reqs);
-    const int64_t total = num_real > 0 ? static_cast<int64_t>(num_real) * p.top_k : 0;
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * tile; base < total;
-         base += static_cast<int64_t>(gridDim.x) * tile) {
-        const int64_t pos = base + threadIdx.x;
+    return num_real > 0 ? static_cast<int64_t>(num_real) * p.top_k : 0;
+}
+
+// The rule for one position: its segment row and hot row.
+__device__ __forceinline__ bool rows_of(const GatherParams &p, const RowCodec &c, int64_t pos, const uint8_t **seg_row,
+                                        uint8_t **hot_row)
+{
+    if (p.is_miss[pos] == 0) return false;
+    const int64_t bid = pos / p.top_k;
+    const int32_t slot = p.slots[pos];
+    const int64_t req = p.req_pool[bid];
+    if (!gather_source(p, pos, 1, p.topk[pos], slot, req, p.host_base[bid], seg_row)) return false;
+    *hot_row = p.hot + static_cast<uint64_t>(req) * p.hot_req_stride_bytes +
+               static_cast<uint64_t>(slot) * codec_row_bytes(c);
+    return true;
+}
+
+// Miss rows read back under the gather's rules.
+template <typename T, typename Code>
+__global__ void __launch_bounds__(kThreads, 4) import_quant_kernel(const GatherParams p, const RowCodec c, int tile,
+                                                                   Magics magics)
+{
+    __shared__ List<kThreads> list;
+    __shared__ int s_n;
+    const int thread = threadIdx.x;
+    const int64_t total = real_positions(p), step = static_cast<int64_t>(gridDim.x) * tile;
+    if (thread == 0) s_n = 0;
+    __syncthreads();
+    for (int64_t pos = static_cast<int64_t>(blockIdx.x) * tile + thread; pos - thread < total; pos += step) {
         const uint8_t *seg_row = nullptr;
         uint8_t *hot_row = nullptr;
-        bool ok = false;
-        if (threadIdx.x < tile && pos < total && p.is_miss[pos] != 0) {
-            const int64_t bid = pos / p.top_k;
-            const int32_t slot = p.slots[pos];
-            const int64_t req = p.req_pool[bid];
-            ok = gather_source(p, pos, 1, p.topk[pos], slot, req, p.host_base[bid], &seg_row);
-            if (ok)
-                hot_row = p.hot + static_cast<uint64_t>(req) * p.hot_req_stride_bytes +
-                          static_cast<uint64_t>(slot) * codec_row_bytes(c);
-        }
-        list_append(ok, kWrite ? hot_row : seg_row, kWrite ? const_cast<uint8_t *>(seg_row) : hot_row, s_src, s_dst,
-                    &s_n);
+        const bool ok = thread < tile && pos < total && rows_of(p, c, pos, &seg_row, &hot_row);
+        list_append(ok, seg_row, hot_row, list.src, list.dst, &s_n);
         __syncthreads();
-        if (kWrite) cta_encode_rows<T, Code>(c, s_src, s_dst, s_n, magic);
-        else cta_decode_rows<T, Code>(c, s_src, s_dst, s_n, magic);
+        decode_rows<T, Code>(c, list, s_n, magics);
         __syncthreads();
-        if (threadIdx.x == 0) s_n = 0;
+        if (thread == 0) s_n = 0;
         __syncthreads();
+    }
+    __syncthreads();
+    if (thread == 0) arrive_and_publish(p.st);
+}
+
+// Flagged hot rows written under the gather's rules.
+template <typename T, typename Code, int kRun>
+__global__ void __launch_bounds__(kThreads, 4) scatter_quant_kernel(const GatherParams p, const RowCodec c, int tile,
+                                                                    Magics magics)
+{
+    __shared__ List<32> lists[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (tiles of a CTA's warps lie a grid apart, so that few positions use many CTAs)
+    const int64_t total = real_positions(p), step = static_cast<int64_t>(gridDim.x) * kWarps * tile;
+    for (int64_t pos = (static_cast<int64_t>(warp) * gridDim.x + blockIdx.x) * tile + lane; pos - lane < total; pos += step) {
+        const uint8_t *seg_row = nullptr;
+        uint8_t *hot_row = nullptr;
+        const bool ok = lane < tile && pos < total && rows_of(p, c, pos, &seg_row, &hot_row);
+        const int n = list_rows(lists[warp], ok, hot_row, const_cast<uint8_t *>(seg_row), lane);
+        encode_rows<T, Code, kRun>(c, lists[warp], n, magics, lane);
     }
     __syncthreads();
     if (threadIdx.x == 0) arrive_and_publish(p.st);
 }
 
-template <typename T, typename Code>
-__global__ void __launch_bounds__(kThreads, 4) export_quant_kernel(const ExportQuantParams p, uint32_t tile, uint32_t magic)
+template <typename T, typename Code, int kRun>
+__global__ void __launch_bounds__(kThreads, 4) export_quant_kernel(const ExportQuantParams p, int tile, Magics magics)
 {
-    __shared__ const uint8_t *s_src[kThreads];
-    __shared__ uint8_t *s_dst[kThreads];
-    __shared__ int s_n;
+    __shared__ List<32> lists[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint64_t total = p.units_per_layer * p.layer_num;
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
-    for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * tile; base < total;
-         base += static_cast<uint64_t>(gridDim.x) * tile) {
-        const uint64_t u = base + threadIdx.x;
+    for (uint64_t base = (static_cast<uint64_t>(warp) * gridDim.x + blockIdx.x) * tile; base < total;
+         base += static_cast<uint64_t>(gridDim.x) * kWarps * tile) {
+        const uint64_t u = base + lane;
         bool ok = false;
         const uint8_t *src = nullptr;
         uint8_t *dst = nullptr;
-        if (threadIdx.x < tile && u < total) {
+        if (lane < tile && u < total) {
             const uint64_t l = u / p.units_per_layer, k = u - l * p.units_per_layer;
             // Unit k is the k-th row, or (reference map) the last row in range of the k-th stripe, the
             // one that the reference's ascending per-row writes leave in the shared segment row.
@@ -197,46 +261,60 @@ __global__ void __launch_bounds__(kThreads, 4) export_quant_kernel(const ExportQ
                 ok = true;
             }
         }
-        list_append(ok, src, dst, s_src, s_dst, &s_n);
-        __syncthreads();
-        cta_encode_rows<T, Code>(p.codec, s_src, s_dst, s_n, magic);
-        __syncthreads();
-        if (threadIdx.x == 0) s_n = 0;
-        __syncthreads();
+        const int n = list_rows(lists[warp], ok, src, dst, lane);
+        encode_rows<T, Code, kRun>(p.codec, lists[warp], n, magics, lane);
     }
     __syncthreads();
     if (threadIdx.x == 0) arrive_and_publish(p.st);
 }
 
-// Positions per tile (at most one per thread) and grid of a launch: tiles of `most` positions, or smaller
-// ones where those leave CTAs without any.
+// Positions per tile and grid of a launch.
 struct Shape {
-    uint32_t tile;
-    int grid;
+    int tile, grid;
 };
 
-Shape shape_of(uint64_t positions, uint32_t most, int sm_count)
+Shape shape_of(uint64_t positions, int sm_count, bool write)
 {
     Shape s;
-    const uint64_t cap = static_cast<uint64_t>(sm_count > 0 ? sm_count : 148) * 4;
-    s.tile = most;
-    while (s.tile > 16 && positions <= cap * (s.tile / 2)) s.tile /= 2;
+    const uint64_t ctas = static_cast<uint64_t>(sm_count > 0 ? sm_count : 148) * 4;
+    if (write) {
+        // At least eight tiles a warp, so that the last one costs little (8192 rows of 61 layers: 189 us, with
+        // 32 positions a tile 215), down to tiles of four rows, which are one round of loads; below that,
+        // one tile a warp.
+        s.tile = 32;
+        while (s.tile > 4 && positions <= 8 * ctas * kWarps * (s.tile / 2)) s.tile /= 2;
+        while (s.tile > 1 && positions <= ctas * kWarps * (s.tile / 2)) s.tile /= 2;
+    } else {
+        // One for every thread, since few may be misses; fewer where that leaves CTAs without any (131,072
+        // positions, a fifth of them misses: 18 us, with 64 positions a tile 25).
+        s.tile = kThreads;
+        while (s.tile > 16 && positions <= ctas * (s.tile / 2)) s.tile /= 2;
+    }
     const uint64_t tiles = (positions + s.tile - 1) / s.tile;
-    s.grid = static_cast<int>(tiles < 1 ? 1 : (tiles < cap ? tiles : cap));
+    s.grid = static_cast<int>(tiles < 1 ? 1 : (tiles < ctas ? tiles : ctas));
     return s;
 }
 
 // The multiplier of div_magic for indexes up to one round past a tile's last, or 0.
 uint32_t magic_of(uint64_t d)
 {
-    return d * (kThreads * d + kThreads * 8) < (1ull << 32) ? static_cast<uint32_t>(((1ull << 32) + d - 1) / d) : 0u;
+    return d != 0 && d * (kThreads * d + kThreads * kUnroll) < (1ull << 32) ? static_cast<uint32_t>(((1ull << 32) + d - 1) / d) : 0u;
+}
+
+// Four groups of a row at a time, where the row has that many.
+bool by_fours(const RowCodec &c) { return c.quant_elems % (4 * kQuantGroup) == 0; }
+
+Magics magics_of(const RowCodec &c, bool write)
+{
+    return {magic_of(!write ? c.quant_elems / 16 : c.quant_elems / (by_fours(c) ? 4 * kQuantGroup : kQuantGroup)),
+            magic_of(c.plain_elems / 8)};
 }
 
 template <typename T, typename Code>
 cudaError_t launch_gather_as(const GatherParams &p, const RowCodec &c, bool write, cudaStream_t s, int sm_count)
 {
-    const Shape sh = shape_of(static_cast<uint64_t>(p.max_num_reqs) * p.top_k, kThreads, sm_count);
-    const uint32_t magic = magic_of(write ? c.quant_elems / kQuantGroup : c.quant_elems / 16);
+    const Shape sh = shape_of(static_cast<uint64_t>(p.max_num_reqs) * p.top_k, sm_count, write);
+    const Magics magics = magics_of(c, write);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(sh.grid);
     cfg.blockDim = dim3(kThreads);
@@ -246,15 +324,18 @@ cudaError_t launch_gather_as(const GatherParams &p, const RowCodec &c, bool writ
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return write ? cudaLaunchKernelEx(&cfg, gather_quant_kernel<T, Code, true>, p, c, sh.tile, magic)
-                 : cudaLaunchKernelEx(&cfg, gather_quant_kernel<T, Code, false>, p, c, sh.tile, magic);
+    if (!write) return cudaLaunchKernelEx(&cfg, import_quant_kernel<T, Code>, p, c, sh.tile, magics);
+    return by_fours(c) ? cudaLaunchKernelEx(&cfg, scatter_quant_kernel<T, Code, 4>, p, c, sh.tile, magics)
+                       : cudaLaunchKernelEx(&cfg, scatter_quant_kernel<T, Code, 1>, p, c, sh.tile, magics);
 }
 
 template <typename T, typename Code>
 cudaError_t launch_export_as(const ExportQuantParams &p, cudaStream_t s, int sm_count)
 {
-    const Shape sh = shape_of(p.units_per_layer * p.layer_num, kThreads / 2, sm_count);
-    export_quant_kernel<T, Code><<<sh.grid, kThreads, 0, s>>>(p, sh.tile, magic_of(p.codec.quant_elems / kQuantGroup));
+    const Shape sh = shape_of(p.units_per_layer * p.layer_num, sm_count, true);
+    const Magics magics = magics_of(p.codec, true);
+    if (by_fours(p.codec)) export_quant_kernel<T, Code, 4><<<sh.grid, kThreads, 0, s>>>(p, sh.tile, magics);
+    else export_quant_kernel<T, Code, 1><<<sh.grid, kThreads, 0, s>>>(p, sh.tile, magics);
     return cudaGetLastError();
 }
 
