@@ -180,31 +180,39 @@ class XdsOffloadCoordinator:
         and workspace (uint8, at least _kvops.attend_workspace(...) bytes, used by one call at a
         time) may be given; otherwise they are allocated for the call. err_word: address (or int32
         tensor) of a word that receives errCode 0x103 if a wait inside the kernel gave up."""
-        squeeze = q.dim() == 3
+        shape = q.shape
+        squeeze = len(shape) == 3
         if squeeze:
             q = q.unsqueeze(1)
-        if q.dim() != 4 or q.shape[3] != KEY_DIM or q.stride(3) != 1:
+            shape = q.shape
+        strides = q.stride()
+        if len(shape) != 4 or shape[3] != KEY_DIM or strides[3] != 1:
             raise ValueError("attend: q must be [B, heads, 576] or [B, tokens, heads, 576] with unit last stride")
-        B, T, H, _ = q.shape
+        B, T, H, _ = shape
         dtype = dtype_name(q.dtype)
         if B > self.max_num_reqs:
             raise ValueError("attend: {} batch rows, max_num_reqs is {}".format(B, self.max_num_reqs))
         if self._req_pool_indices is None or self._req_pool_indices.shape[0] < B:
             raise RuntimeError("attend: call set_batch() with at least q's batch rows first")
         slots = self.top_k_device_slots if topk_device_slots is None else topk_device_slots
-        if slots.dtype != torch.int32 or slots.dim() not in (2, 3) or slots.shape[0] < B or \
-                (slots.dim() == 3 and slots.shape[1] != T) or (slots.shape[-1] > 1 and slots.stride(-1) != 1):
+        s_shape, s_strides = slots.shape, slots.stride()
+        if slots.dtype != torch.int32 or len(s_shape) not in (2, 3) or s_shape[0] < B or \
+                (len(s_shape) == 3 and s_shape[1] != T) or (s_shape[-1] > 1 and s_strides[-1] != 1):
             raise ValueError("attend: topk_device_slots must be int32 [B, K] or [B, tokens, K] with unit last stride")
+        K = s_shape[-1]
         if row_format not in ROW_BYTES:
             raise ValueError("attend: row_format must be 'raw', 'e4m3' or 'int8', got {!r}".format(row_format))
         if hot_rows is None:
             hot_rows = hot_req_stride_rows or self.device_buffer_size
-        D = 0
+        D, draft_at, draft_strides = 0, 0, (0, 0)
         if draft_rows is not None:
             if draft_rows.dim() != 3 or draft_rows.shape[0] < B or draft_rows.shape[2] != KEY_DIM or \
                     draft_rows.dtype != q.dtype or draft_rows.stride(2) != 1:
                 raise ValueError("attend: draft_rows must be [B, drafts, 576] of q's type with unit last stride")
             D = draft_rows.shape[1]
+            if D:
+                draft_at = draft_rows.data_ptr()
+                draft_strides = (draft_rows.stride(0) if draft_rows.shape[0] > 1 else 0, draft_rows.stride(1) if D > 1 else 0)
         if tree is not None and (tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] < B or
                                  tree.shape[1] != T or not tree.is_contiguous()):
             raise ValueError("attend: tree must be a contiguous int64 [B, tokens]")
@@ -212,47 +220,44 @@ class XdsOffloadCoordinator:
             need = ((self.pool_size - 1) * hot_req_stride_rows + hot_rows) * ROW_BYTES[row_format]
             if hot_row_base.numel() * hot_row_base.element_size() < need or not hot_row_base.is_contiguous():
                 raise ValueError("attend: hot rows must be contiguous and hold {} bytes".format(need))
+            if hot_row_base.device != self.top_k_device_slots.device:
+                raise ValueError("attend: hot rows must be on {}".format(self.top_k_device_slots.device))
             hot = hot_row_base.data_ptr()
         else:
             hot = hot_row_base
-        for name, x, shape, want in (("out", out, (B, T, H, VALUE_DIM), q.dtype), ("lse", lse, (B, T, H), torch.float32)):
-            if x is not None and (x.dtype != want or not x.is_contiguous() or x.numel() != B * T * H * (
-                    VALUE_DIM if name == "out" else 1) or x.device != q.device):
-                raise ValueError("attend: {} must be a contiguous {} {}".format(name, want, shape))
-        for x in (q, slots, draft_rows, tree, workspace):
-            if x is not None and x.device != self.top_k_device_slots.device:
-                raise ValueError("attend: every tensor must be on {}".format(self.top_k_device_slots.device))
-        with self._on_device():
-            if stream is None:
-                return self._attend(q, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale, slots, draft_rows,
-                                    D, tree, out, lse, workspace, self._stream(), squeeze, err_word)
-            # what is allocated below belongs to the stream that uses it
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
-                return self._attend(q, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale, slots, draft_rows,
-                                    D, tree, out, lse, workspace, stream, squeeze, err_word)
-
-    def _attend(self, q, hot, stride, hot_rows, row_format, dtype, scale, slots, draft, D, tree, out, lse, workspace,
-                stream, squeeze, err_word):
-        B, T, H, _ = q.shape
-        K = slots.shape[-1]
-
-        def step(x, d):  # the stride of a dimension of one entry is never used
-            return x.stride(d) if x.shape[d] > 1 else 0
-
-        if out is None:
-            out = torch.empty((B, H, VALUE_DIM) if squeeze else (B, T, H, VALUE_DIM), dtype=q.dtype, device=q.device)
-        if lse is None:
-            lse = torch.empty((B, H) if squeeze else (B, T, H), dtype=torch.float32, device=q.device)
-        if workspace is None:
-            need = self._k.attend_workspace(B, T, H, K, D, row_format, dtype)
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        self._k.attend_hot(
-            q.data_ptr(), step(q, 0), step(q, 1), step(q, 2), hot, stride, hot_rows,
-            self._req_pool_indices.data_ptr(), self.pool_size, slots.data_ptr(), step(slots, 0),
-            step(slots, 1) if slots.dim() == 3 else 0, self.num_real.data_ptr(),
-            draft.data_ptr() if D else 0, step(draft, 0) if D else 0, step(draft, 1) if D else 0,
-            tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
-            workspace.data_ptr() if workspace is not None else 0, workspace.numel() if workspace is not None else 0,
-            B, T, H, K, D, row_format, dtype, KEY_DIM ** -0.5 if scale is None else scale, stream,
-            err_word=err_word if isinstance(err_word, int) else err_word.data_ptr())
+        for name, x, want, each in (("out", out, q.dtype, VALUE_DIM), ("lse", lse, torch.float32, 1)):
+            if x is not None and (x.dtype != want or not x.is_contiguous() or x.numel() != B * T * H * each):
+                raise ValueError("attend: {} must be a contiguous {} of {} elements".format(name, want, B * T * H * each))
+        dev = self.top_k_device_slots.device
+        for x in (q, slots, draft_rows, tree, out, lse, workspace):
+            if x is not None and x.device != dev:
+                raise ValueError("attend: every tensor must be on {}".format(dev))
+        with contextlib.ExitStack() as stack:
+            if dev.type == "cuda":
+                if torch.cuda.current_device() != dev.index:
+                    stack.enter_context(torch.cuda.device(dev))
+                if stream is None:
+                    stream = torch._C._cuda_getCurrentRawStream(dev.index)  # (no Stream object: 4 us of a 25 us call)
+                elif out is None or lse is None or workspace is None:
+                    # what is allocated below belongs to the stream that uses it
+                    stack.enter_context(torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev)))
+            if out is None:
+                out = q.new_empty((B, H, VALUE_DIM) if squeeze else (B, T, H, VALUE_DIM))
+            if lse is None:
+                lse = q.new_empty((B, H) if squeeze else (B, T, H), dtype=torch.float32)
+            room = workspace.numel() if workspace is not None else 0
+            if workspace is None:
+                room = self._k.attend_workspace(B, T, H, K, D, row_format, dtype)
+                if room:
+                    workspace = q.new_empty(room, dtype=torch.uint8)
+            # (the stride of a dimension of one entry is never used)
+            self._k.attend_hot(
+                q.data_ptr(), strides[0] if B > 1 else 0, strides[1] if T > 1 else 0, strides[2] if H > 1 else 0, hot,
+                hot_req_stride_rows, hot_rows, self._req_pool_indices.data_ptr(), self.pool_size, slots.data_ptr(),
+                s_strides[0] if s_shape[0] > 1 else 0, s_strides[1] if len(s_shape) == 3 and T > 1 else 0,
+                self.num_real.data_ptr(), draft_at, draft_strides[0], draft_strides[1],
+                tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
+                workspace.data_ptr() if room else 0, room, B, T, H, K, D, row_format, dtype,
+                KEY_DIM ** -0.5 if scale is None else scale, stream or 0,
+                err_word=err_word if isinstance(err_word, int) else err_word.data_ptr())
         return out, lse
