@@ -54,11 +54,17 @@ constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kWeighWarp = kScoreWarp +
 constexpr int kThreads = (kFindWarp + 1) * 32;
 constexpr uint32_t kAhead = 4;  // tiles whose rows are known at a time
 
-// A running reference is kept this far (in powers of two) below the largest score seen, so that
-// the probabilities, up to 2^kLift, lose none of their small neighbours to fp16's subnormals, and it is
-// only moved when a score passes it by kLift + kSlack (2^15 still is an fp16 number): moving it means
-// scaling the outputs in tensor memory.
-constexpr float kLift = 11.f, kSlack = 4.f;
+// A column's running reference: probabilities are 2^(score - reference), and it is set kLift (in powers of
+// two) below the largest score so far when a score passes it by kLift + kSlack. They stay below
+// 2^15, which is an fp16 number; moving the reference means scaling the outputs in tensor memory, so it should
+// be rare: kSlack is what a later score may exceed the first tile's largest by. (Normal scores of variance
+// 3, as of unit-variance queries and rows: with a slack of 4, 106 us for 64 requests x 128 heads, with
+// 11, 81.) fp16's smallest step is 2^-24, that is 2^-28 of the largest probability at the least: with 2^16 keys
+// all rounded by half of it the same way, 2^-13 of the output, below its own rounding. bf16 has no such limit.
+template <typename T>
+constexpr float kLift = std::is_same<T, Bf16>::value ? -5.f : 4.f;
+template <typename T>
+constexpr float kSlack = 15.f - kLift<T>;
 
 // How the (query tile, key tile) pairs are dealt out. Units are query tiles: group (a request, or a
 // request's token where every token has its own list) by group.
@@ -69,6 +75,7 @@ struct Plan {
     uint32_t list_end;    // top_k rounded up to four: where the drafted rows start among the keys
     uint32_t tiles;       // key tiles per unit
     uint32_t ctas;
+    uint32_t run_at_most; // pairs of a run, with every request real
     uint32_t whole;       // > 0: every CTA takes this many whole units; 0: runs of pairs of one length
     float2 *part_ml;      // [2 * ctas][NQ] reference and sum of a unit's part
     float *part_o;        // [2 * ctas][NQ * 512] its weighted sums, in part_at's order
@@ -752,7 +759,7 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 // the warps need not wait for one another before, and again in the rare tile where one has.
                 const float excess = lower();
                 write();
-                move_all = group_any(1 + half, 128, excess > kLift + kSlack || (open && excess > -INFINITY));
+                move_all = group_any(1 + half, 128, excess > kLift<T> + kSlack<T> || (open && excess > -INFINITY));
                 if (move_all) scores();
             }
             if (move_all) {
@@ -765,9 +772,9 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 // the same decision in the four warps of this half
                 top = fmaxf(fmaxf(sh.top[half][0][column], sh.top[half][1][column]),
                             fmaxf(sh.top[half][2][column], sh.top[half][3][column]));
-                const bool move = top > ref + (kLift + kSlack) || (ref == -INFINITY && top > -INFINITY);
+                const bool move = top > ref + (kLift<T> + kSlack<T>) || (ref == -INFINITY && top > -INFINITY);
                 const float was = ref;
-                if (move) ref = top - kLift;
+                if (move) ref = top - kLift<T>;
                 if (started && __any_sync(0xFFFFFFFFu, move)) {
                     spread(move ? exp2_fast(was - ref) : 1.f);
                     mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
@@ -968,15 +975,16 @@ static_assert(sizeof(Shared) <= 6 * 1024, "as Layout counts it");
 static_assert(offsetof(Shared, per_warp) % 16 == 0 && alignof(Shared) % 16 == 0, "read as float4");
 
 // Joins the parts of the units that the ends of runs cut. Block x is the cut behind CTA x's run, and does
-// its unit if it is the first cut in it; block y takes four query rows, block z 128 dimensions, a thread
-// one of them. The parts are added in their order.
+// its unit if it is the first cut in it; block y takes four query rows, and block z kBlocks of the
+// four blocks of 128 dimensions, a thread one of each. The parts are added in their order. Every warp works
+// the weights out for itself and the first parts are fetched meanwhile, so that a block is one chain of
+// two loads and the blocks, which have little to do, are few.
 constexpr int kJoinThreads = 128;
-template <typename T, int NQ>
+template <typename T, int NQ, int kBlocks>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const KvopsAttend a, const Plan plan)
 {
-    __shared__ alignas(16) uint16_t rows[4][kJoinThreads];
-    __shared__ float4 weight[kJoinThreads];  // of a part, by row
-    __shared__ float top_of[4][4], sum_of[4][4];
+    constexpr uint32_t kFirst = 16 / kBlocks;  // parts fetched ahead
+    __shared__ float4 weight[kJoinThreads / 32][32];  // of a part, by row
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t units = real_units(a, plan), run = run_length(plan, units), cut = (blockIdx.x + 1) * run;
     if (cut >= units * plan.tiles || cut % plan.tiles == 0) return;
@@ -984,72 +992,97 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const KvopsAttend a,
     const uint32_t first = begin / run, parts = (end - 1) / run - first + 1;
     if (first != blockIdx.x) return;
     const Unit u = unit_at<NQ>(plan, unit);
-    const uint32_t row = blockIdx.y * 4, thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
+    const uint32_t row = blockIdx.y * 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (row >= u.rows) return;
-    const uint32_t half = row / (NQ / 2), i = row % (NQ / 2) / 4;
+    const uint32_t half = row / (NQ / 2), i = row % (NQ / 2) / 4, block0 = blockIdx.z * kBlocks;
     // the part of CTA c: slot 2 c, or 2 c + 1 where its run started in an earlier unit (the first's may have)
     const auto slot_of = [&](uint32_t n) { return 2 * (first + n) + (n == 0 && first * run < begin ? 1 : 0); };
-    const auto at_most = [&](float x, float (&of)[4][4], int k) {  // over the block's threads
-        for (int w = 16; w > 0; w /= 2) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, w));
-        if (lane == 0) of[k][warp] = x;
+    const float4 *o = reinterpret_cast<const float4 *>(plan.part_o);
+    float4 ahead[kFirst][kBlocks];
+#pragma unroll
+    for (uint32_t n = 0; n < kFirst; ++n)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+            if (n < parts) ahead[n][b] = o[part_at<NQ>(slot_of(n), block0 + b, warp, half, i, lane)];
+    struct Stats {
+        float top[4], sum[4];  // reference and sum of a part, by row
     };
-    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, total[4] = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t n = thread; n < parts; n += kJoinThreads) {
+    const auto stats = [&](uint32_t n) {  // of part n; of none, and in rows behind the last, nothing
+        Stats x;
         const float2 *ml = plan.part_ml + static_cast<uint64_t>(slot_of(n)) * NQ + row;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (row + k < u.rows) top[k] = fmaxf(top[k], ml[k].x);
+        for (int k = 0; k < 4; ++k) {
+            const bool some = n < parts && row + k < u.rows;
+            const float2 v = some ? ml[k] : make_float2(-INFINITY, 0.f);
+            x.top[k] = v.x, x.sum[k] = v.y;
+        }
+        return x;
+    };
+    Stats x = stats(lane);
+    float top[4], total[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top[k] = x.top[k];
+    for (uint32_t n = 32 + lane; n < parts; n += 32) {
+        const Stats y = stats(n);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], y.top[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) at_most(top[k], top_of, k);
-    __syncthreads();
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) top[k] = fmaxf(fmaxf(top_of[k][0], top_of[k][1]), fmaxf(top_of[k][2], top_of[k][3]));
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t n0 = 0; n0 < parts; n0 += kJoinThreads) {
-        const uint32_t some = min(parts - n0, static_cast<uint32_t>(kJoinThreads));
-        if (thread < some) {
-            const float2 *ml = plan.part_ml + static_cast<uint64_t>(slot_of(n0 + thread)) * NQ + row;
-            float w[4];
+        for (int w = 16; w > 0; w /= 2) top[k] = fmaxf(top[k], __shfl_xor_sync(0xFFFFFFFFu, top[k], w));
+    float4 acc[kBlocks];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                w[k] = 0.f;
-                if (row + k < u.rows && (ml[k].x != -INFINITY || ml[k].y != 0.f)) {
-                    w[k] = exp2_fast(ml[k].x - top[k]);
-                    total[k] += ml[k].y * w[k];
-                }
-            }
-            weight[thread] = make_float4(w[0], w[1], w[2], w[3]);
+    for (int b = 0; b < kBlocks; ++b) acc[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](int b, const float4 &v, const float4 &w) {
+        acc[b].x += v.x * w.x, acc[b].y += v.y * w.y, acc[b].z += v.z * w.z, acc[b].w += v.w * w.w;
+    };
+    for (uint32_t n0 = 0; n0 < parts; n0 += 32) {
+        if (n0 > 0) x = stats(n0 + lane);
+        float w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // (a part without any key has reference -inf and sum 0, or NaN)
+            w[k] = x.top[k] != -INFINITY || x.sum[k] != 0.f ? exp2_fast(x.top[k] - top[k]) : 0.f;
+            total[k] += x.sum[k] * w[k];
         }
-        __syncthreads();
-        const float4 *o = reinterpret_cast<const float4 *>(plan.part_o);
+        __syncwarp();
+        weight[warp][lane] = make_float4(w[0], w[1], w[2], w[3]);
+        __syncwarp();
+        const uint32_t some = min(parts - n0, 32u);
+        if (n0 == 0) {
+#pragma unroll
+            for (uint32_t n = 0; n < kFirst; ++n)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+                    if (n < parts) add(b, ahead[n][b], weight[warp][n]);
+        }
 #pragma unroll 8
-        for (uint32_t n = 0; n < some; ++n) {
-            const float4 v = o[part_at<NQ>(slot_of(n0 + n), blockIdx.z, warp, half, i, lane)], w = weight[n];
-            acc.x += v.x * w.x, acc.y += v.y * w.y, acc.z += v.z * w.z, acc.w += v.w * w.w;
-        }
-        __syncthreads();
+        for (uint32_t n = n0 == 0 ? kFirst : 0; n < some; ++n)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+                add(b, o[part_at<NQ>(slot_of(n0 + n), block0 + b, warp, half, i, lane)], weight[warp][n]);
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
         for (int w = 16; w > 0; w /= 2) total[k] += __shfl_xor_sync(0xFFFFFFFFu, total[k], w);
-        if (lane == 0) sum_of[k][warp] = total[k];
-    }
-    __syncthreads();
-    const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+    float f[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        total[k] = (sum_of[k][0] + sum_of[k][1]) + (sum_of[k][2] + sum_of[k][3]);
-        rows[k][thread] = static_cast<uint16_t>(T::pack(total[k] == 0.f ? 0.f : v[k] * (1.f / total[k]), 0.f));
+    for (int k = 0; k < 4; ++k) f[k] = total[k] == 0.f ? 0.f : 1.f / total[k];
+    const bool odd = lane & 1;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        const float v[4] = {total[0] == 0.f ? 0.f : acc[b].x * f[0], total[1] == 0.f ? 0.f : acc[b].y * f[1],
+                            total[2] == 0.f ? 0.f : acc[b].z * f[2], total[3] == 0.f ? 0.f : acc[b].w * f[3]};
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {  // an even lane takes row c of its dimension and the next, an odd one c + 1
+            const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[c] : v[c + 1], 1);
+            const uint32_t two = odd ? T::pack(other, v[c + 1]) : T::pack(v[c], other), k = row + c + odd;
+            if (k < u.rows)
+                reinterpret_cast<uint32_t *>(a.out)[((u.out_row + k) * kValueDim + (block0 + b) * 128 + warp * 32 + (lane & ~1u)) / 2] = two;
+        }
     }
-    __syncthreads();
-    if (thread < 64) {
-        const uint32_t k = thread >> 4, q = thread & 15;
-        if (row + k < u.rows)
-            reinterpret_cast<uint4 *>(a.out)[(u.out_row + row + k) * (kValueDim / 8) + blockIdx.z * 16 + q] =
-                *reinterpret_cast<const uint4 *>(&rows[k][q * 8]);
-    }
-    if (thread == 0 && blockIdx.z == 0 && a.lse != 0) {
+    if (threadIdx.x == 0 && block0 == 0 && a.lse != 0) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (row + k < u.rows)
@@ -1110,12 +1143,18 @@ Plan make_plan(const KvopsAttend &a, uint32_t lists, uint32_t nq, int sms)
     p.tiles = (p.list_end + a.drafts + kTile - 1) / kTile;
     if (p.tiles == 0) p.tiles = 1;  // no keys at all: outputs of zero
     const uint64_t units = static_cast<uint64_t>(a.max_num_reqs) * lists * p.qtiles, pairs = units * p.tiles;
-    // Whole units need no joining, equal runs of pairs leave no SM idle. In tiles' times: a unit costs
-    // its tiles and about one more for its queries and outputs, a cut unit its parts and the joining.
+    // Whole units need no joining, equal runs of pairs leave no SM idle. In tiles' times: a unit costs its
+    // tiles and about two more for its queries and outputs, a cut unit these for each part; the joining
+    // costs four and, for its sums, more with wider tiles; and runs that cut a list's query tiles in different
+    // places read its rows at different times, which costs an eighth. Whole units against runs, in us: 64
+    // requests x 128 heads 74, 97; with four tokens 272, 327; 100 requests x 128 heads x 1024 keys 76, 88; 7 x
+    // 3 lists x 24 heads x 333 keys 16.7, 18.6; but 64 requests x 16 heads 88, 57; 16 requests x 12 tokens
+    // x 16 heads 103, 62.
     const uint64_t whole = (units + sms - 1) / sms;
     const uint64_t run = (pairs + sms - 1) / sms;
-    const uint64_t cuts = run / p.tiles + 2;
-    if (p.tiles == 1 || whole * (p.tiles + 1) <= run + cuts + 3) {
+    p.run_at_most = static_cast<uint32_t>(run);
+    const uint64_t cost_runs = run + (p.qtiles > 1 ? run / 8 : 0) + 2 * (run / p.tiles + 2) + 4 + nq / 8;
+    if (p.tiles == 1 || whole * (p.tiles + 2) <= cost_runs) {
         p.whole = static_cast<uint32_t>(whole);
         p.ctas = static_cast<uint32_t>((units + whole - 1) / whole);
     } else {
@@ -1139,7 +1178,9 @@ cudaError_t launch_as(const KvopsAttend &a, const Plan &p, cudaStream_t s)
     e = cudaGetLastError();
     if (e != cudaSuccess || p.whole > 0 || p.ctas < 2) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.ctas - 1, (p.group_rows < NQ ? p.group_rows + 3 : NQ) / 4, kValueDim / kJoinThreads);
+    // All the dimensions of a row to a block where a unit has few parts, else four blocks for them.
+    const bool few = p.run_at_most * 3 >= p.tiles;
+    cfg.gridDim = dim3(p.ctas - 1, (p.group_rows < NQ ? p.group_rows + 3 : NQ) / 4, few ? 1 : 4);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -1147,7 +1188,7 @@ cudaError_t launch_as(const KvopsAttend &a, const Plan &p, cudaStream_t s)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<T, NQ>, a, p);
+    return few ? cudaLaunchKernelEx(&cfg, join_kernel<T, NQ, 4>, a, p) : cudaLaunchKernelEx(&cfg, join_kernel<T, NQ, 1>, a, p);
 }
 
 template <typename T, int NQ>
