@@ -466,7 +466,7 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
                 copy(std::integral_constant<int, 2>(), n, 2 * warp, lo, hi, rope + warp * 1024,
                      kStored ? kStoredPlain : 2 * kValueDim);
                 const int from = max(lo, 2 * warp), till = min(hi, 2 * warp + 2);
-                bring_drafts(rope, 8, 1, from, till);
+                if (from < till) bring_drafts(rope, 8, 1, from, till);
                 arrive(&sh.rope_full[half], from < till);
             };
             // this warp's group and its place
@@ -501,14 +501,23 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
                 const uint32_t to = smem + place * kGroupBytes;
                 const int from = max(lo, static_cast<int>(side) * 8), till = min(hi, static_cast<int>(side) * 8 + 8);
                 if (!(static_cast<int>(r >> 2) >= lo && static_cast<int>(r >> 2) < hi)) {
+                    // A loop, with the codes moving down to the registers that its next round reads: see
+                    // attend_kernel on instructions.
+                    constexpr int kRound = 2;
+#pragma unroll 1
+                    for (int i0 = 0; i0 < 8; i0 += kRound) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint4 &w = code[i >> 1];
-                        store16(to + (i >> 3) * kChunkBytes + r * 128 + (((i & 7) ^ (r & 7)) << 4),
-                                decode_unit<T, Code>(i & 1 ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), scale));
+                        for (int i = 0; i < 2 * kRound; ++i) {
+                            const uint4 &w = code[i >> 1];
+                            const uint32_t unit = 2 * i0 + i;
+                            store16(to + (unit >> 3) * kChunkBytes + r * 128 + (((unit & 7) ^ (r & 7)) << 4),
+                                    decode_unit<T, Code>(i & 1 ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), scale));
+                        }
+#pragma unroll
+                        for (int i = 0; i + kRound < 8; ++i) code[i] = code[i + kRound];
                     }
                 }
-                bring_drafts(to, 2 * group, 2, from, till);
+                if (from < till) bring_drafts(to, 2 * group, 2, from, till);
                 fence_async_shared();
                 mbar_arrive(smem_addr(full));
             } else {
@@ -516,7 +525,7 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
                 if (turn > 0) mbar_wait(smem_addr(&sh.empty[place]), (turn - 1) & 1, &sh.stop);
                 const uint32_t to = smem + place * kGroupBytes + side * kChunkBytes;
                 copy(std::integral_constant<int, kTile / 4>(), n, 0, lo, hi, to, warp * 128);
-                bring_drafts(to, warp, 1, lo, hi);
+                if (lo < hi) bring_drafts(to, warp, 1, lo, hi);
                 arrive(full, lo < hi);
                 bring_rope();
             }
@@ -586,7 +595,7 @@ __device__ __forceinline__ void score_warp(const Plan &plan, Shared &sh, uint32_
         const uint32_t buf = n & 1, s_at = tmem + buf * NQ;
         if (starts) mbar_wait(smem_addr(&sh.q_full), units++ & 1, &sh.stop);
         if (n > 1) mbar_wait(smem_addr(&sh.p_full[buf]), ((n >> 1) - 1) & 1, &sh.stop);
-#pragma unroll
+#pragma unroll 1
         for (int g = 0; g < 4; ++g) {
             mbar_wait(smem_addr(&sh.full[in.place]), in.turn & 1, &sh.stop);
             fence_async_shared();  // what the copies wrote
@@ -627,7 +636,7 @@ __device__ __forceinline__ void weigh_warp(const Plan &plan, Shared &sh, uint32_
         fence_async_shared();
         fence_after_sync();
         const uint64_t probs = probs0 + buf * (kChunkBytes >> 4);
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < 4; ++b) {
             const uint64_t values = values0 + out.place * (kGroupBytes >> 4);
 #pragma unroll
@@ -911,6 +920,11 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
     }
 }
 
+// The roles' code is long and each warp goes through its own once a tile, which is slow where it does not stay in
+// the instruction caches: unrolled, the products' 36 + 16 instructions with their descriptors and the
+// conversion of a row's 128 codes had warps waiting for instructions more than a quarter of the time
+// (64 requests x 128 heads 80 us, now 72; x 16 heads 42, 37; 8-bit rows 58, 48). So these are loops of short
+// bodies, and the waits' slow halves are a function.
 template <typename T, typename Code, bool kStored, int NQ>
 __global__ void __launch_bounds__(kThreads, 1)
     attend_kernel(const KvopsAttend a, const Plan plan)

@@ -34,18 +34,20 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
 // clock, since reading the global timer takes microseconds). The warp leaves together: a lane left
 // behind could find the barrier two phases on, where the parity is its own again, and wait for good.
 constexpr long long kWaitClocks = 1ll << 30;
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *stop)
+__device__ __noinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t *stop)
 {
-    if (!mbar_try(bar, parity)) {
-        const long long start = clock64();
-        while (!mbar_try(bar, parity)) {
-            if (*stop != 0) break;
-            if (clock64() - start > kWaitClocks) {
-                *stop = 1u;
-                break;
-            }
+    const long long start = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (*stop != 0) break;
+        if (clock64() - start > kWaitClocks) {
+            *stop = 1u;
+            break;
         }
     }
+}
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *stop)
+{
+    if (!mbar_try(bar, parity)) mbar_wait_on(bar, parity, stop);
     __syncwarp();
 }
 
