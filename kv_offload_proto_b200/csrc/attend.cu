@@ -150,9 +150,9 @@ struct Shared {
     float top[2][4][32];       // a tile's maxima by column, by half and lane quarter
     uint64_t tree[64];         // of the unit's query rows
     // full: rows have landed; empty: the second product is done with them; done: with a tile; rope_*:
-    // a tile's rotary dimensions, then probabilities; out_free: a unit's outputs have left that place
+    // a tile's rotary dimensions, then probabilities
     uint64_t q_full, full[kMostPlaces], empty[kMostPlaces], rope_full[2], rope_empty[2], s_full[2], p_full[2], done,
-        out_free[2], meta_full[kAhead], meta_empty[kAhead];
+        meta_full[kAhead], meta_empty[kAhead];
     uint64_t row[kAhead][kTile];  // where the tile's hot rows start, 0: no hot row
     uint8_t kind[kAhead][kTile];  // of the tile's keys: kNone, kList, kDraft or kBadDraft
     // 0 for a tile without any key, else 1 | lo << 8 | hi << 16: rows 4 lo .. 4 hi - 1 are drafted ones
@@ -240,11 +240,13 @@ struct Ring {
     }
 };
 
-// The unit's queries, K-major in blocks of 64 dimensions, rows behind the last as zeros. Waits until
-// the scores of the last unit are done with their place; warp w takes rows w, w + 8, ...
+// The unit's queries, K-major in blocks of 64 dimensions, rows behind the last as zeros; warp w takes rows w,
+// w + 8, ... The run's first unit's are always loaded, before its rows are known; a later unit's with its
+// first tile that has a key, once the `done` tiles before are done with the place (or, if there were
+// none, once the first unit's are there).
 template <int NQ>
 __device__ __forceinline__ void load_queries(const KvopsAttend &a, const Plan &plan, Shared &sh, uint32_t q_at,
-                                             const Unit &u, uint32_t done, int warp, int lane)
+                                             const Unit &u, bool later, uint32_t done, int warp, int lane)
 {
     using namespace tc;
     uint64_t from = 0;  // lane i: where row w + 8 i starts, 0: none
@@ -255,7 +257,8 @@ __device__ __forceinline__ void load_queries(const KvopsAttend &a, const Plan &p
             from = a.q + 2 * (u.req * a.q_stride_req + t * a.q_stride_token + h * a.q_stride_head);
         }
     }
-    if (done > 0) mbar_wait(smem_addr(&sh.s_full[(done - 1) & 1]), ((done - 1) >> 1) & 1, &sh.stop);
+    if (later && done > 0) mbar_wait(smem_addr(&sh.s_full[(done - 1) & 1]), ((done - 1) >> 1) & 1, &sh.stop);
+    else if (later) mbar_wait(smem_addr(&sh.q_full), 0, &sh.stop);
 #pragma unroll 4
     for (int i = 0; i < NQ / kLoadWarps; ++i) {
         const uint64_t row = __shfl_sync(0xFFFFFFFFu, from, i);
@@ -439,7 +442,10 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
     Unit u = unit_at<NQ>(plan, unit);
     Ring<L::places> ring;  // of group 0 of the tile
     bool q_loaded = false, sent = false;  // sent: the tile's codes are on their way
-    uint32_t ends0 = 0, ends1 = 0;        // units that ended in a tile of an even number, of an odd one
+    if (begin < end) {
+        load_queries<NQ>(a, plan, sh, smem + L::q, u, false, 0, warp, lane);
+        q_loaded = true;
+    }
     for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
         const uint32_t word = tile_word(sh, n);
         if (word != 0) {
@@ -458,11 +464,9 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
                 }
             };
             const auto bring_rope = [&]() {
-                // the place was the probabilities' of the tile before last, and perhaps its unit's outputs'
+                // the place was the probabilities' of the tile before last
                 const uint32_t half = done & 1, rope = smem + L::rope + half * kChunkBytes;
                 if (done > 1) mbar_wait(smem_addr(&sh.rope_empty[half]), ((done >> 1) - 1) & 1, &sh.stop);
-                const uint32_t ends = half ? ends1 : ends0;
-                if (ends > 0) mbar_wait(smem_addr(&sh.out_free[half]), (ends - 1) & 1, &sh.stop);
                 copy(std::integral_constant<int, 2>(), n, 2 * warp, lo, hi, rope + warp * 1024,
                      kStored ? kStoredPlain : 2 * kValueDim);
                 const int from = max(lo, 2 * warp), till = min(hi, 2 * warp + 2);
@@ -478,7 +482,7 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
             uint64_t *full = &sh.full[place];
             if constexpr (kStored) {
                 if (!sent) send(n, lo, hi);
-                if (first) load_queries<NQ>(a, plan, sh, smem + L::q, u, done, warp, lane);
+                if (first) load_queries<NQ>(a, plan, sh, smem + L::q, u, true, done, warp, lane);
                 copy_wait<0>();
                 __syncwarp();
                 uint4 code[8];
@@ -521,7 +525,7 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
                 fence_async_shared();
                 mbar_arrive(smem_addr(full));
             } else {
-                if (first) load_queries<NQ>(a, plan, sh, smem + L::q, u, done, warp, lane);
+                if (first) load_queries<NQ>(a, plan, sh, smem + L::q, u, true, done, warp, lane);
                 if (turn > 0) mbar_wait(smem_addr(&sh.empty[place]), (turn - 1) & 1, &sh.stop);
                 const uint32_t to = smem + place * kGroupBytes + side * kChunkBytes;
                 copy(std::integral_constant<int, kTile / 4>(), n, 0, lo, hi, to, warp * 128);
@@ -534,15 +538,9 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
             ++done;
         }
         tile_done(sh, n, lane);
-        const bool wraps = tile + 1 == plan.tiles;
-        if (wraps || at + 1 == end) {
-            // a unit's outputs go through the place of its last tile's probabilities
-            if (q_loaded) ++(done & 1 ? ends0 : ends1);
-            q_loaded = false;
-        }
-        ++tile;
-        if (wraps) {
+        if (++tile == plan.tiles) {
             tile = 0;
+            q_loaded = false;
             u = unit_at<NQ>(plan, ++unit);
         }
     }
@@ -552,7 +550,7 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
 
 // ---- the products ------------------------------------------------------------------------------
 
-// A product warp's walk over the tiles: body(starts) for each one with a key, `starts` telling whether
+// A product warp's walk over the tiles: body(starts, at) for each one with a key, `starts` telling whether
 // it is the first of its unit.
 template <typename Body>
 __device__ __forceinline__ void each_tile(const Plan &plan, Shared &sh, uint32_t begin, uint32_t end, const Body &body)
@@ -564,7 +562,7 @@ __device__ __forceinline__ void each_tile(const Plan &plan, Shared &sh, uint32_t
     for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
         const bool any = __shfl_sync(0xFFFFFFFFu, tile_word(sh, n), 0) != 0;
         tile_done(sh, n, lane);
-        if (any) body(starts);
+        if (any) body(starts, at);
         starts = !any && starts;
         if (++tile == plan.tiles) {
             tile = 0;
@@ -591,9 +589,13 @@ __device__ __forceinline__ void score_warp(const Plan &plan, Shared &sh, uint32_
     const uint64_t rotary0 = operand(smem + L::rope, 16, 1024);
     Ring<L::places> in;
     uint32_t n = 0, units = 0;
-    each_tile(plan, sh, begin, end, [&](bool starts) {
+    each_tile(plan, sh, begin, end, [&](bool starts, uint32_t at) {
         const uint32_t buf = n & 1, s_at = tmem + buf * NQ;
-        if (starts) mbar_wait(smem_addr(&sh.q_full), units++ & 1, &sh.stop);
+        if (starts) {
+            // (the first unit's queries are loaded even if it has no key)
+            if (n == 0 && at / plan.tiles != begin / plan.tiles) mbar_wait(smem_addr(&sh.q_full), units++ & 1, &sh.stop);
+            mbar_wait(smem_addr(&sh.q_full), units++ & 1, &sh.stop);
+        }
         if (n > 1) mbar_wait(smem_addr(&sh.p_full[buf]), ((n >> 1) - 1) & 1, &sh.stop);
 #pragma unroll 1
         for (int g = 0; g < 4; ++g) {
@@ -630,7 +632,7 @@ __device__ __forceinline__ void weigh_warp(const Plan &plan, Shared &sh, uint32_
     const uint64_t values0 = operand(smem, kChunkBytes, 1024), probs0 = operand(smem + L::rope, 16, 1024);
     Ring<L::places> out;
     uint32_t n = 0;
-    each_tile(plan, sh, begin, end, [&](bool starts) {
+    each_tile(plan, sh, begin, end, [&](bool starts, uint32_t) {
         const uint32_t buf = n & 1;
         mbar_wait(smem_addr(&sh.p_full[buf]), (n >> 1) & 1, &sh.stop);
         fence_async_shared();
@@ -852,11 +854,6 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
             }
             // 16 queries of 128 dimensions at a time (8, where a half has no more).
             constexpr int kRows = NH < 16 ? NH : 16;
-            // The last probabilities' place turns [dimension][query] into rows of 128 dimensions (256
-            // bytes; odd rows with their halves swapped in each 128 bytes, to keep the two rows that a
-            // pair of lanes writes in different banks).
-            const uint32_t place = (done - 1) & 1;
-            const uint32_t rows = smem + Layout<NQ, kStored>::rope + place * kChunkBytes + half * kRows * 256;
 #pragma unroll 1
             for (int b = 0; b < 4 * NH / kRows; ++b) {
                 const uint32_t block = b / (NH / kRows), first = b % (NH / kRows) * kRows;  // of the half's queries
@@ -879,38 +876,29 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                             reinterpret_cast<uint16_t *>(a.out)[(u.out_row + r0 + i) * kValueDim + block * 128 + dim] = 0;
                     continue;
                 }
-                group_barrier(1 + half, 128);
+                // A thread has one dimension of kRows queries. Four lanes exchange theirs, so that each has
+                // four dimensions of a quarter of the queries and eight lanes write 64 bytes of a row.
+                uint32_t two[kRows / 2];  // of an even lane rows 0, 2, .. with the next dimension, of an odd one rows 1, 3, ..
+                const bool odd = lane & 1, upper = lane & 2;
 #pragma unroll
                 for (int i = 0; i < kRows; i += 4) {
                     const float4 f = spread4(first + i);
                     v[i] *= f.x, v[i + 1] *= f.y, v[i + 2] *= f.z, v[i + 3] *= f.w;
 #pragma unroll
                     for (int c = i; c < i + 4; c += 2) {
-                        // an even lane takes query c of its dimension and the next, an odd one c + 1
-                        const bool odd = lane & 1;
                         const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[c] : v[c + 1], 1);
-                        const uint32_t w = odd ? T::pack(other, v[c + 1]) : T::pack(v[c], other);
-                        const uint32_t r = c + odd, word = dim >> 1;
-                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(rows + r * 256 + ((word ^ (odd ? 16 : 0)) << 2)), "r"(w)
-                                     : "memory");
+                        two[c / 2] = odd ? T::pack(other, v[c + 1]) : T::pack(v[c], other);
                     }
-                }
-                group_barrier(1 + half, 128);
-#pragma unroll
-                for (int i = 0; i < kRows / 8; ++i) {
-                    const uint32_t n = i * 128 + dim, r = n >> 4, q = n & 15;
-                    uint4 w;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                                 : "r"(rows + r * 256 + ((q ^ ((r & 1) << 2)) << 4)) : "memory");
-                    if (r0 + r < u.rows)
-                        reinterpret_cast<uint4 *>(a.out)[(u.out_row + r0 + r) * (kValueDim / 8) + block * 16 + q] = w;
+                    const uint32_t keep = upper ? two[i / 2 + 1] : two[i / 2], give = upper ? two[i / 2] : two[i / 2 + 1];
+                    const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, give, 2);
+                    const uint32_t r = r0 + i + (upper ? 2 : 0) + odd;
+                    if (r < u.rows)
+                        reinterpret_cast<uint2 *>(a.out)[(u.out_row + r) * (kValueDim / 4) + block * 32 + (dim >> 2)] =
+                            upper ? make_uint2(got, keep) : make_uint2(keep, got);
                 }
             }
-            group_barrier(1 + half, 128);
-            fence_before_sync();
-            fence_async_shared();
+            fence_before_sync();  // ahead of the next unit's first product, which its probabilities release
             __syncwarp();
-            if (started && lane == 0) mbar_arrive(smem_addr(&sh.out_free[place]));
             fresh = true;
         }
         if (++tile == plan.tiles) {
@@ -934,7 +922,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ Shared sh;
     const uint32_t smem = (smem_addr(dynamic) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // join_kernel may take its seats and wait
+    // join_kernel, or the kernel behind, may take its seats and wait. (This grid has all of its own by then, and
+    // two of its CTAs never share an SM, whose shared memory and tensor memory one fills.)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         sh.stop = 0;
         mbar_init(smem_addr(&sh.q_full), kLoadWarps * 32);
@@ -948,7 +938,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_addr(&sh.rope_empty[b]), 1);
             mbar_init(smem_addr(&sh.s_full[b]), 1);
             mbar_init(smem_addr(&sh.p_full[b]), kSoftmaxWarps);
-            mbar_init(smem_addr(&sh.out_free[b]), kSoftmaxWarps);
         }
         for (uint32_t b = 0; b < kAhead; ++b) {
             mbar_init(smem_addr(&sh.meta_full[b]), 1);
@@ -960,6 +949,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
+    // Launched as a programmatic dependent: what is above may run before the kernel ahead has ended.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t units = real_units(a, plan);
     const uint32_t run = run_length(plan, units), pairs = units * plan.tiles;
     const uint32_t begin = min(blockIdx.x * run, pairs), end = min(begin + run, pairs);
@@ -999,6 +990,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const KvopsAttend a,
 {
     constexpr uint32_t kFirst = 16 / kBlocks;  // parts fetched ahead
     __shared__ float4 weight[kJoinThreads / 32][32];  // of a part, by row
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t units = real_units(a, plan), run = run_length(plan, units), cut = (blockIdx.x + 1) * run;
     if (cut >= units * plan.tiles || cut % plan.tiles == 0) return;
@@ -1188,20 +1180,23 @@ cudaError_t launch_as(const KvopsAttend &a, const Plan &p, cudaStream_t s)
     const auto kernel = attend_kernel<T, Code, kStored, NQ>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<NQ, kStored>::bytes);
     if (e != cudaSuccess) return e;
-    kernel<<<p.ctas, kThreads, Layout<NQ, kStored>::bytes, s>>>(a, p);
-    e = cudaGetLastError();
-    if (e != cudaSuccess || p.whole > 0 || p.ctas < 2) return e;
     cudaLaunchConfig_t cfg{};
-    // All the dimensions of a row to a block where a unit has few parts, else four blocks for them.
-    const bool few = p.run_at_most * 3 >= p.tiles;
-    cfg.gridDim = dim3(p.ctas - 1, (p.group_rows < NQ ? p.group_rows + 3 : NQ) / 4, few ? 1 : 4);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    cfg.stream = s;
+    cfg.gridDim = dim3(p.ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Layout<NQ, kStored>::bytes;
+    e = cudaLaunchKernelEx(&cfg, kernel, a, p);
+    if (e != cudaSuccess || p.whole > 0 || p.ctas < 2) return e;
+    cfg.dynamicSmemBytes = 0;
+    // All the dimensions of a row to a block where a unit has few parts, else four blocks for them.
+    const bool few = p.run_at_most * 3 >= p.tiles;
+    cfg.gridDim = dim3(p.ctas - 1, (p.group_rows < NQ ? p.group_rows + 3 : NQ) / 4, few ? 1 : 4);
+    cfg.blockDim = dim3(kJoinThreads);
     return few ? cudaLaunchKernelEx(&cfg, join_kernel<T, NQ, 4>, a, p) : cudaLaunchKernelEx(&cfg, join_kernel<T, NQ, 1>, a, p);
 }
 

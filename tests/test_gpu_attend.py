@@ -133,6 +133,30 @@ def test_parity(shape, fmt, dtype):
     c.check(*c.call())
 
 
+@pytest.mark.parametrize("empty", ["first", "most", "all", "none"])
+@pytest.mark.parametrize("fmt", ["raw", "int8"])
+@pytest.mark.parametrize("B, H, K", [(400, 5, 40), (160, 130 // 2, 100), (90, 16, 700)])
+def test_requests_without_any_key_among_others(B, H, K, fmt, empty):
+    """A CTA's run has several requests (whole ones, or with ends that others share), and their queries are
+    fetched ahead of the rows that none of them may have."""
+    c = Case(31, B=B, H=H, K=K, rows=256, shared=True, fmt=fmt, holes=0.2)
+    gone = {"first": torch.arange(B, device="cuda") % 5 < 2, "most": torch.arange(B, device="cuda") % 5 != 3,
+            "all": torch.ones(B, device="cuda", dtype=torch.bool), "none": torch.zeros(B, device="cuda", dtype=torch.bool)}[empty]
+    c.slots[gone] = -1
+    c.check(*c.call())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("K, B", [(2000, 1), (2000, 40), (64 * 150, 2)])
+def test_scores_that_grow_along_the_list(K, B, dtype):
+    """Later keys score higher and higher: the running references move again and again, in whole lists and in
+    joined parts, and earlier probabilities become nothing."""
+    c = Case(32, B=B, H=17, K=K, rows=K, shared=True, dtype=dtype, holes=0.0)
+    c.slots[:] = torch.arange(K, dtype=torch.int32, device="cuda")
+    c.read *= torch.linspace(0.1, 8.0, K, device="cuda", dtype=torch.float32).to(c.read.dtype)[:, None]
+    c.check(*c.call())
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_peaked_and_large_scores(dtype):
     """Scores up to hundreds: one key takes nearly all, and the running maximum moves late."""
