@@ -12,7 +12,7 @@
 // Operands come from shared memory at 128 bytes a cycle, which bounds both products: 48 cycles for
 // 16 dimensions (or keys) at NQ = 64, 36 + 16 of them a tile. Tiles of 128 keys would take 48 cycles
 // for twice the keys in the first product, but leave no room for a second tile beside the queries:
-// rows, products and softmax then take turns (12200 cycles for 128 keys, where this takes REPLACE).
+// rows, products and softmax then take turns (12200 cycles for 128 keys, where this takes 2 x 3300).
 //
 // One CTA per SM takes a run of (query tile, key tile) pairs. Warps 0-7: the softmax, a thread per
 // key and half of the queries, and the outputs. Warps 8-15: the rows,
@@ -51,7 +51,7 @@ constexpr int kSoftmaxWarps = 8;
 
 constexpr int kLoadWarps = 8;
 constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kWeighWarp = kScoreWarp + 1, kFindWarp = kScoreWarp + 2;
-constexpr int kThreads = (kFindWarp + 1) * 32;
+constexpr int kThreads = (kFindWarp + 1) * 32;  // five warps to a scheduler leave a thread 96 registers, six 80
 constexpr uint32_t kAhead = 4;  // tiles whose rows are known at a time
 
 // A column's running reference: probabilities are 2^(score - reference), and it is set kLift (in powers of
@@ -151,7 +151,7 @@ struct Shared {
     uint64_t tree[64];         // of the unit's query rows
     // full: rows have landed; empty: the second product is done with them; done: with a tile; rope_*:
     // a tile's rotary dimensions, then probabilities
-    uint64_t q_full, full[kMostPlaces], empty[kMostPlaces], rope_full[2], rope_empty[2], s_full[2], p_full[2], done,
+    uint64_t q_full, full[kMostPlaces], empty[kMostPlaces], rope_full[2], rope_empty[2], s_full[2], p_full[2], done[2],
         meta_full[kAhead], meta_empty[kAhead];
     uint64_t row[kAhead][kTile];  // where the tile's hot rows start, 0: no hot row
     uint8_t kind[kAhead][kTile];  // of the tile's keys: kNone, kList, kDraft or kBadDraft
@@ -384,9 +384,66 @@ __device__ __forceinline__ void tile_done(Shared &sh, uint32_t n, int lane)
     if (lane == 0) tc::mbar_arrive(tc::smem_addr(&sh.meta_empty[n % kAhead]));
 }
 
+// Copies 128 bytes from byte `column` of kFours fours of rows (from `from` on, an even four) of tile n to `to`,
+// four rows an instruction, leaving out the fours [lo, hi); rows that are none become zeros.
+template <int kFours>
+__device__ __forceinline__ void copy_rows(const KvopsAttend &a, const Shared &sh, uint32_t n, int from, int lo, int hi,
+                                          uint32_t to, uint32_t column)
+{
+    constexpr int kBatch = kFours < 8 ? kFours : 8;
+    const uint32_t n16 = threadIdx.x & 7, r4 = threadIdx.x >> 3 & 3;
+    const uint64_t *row = &sh.row[n % kAhead][4 * from + r4];
+    const uint64_t add = column + n16 * 16;
+    to += r4 * 128;
+    const uint32_t even = (n16 ^ r4) << 4, odd = (n16 ^ (r4 + 4)) << 4;
+#pragma unroll
+    for (int b = 0; b < kFours; b += kBatch) {
+        uint64_t at[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) at[i] = row[4 * (b + i)];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const bool some = at[i] != 0, skip = from + b + i >= lo && from + b + i < hi;
+            if (!skip)
+                copy16(to + (b + i) * 512 + ((b + i) & 1 ? odd : even),
+                       reinterpret_cast<const uint8_t *>(some ? at[i] + add : a.q), some);
+        }
+    }
+}
+
+// Drafted rows' values from 64 * chunk on, of the fours from .. till of tile n, the tile-th of its unit, to `to`, where
+// the tile's first row is; zeros behind the last row.
+template <typename T>
+__device__ __forceinline__ void bring_drafts(const KvopsAttend &a, const Plan &plan, Shared &sh, const Unit &u, uint32_t n,
+                                             uint32_t tile, uint32_t to, uint32_t chunk, uint32_t chunks, int from, int till)
+{
+    for (uint32_t i = 4 * from * chunks * 8 + (threadIdx.x & 31); i < 4 * till * chunks * 8; i += 32) {
+        const uint32_t c16 = i & 7, c = chunks == 2 ? i >> 3 & 1 : 0, r = chunks == 2 ? i >> 4 : i >> 3;
+        const uint32_t j = tile * kTile + r - plan.list_end;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (j < a.drafts) v = draft_unit<T>(draft_row(a, u, j) + (chunk + c) * 128 + c16 * 16, &sh.kind[n % kAhead][r]);
+        store16(to + c * kChunkBytes + r * 128 + ((c16 ^ (r & 7)) << 4), v);
+    }
+}
+
+// Every lane's arrival, after its copies and (if any) the drafted rows that it stored itself.
+__device__ __forceinline__ void rows_arrive(uint64_t *bar, bool stored_some)
+{
+    using namespace tc;
+    if (stored_some) {
+        copy_close();
+        copy_wait<0>();
+        fence_async_shared();
+        mbar_arrive(smem_addr(bar));
+    } else {
+        copies_arrive(smem_addr(bar));
+    }
+}
+
 // Load warp w brings, of 16-bit rows, chunk w (64 dimensions) of all 64 rows; of stored rows, the codes
-// of group w / 2 of 32 rows, which it converts; and of either, the rotary dimensions of eight rows. Drafted rows,
-// whose first is at a multiple of four, come through registers.
+// of group w / 2 of 32 rows, which it converts; and of either, the rotary dimensions of eight rows. (A warp of
+// their own for these makes them late: they wait for the probabilities of the tile before last.) Drafted
+// rows, whose first is at a multiple of four, come through registers.
 template <typename T, typename Code, bool kStored, int NQ>
 __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &plan, Shared &sh, uint32_t smem,
                                            uint32_t begin, uint32_t end)
@@ -394,47 +451,14 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
     using namespace tc;
     using L = Layout<NQ, kStored>;
     const int warp = (threadIdx.x >> 5) - kSoftmaxWarps, lane = threadIdx.x & 31;
-    const uint32_t group = warp >> 1, side = warp & 1, n16 = lane & 7, r4 = lane >> 3;
-    // Copies 128 bytes from byte `column` of kFours fours of rows (from `from` on, an even four) of tile n to
-    // `to`, four rows an instruction, leaving out the fours [lo, hi); rows that are none become zeros.
-    const auto copy = [&](auto fours, uint32_t n, int from, int lo, int hi, uint32_t to, uint32_t column) {
-        constexpr int kFours = decltype(fours)::value, kBatch = kFours < 8 ? kFours : 8;
-        const uint64_t *row = &sh.row[n % kAhead][4 * from + r4];
-        const uint64_t add = column + n16 * 16;
-        to += r4 * 128;
-        const uint32_t even = (n16 ^ r4) << 4, odd = (n16 ^ (r4 + 4)) << 4;
-#pragma unroll
-        for (int b = 0; b < kFours; b += kBatch) {
-            uint64_t at[kBatch];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) at[i] = row[4 * (b + i)];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const bool some = at[i] != 0, skip = from + b + i >= lo && from + b + i < hi;
-                if (!skip)
-                    copy16(to + (b + i) * 512 + ((b + i) & 1 ? odd : even),
-                           reinterpret_cast<const uint8_t *>(some ? at[i] + add : a.q), some);
-            }
-        }
-    };
-    // Every lane's arrival, after its copies and (if any) the drafted rows that it stored itself.
-    const auto arrive = [&](uint64_t *bar, bool stored_some) {
-        if (stored_some) {
-            copy_close();
-            copy_wait<0>();
-            fence_async_shared();
-            mbar_arrive(smem_addr(bar));
-        } else {
-            copies_arrive(smem_addr(bar));
-        }
-    };
+    const uint32_t group = warp >> 1, side = warp & 1;
     const uint32_t stage = smem + L::stage + warp * (32 * 128);
     float next_scale = 0.f;  // stored: of row 32 side + lane, group `group`, of the codes on their way
     const auto send = [&](uint32_t n, int lo, int hi) {  // the codes of this warp's rows of tile n, and their scales
         const uint64_t mine = sh.row[n % kAhead][side * 32 + lane];
         next_scale = 0.f;
         if (mine != 0) next_scale = __ldg(reinterpret_cast<const float *>(mine + kValueDim) + group);
-        copy(std::integral_constant<int, 8>(), n, side * 8, lo, hi, stage, group * 128);
+        copy_rows<8>(a, sh, n, side * 8, lo, hi, stage, group * 128);
         copy_close();
     };
 
@@ -452,26 +476,14 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
             const int lo = word >> 8 & 0xFF, hi = word >> 16;
             const bool first = !q_loaded;
             q_loaded = true;
-            // Drafted rows' values from 64 * chunk on, of the fours from .. till; zeros behind the last row.
-            const auto bring_drafts = [&](uint32_t to, uint32_t chunk, uint32_t chunks, int from, int till) {
-                for (uint32_t i = 4 * from * chunks * 8 + lane; i < 4 * till * chunks * 8; i += 32) {
-                    const uint32_t c16 = i & 7, c = chunks == 2 ? i >> 3 & 1 : 0, r = chunks == 2 ? i >> 4 : i >> 3;
-                    const uint32_t j = tile * kTile + r - plan.list_end;
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (j < a.drafts)
-                        v = draft_unit<T>(draft_row(a, u, j) + (chunk + c) * 128 + c16 * 16, &sh.kind[n % kAhead][r]);
-                    store16(to + c * kChunkBytes + r * 128 + ((c16 ^ (r & 7)) << 4), v);
-                }
-            };
             const auto bring_rope = [&]() {
                 // the place was the probabilities' of the tile before last
                 const uint32_t half = done & 1, rope = smem + L::rope + half * kChunkBytes;
                 if (done > 1) mbar_wait(smem_addr(&sh.rope_empty[half]), ((done >> 1) - 1) & 1, &sh.stop);
-                copy(std::integral_constant<int, 2>(), n, 2 * warp, lo, hi, rope + warp * 1024,
-                     kStored ? kStoredPlain : 2 * kValueDim);
+                copy_rows<2>(a, sh, n, 2 * warp, lo, hi, rope + warp * 1024, kStored ? kStoredPlain : 2 * kValueDim);
                 const int from = max(lo, 2 * warp), till = min(hi, 2 * warp + 2);
-                if (from < till) bring_drafts(rope, 8, 1, from, till);
-                arrive(&sh.rope_full[half], from < till);
+                if (from < till) bring_drafts<T>(a, plan, sh, u, n, tile, rope, 8, 1, from, till);
+                rows_arrive(&sh.rope_full[half], from < till);
             };
             // this warp's group and its place
             uint32_t place = ring.place + group, turn = ring.turn;
@@ -521,16 +533,16 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
                         for (int i = 0; i + kRound < 8; ++i) code[i] = code[i + kRound];
                     }
                 }
-                if (from < till) bring_drafts(to, 2 * group, 2, from, till);
+                if (from < till) bring_drafts<T>(a, plan, sh, u, n, tile, to, 2 * group, 2, from, till);
                 fence_async_shared();
                 mbar_arrive(smem_addr(full));
             } else {
                 if (first) load_queries<NQ>(a, plan, sh, smem + L::q, u, true, done, warp, lane);
                 if (turn > 0) mbar_wait(smem_addr(&sh.empty[place]), (turn - 1) & 1, &sh.stop);
                 const uint32_t to = smem + place * kGroupBytes + side * kChunkBytes;
-                copy(std::integral_constant<int, kTile / 4>(), n, 0, lo, hi, to, warp * 128);
-                if (lo < hi) bring_drafts(to, warp, 1, lo, hi);
-                arrive(full, lo < hi);
+                copy_rows<kTile / 4>(a, sh, n, 0, lo, hi, to, warp * 128);
+                if (lo < hi) bring_drafts<T>(a, plan, sh, u, n, tile, to, warp, 1, lo, hi);
+                rows_arrive(full, lo < hi);
                 bring_rope();
             }
 #pragma unroll
@@ -648,7 +660,7 @@ __device__ __forceinline__ void weigh_warp(const Plan &plan, Shared &sh, uint32_
             out.next();
         }
         commit(elected, smem_addr(&sh.rope_empty[buf]));
-        commit(elected, smem_addr(&sh.done));
+        commit(elected, smem_addr(&sh.done[buf]));
         ++n;
     });
 }
@@ -689,6 +701,9 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                      : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(smem_addr(mine + i)) : "memory");
         return f;
     };
+    const auto ended = [&](uint32_t n) {  // waits until the second product of the n-th tile (with a key) has ended
+        mbar_wait(smem_addr(&sh.done[n & 1]), (n >> 1) & 1, &sh.stop);
+    };
     uint32_t done = 0, unit = begin / plan.tiles, tile = begin - unit * plan.tiles, start_tile = tile;
     bool fresh = true, started = false, open = false;
     Unit u{};
@@ -721,7 +736,6 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
         }
         const uint8_t kind[2] = {*const_cast<volatile uint8_t *>(&sh.kind[meta % kAhead][key]),
                                  *const_cast<volatile uint8_t *>(&sh.kind[meta % kAhead][key + 8])};
-        tile_done(sh, meta, lane);
         if (any) {
             // The scores in powers of two, then less their references, then probabilities.
             float y[4 * kBlocks];
@@ -788,7 +802,7 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 if (move) ref = top - kLift<T>;
                 if (started && __any_sync(0xFFFFFFFFu, move)) {
                     spread(move ? exp2_fast(was - ref) : 1.f);
-                    mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
+                    ended(done - 1);
                     fence_after_sync();
 #pragma unroll
                     for (int b = 0; b < kBlocks; ++b) {
@@ -813,18 +827,20 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 lower();
                 write();
             }
-#pragma unroll
-            for (int i = 0; i < 2 * kBlocks; ++i) sum[i] += y[4 * (i >> 1) + (i & 1)] + y[4 * (i >> 1) + 2 + (i & 1)];
-            // Every tile's end is waited for in its turn, since a parity only tells a phase from its
-            // neighbours. This one was reached before the next tile's first product, as a rule.
-            if (done > 0) mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
             fence_async_shared();
             fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&sh.p_full[done & 1]));
+            // Off the way to the second product: the sums, and the wait for the end of the tile before. Every
+            // tile's is waited for in its turn, since a parity only tells a phase from its neighbours, and
+            // before the next tile of the same parity can end, which needs this warp's next arrival.
+#pragma unroll
+            for (int i = 0; i < 2 * kBlocks; ++i) sum[i] += y[4 * (i >> 1) + (i & 1)] + y[4 * (i >> 1) + 2 + (i & 1)];
+            if (done > 0) ended(done - 1);
             started = true;
             ++done;
         }
+        tile_done(sh, meta, lane);
         const bool ends = tile + 1 == plan.tiles;
         if (ends || at + 1 == end) {
             const bool complete = ends && start_tile == 0;
@@ -849,7 +865,7 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
             if (lane < NH) mine[lane] = total == 0.f ? 0.f : 1.f / total;
             __syncwarp();
             if (started) {
-                mbar_wait(smem_addr(&sh.done), (done - 1) & 1, &sh.stop);
+                ended(done - 1);
                 fence_after_sync();
             }
             // 16 queries of 128 dimensions at a time (8, where a half has no more).
@@ -932,11 +948,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_addr(&sh.full[g]), 2 * 32);
             mbar_init(smem_addr(&sh.empty[g]), 1);
         }
-        mbar_init(smem_addr(&sh.done), 1);
         for (int b = 0; b < 2; ++b) {
             mbar_init(smem_addr(&sh.rope_full[b]), kLoadWarps * 32);
             mbar_init(smem_addr(&sh.rope_empty[b]), 1);
             mbar_init(smem_addr(&sh.s_full[b]), 1);
+            mbar_init(smem_addr(&sh.done[b]), 1);
             mbar_init(smem_addr(&sh.p_full[b]), kSoftmaxWarps);
         }
         for (uint32_t b = 0; b < kAhead; ++b) {
@@ -1264,7 +1280,8 @@ extern "C" int kvops_attend_hot(const KvopsAttend *a, uint64_t stream)
     const uint32_t lists = a->tokens > 1 && a->slots_stride_token != 0 && a->top_k > 0 ? a->tokens : 1;
     const uint32_t nq = kvb::queries_per_tile(*a, lists, sms);
     kvb::Plan p = kvb::make_plan(*a, lists, nq, sms);
-    if (static_cast<uint64_t>(a->max_num_reqs) * lists * p.qtiles * p.tiles >= (1ull << 32))
+    // (the end of a CTA's run is a 32-bit number, rounded up to a whole run for each CTA)
+    if (static_cast<uint64_t>(a->max_num_reqs) * lists * p.qtiles * p.tiles >= (1ull << 31))
         return invalid("attend_hot: requests x lists x keys out of range");
     const uint64_t need = kvb::workspace_of(p, nq);
     if (need > 0) {
