@@ -15,6 +15,10 @@ Differences from the reference, each on purpose:
     decode-extension slots (-2-off) mapped to the kernel's padded+off before comparing, and
     one model state per (layer, request): the reference keeps one per request, which matches
     the kernels' per-layer state only when --layers is 1 (the loop alternates layers).
+  * --row-format stores the pool's rows in 8 bits (the rows then hold finite fp16 values, and the spot check allows
+    for their rounding); --attend-heads runs each step's attention over the hot rows that the step's top-K
+    names (512 + 64 values a row, per-request hot rows), with --draft-tokens tokens verified along a chain of
+    drafted rows, and checks the first request's outputs against the formula in 64 bits.
 The top-K sampler is the reference's numpy sequence (workload.ref_topk_batch), so a seed
 feeds the same positions the reference driver would.
 """
@@ -54,6 +58,9 @@ def parse_args(argv=None):
     p.add_argument("--injective", action="store_true",
                    help="collision-free stripe map (with the reference map and --stripe-rows > 1 the rows of a "
                         "stripe share one segment row, so checks fail)")
+    p.add_argument("--row-format", choices=["raw", "e4m3", "int8"], default="raw", help="how the pool stores rows")
+    p.add_argument("--attend-heads", type=int, default=0, help="heads of each step's attention over the hot rows (0: none)")
+    p.add_argument("--draft-tokens", type=int, default=1, help="tokens that a step's attention verifies")
     p.add_argument("--run-dir", default="./log")
     return p.parse_args(argv)
 
@@ -120,14 +127,45 @@ class SieveChecker:
         return slots, miss
 
 
-def _fill_fingerprints(torch, hbm, layer, rows, row_words32):
+FINITE = 0xBFFFBFFF  # both fp16 numbers of a fingerprint word without the top bit of their exponents: below 2
+
+
+def _fill_fingerprints(torch, hbm, layer, rows, row_words32, mask=0xFFFFFFFF):
     """hbm[layer, rows] = fingerprint words (xds_decode.py:177-181) computed on the GPU (the
     uint64 arithmetic of the reference in int64, whose low 32 bits are the same)."""
     r = torch.as_tensor(rows, dtype=torch.int64, device=hbm.device)
     v = ((r * P1 + layer * P2) * M1) ^ M2
     k = torch.arange(row_words32, dtype=torch.int64, device=hbm.device) * M1
-    w = (v[:, None] + k[None, :]) & 0xFFFFFFFF
+    w = (v[:, None] + k[None, :]) & mask
     hbm[layer, r] = torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)  # same 32 bits
+
+
+def row_matches(got, want, row_format, quant):
+    """Whether fp16 row `got` is `want`, or what a pool row of 8 bits may read back as in its first `quant` values:
+    off by half a step of the code at the most, and by fp16's own rounding."""
+    if row_format == "raw":
+        return np.array_equal(got.view(np.uint16), want.view(np.uint16))
+    if not np.array_equal(got[quant:].view(np.uint16), want[quant:].view(np.uint16)):
+        return False
+    g, w = got[:quant].astype(np.float64).reshape(-1, 128), want[:quant].astype(np.float64).reshape(-1, 128)
+    top = np.abs(w).max(1, keepdims=True)
+    step = top / 254 if row_format == "int8" else np.maximum(np.abs(w) * 2.0 ** -4, top / 448 * 2.0 ** -10)
+    return bool((np.abs(g - w) <= step * (1 + 2.0 ** -10) + np.abs(w) * 2.0 ** -10 + 2.0 ** -24).all())
+
+
+def attention_error(torch, q, keys, scale, drafts, out, lse):
+    """The largest error of one request's attention, in units of what fp16 and the sums may be off by: q [T, H, 576], keys
+    [K, 576] (hot rows), drafts [T, 576] or None (token t sees 0..t), out [T, H, 512], lse [T, H]."""
+    worst = 0.0
+    for t in range(q.shape[0]):
+        k = keys if drafts is None else torch.cat([keys, drafts[:t + 1]])
+        k = k.double()
+        s = q[t].double() @ k.T * scale
+        p = torch.softmax(s, 1)
+        room = 2.0 ** -8 * (p @ k[:, :512].abs()) + 2.0 ** -24
+        worst = max(worst, float(((out[t].double() - p @ k[:, :512]).abs() / room).max()),
+                    float(((lse[t].double() - torch.logsumexp(s, 1)).abs() / 2.0 ** -9).max()))
+    return worst
 
 
 def main(argv=None):
@@ -140,6 +178,16 @@ def main(argv=None):
     dbs = args.device_buffer_size
     if dbs >= args.prefill:
         log("[xds][WARN] device-buffer-size >= prefill: no misses, --miss-ratio has no effect")
+    heads, tokens, quant = args.attend_heads, args.draft_tokens, args.kv_lora_rank
+    if heads and (args.kv_lora_rank != 512 or args.qk_rope != 64 or args.shared_hot or not 0 < heads <= 128 or
+                  not 0 < tokens <= 64):
+        log("[xds][ERROR] --attend-heads (1..128) needs rows of 512 + 64 values, per-request hot rows and 1..64 draft tokens")
+        return 1
+    if args.row_format != "raw" and (quant % 128 or args.qk_rope % 8):
+        log("[xds][ERROR] --row-format {} needs a kv-lora-rank of groups of 128 and a qk-rope of groups of 8".format(
+            args.row_format))
+        return 1
+    mask = 0xFFFFFFFF if args.row_format == "raw" and not heads else FINITE
     import torch
 
     import kv_offload_proto_b200 as kp
@@ -160,7 +208,7 @@ def main(argv=None):
     hbm = torch.zeros((args.layers, args.layer_rows, words32), dtype=torch.int32, device=dev)
     devices = [int(x) for x in args.segment_devices.split(",") if x.strip() != ""]
     pool = DevicePool(args.device, args.layers, args.layer_rows, row_bytes, args.stripe_rows, segment_devices=devices,
-                      injective=args.injective)
+                      injective=args.injective, row_format=args.row_format, plain_elems=row_bytes // 2 - quant)
     log("[xds] pool ready: nodes={} perLayerSegRows={} channels={} fatbin={}".format(
         pool.node_num, pool.per_layer_seg_rows, len(pool.channels), "(linked in)"))
     coord = XdsOffloadCoordinator(dev, args.layers, args.req_num, dbs, args.topk, args.req_num, args.prefill)
@@ -176,7 +224,7 @@ def main(argv=None):
         assert rows == list(range(rows[0], rows[0] + args.prefill)), "row contiguity contract broken"
         host_bases.append(rows[0])
         for layer in range(args.layers):
-            _fill_fingerprints(torch, hbm, layer, rows, words32)
+            _fill_fingerprints(torch, hbm, layer, rows, words32, mask)
     st = pool.batch_write_alllayers(0, args.req_num * args.prefill, hbm[0, 0], args.layer_rows * row_bytes)
     pool.wait(st)
     t_export = time.perf_counter() - t0
@@ -195,7 +243,8 @@ def main(argv=None):
     req_pool_indices = torch.arange(args.req_num, dtype=torch.int64, device=dev)
     coord.set_batch(req_pool_indices, seq_lens)
     stride = dbs if strided else 0
-    total_miss, t_read_total = 0, 0.0
+    total_miss, t_read_total, t_attend_total = 0, 0.0, 0.0
+    gen = torch.Generator(device=dev).manual_seed(args.seed)
     stream = torch.cuda.current_stream(dev).cuda_stream
     for step in range(args.steps):
         batch = ref_topk_batch(rng, args.req_num, args.topk, args.prefill, dbs, args.miss_ratio)
@@ -239,18 +288,43 @@ def main(argv=None):
                 continue
             row = host_bases[r] + int(batch[r][k])
             got = int(hot_h[r * stride + slot, 0])
-            if got != row_word(row, layer, 0):
+            if mask != 0xFFFFFFFF:
+                want = np.array([row_word(row, layer, i) & mask for i in range(words32)], np.uint32)
+                same = row_matches(hot_h[r * stride + slot].view(np.float16), want.view(np.float16), args.row_format, quant)
+            else:
+                same = got == row_word(row, layer, 0)
+            if not same:
                 log("[xds][ERROR] verify failed step={} layer={} req={} token={} row={} slot={} expect={} got={}".format(
                     step, layer, r, int(batch[r][k]), row, slot, row_word(row, layer, 0), got))
                 return 1
             checked += 1
         log("[xds] step {}: layer={} miss={} rows in {:.1f} us (checked={})".format(step, layer, miss_cnt, dt * 1e6,
                                                                                   checked))
+        if heads:
+            q = torch.randn((args.req_num, tokens, heads, 576), generator=gen, device=dev).half()
+            drafts = torch.randn((args.req_num, tokens, 576), generator=gen, device=dev).half() if tokens > 1 else None
+            rows16 = hot.view(torch.float16)
+            torch.cuda.synchronize(dev)
+            t0 = time.perf_counter()
+            out, lse = coord.attend(q, rows16, hot_req_stride_rows=dbs, scale=576 ** -0.5, draft_rows=drafts)
+            torch.cuda.synchronize(dev)
+            dt = time.perf_counter() - t0
+            t_attend_total += dt
+            at = slots_h[0][(slots_h[0] >= 0) & (slots_h[0] < dbs)]
+            off = attention_error(torch, q[0], rows16[torch.from_numpy(at).long().to(dev)], 576 ** -0.5,
+                                  None if drafts is None else drafts[0], out[0], lse[0])
+            if not off <= 1.0:
+                log("[xds][ERROR] attention off by {:.2f} of its tolerance, step={} layer={}".format(off, step, layer))
+                return 1
+            log("[xds] step {}: attended {} tokens x {} heads of {} requests in {:.1f} us (error {:.2f} of tolerance)".format(
+                step, tokens, heads, args.req_num, dt * 1e6, off))
     if total_miss > 0:
         log("[xds] summary: imported {} miss rows, avg {:.1f} us/row, aggregate {:.2f} GB/s".format(
             total_miss, t_read_total * 1e6 / total_miss, total_miss * row_bytes / t_read_total / 1e9))
     else:
         log("[xds] summary: no miss rows imported")
+    if heads:
+        log("[xds] summary: attention avg {:.1f} us".format(t_attend_total * 1e6 / max(args.steps, 1)))
     pool.destroy()
     log("[xds] all done, log: {}".format(log.path))
     log.close()
