@@ -457,7 +457,8 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
     const auto send = [&](uint32_t n, int lo, int hi) {  // the codes of this warp's rows of tile n, and their scales
         const uint64_t mine = sh.row[n % kAhead][side * 32 + lane];
         next_scale = 0.f;
-        if (mine != 0) next_scale = __ldg(reinterpret_cast<const float *>(mine + kValueDim) + group);
+        // (not the read-only path: the kernel ahead may write the rows while this one has begun and waits)
+        if (mine != 0) next_scale = reinterpret_cast<const float *>(mine + kValueDim)[group];
         copy_rows<8>(a, sh, n, side * 8, lo, hi, stage, group * 128);
         copy_close();
     };

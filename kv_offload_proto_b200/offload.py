@@ -88,6 +88,8 @@ class XdsOffloadCoordinator:
         self.num_real = torch.zeros(1, dtype=torch.int32, device=dev)
         self._req_pool_indices = None
         self._seq_lens = None
+        # pinned, where attend's launches leave their first errCode (made here, not in a call that may be captured)
+        self._attend_err = torch.zeros(1, dtype=torch.int32, pin_memory=True).numpy() if dev.type == "cuda" else None
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream if self.device.type == "cuda" else 0
@@ -159,6 +161,13 @@ class XdsOffloadCoordinator:
         """Device-side miss count tensor (xds_offload.py:103-106)."""
         return self.is_miss.sum()
 
+    def attend_error(self):
+        """The first errCode that a launch of attend() left since the last look (0: none), which clears it."""
+        if self._attend_err is None:
+            return 0
+        code, self._attend_err[0] = int(self._attend_err[0]), 0
+        return code
+
     def attend(self, q, hot_row_base, *, hot_req_stride_rows=0, hot_rows=None, row_format="raw", scale=None,
                topk_device_slots=None, draft_rows=None, tree=None, out=None, lse=None, workspace=None, stream=None,
                err_word=0):
@@ -179,7 +188,9 @@ class XdsOffloadCoordinator:
         batch rows below num_real only. A token without any key gets out 0 and lse -inf. out, lse
         and workspace (uint8, at least _kvops.attend_workspace(...) bytes, used by one call at a
         time) may be given; otherwise they are allocated for the call. err_word: address (or int32
-        tensor) of a word that receives errCode 0x103 if a wait inside the kernel gave up."""
+        tensor) of a word that receives errCode 0x103 if a wait inside the kernel gave up, which leaves
+        outputs undefined; by default a word of the coordinator's, whose code the next call raises
+        (and `attend_error()` returns, once the launch has ended)."""
         shape = q.shape
         squeeze = len(shape) == 3
         if squeeze:
@@ -232,6 +243,10 @@ class XdsOffloadCoordinator:
         for x in (q, slots, draft_rows, tree, out, lse, workspace):
             if x is not None and x.device != dev:
                 raise ValueError("attend: every tensor must be on {}".format(dev))
+        if err_word == 0 and dev.type == "cuda":
+            if self._attend_err[0] != 0:
+                raise RuntimeError("attend: a wait inside an earlier call gave up (errCode 0x{:x})".format(self.attend_error()))
+            err_word = self._attend_err.ctypes.data
         with contextlib.ExitStack() as stack:
             if dev.type == "cuda":
                 if torch.cuda.current_device() != dev.index:

@@ -332,6 +332,95 @@ def test_captured_and_replayed():
             assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
 
 
+def test_captured_first_behind_a_copy_and_behind_a_join_of_streams():
+    """The launch is a programmatic dependent of the kernel before it: a graph whose node before is none, a copy, or two
+    streams' ends has to order it all the same."""
+    c = Case(33, B=3, T=2, H=64, K=900, D=2, rows=1000)
+    new_q, new_slots = torch.randn_like(c.q), torch.randint(-1, 1000, c.slots.shape, device="cuda", dtype=torch.int32)
+    c.call()
+    first, copy, join = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        o1 = c.call()
+    with torch.cuda.graph(copy):
+        c.q.copy_(new_q)  # (a copy node)
+        o2 = c.call()
+        again = c.call()
+    side = torch.cuda.Stream()
+    with torch.cuda.graph(join):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            c.slots.copy_(new_slots)
+        c.q.mul_(0.5)
+        here.wait_stream(side)
+        o3 = c.call()
+    first.replay()
+    torch.cuda.synchronize()
+    c.check(*o1)
+    copy.replay()
+    torch.cuda.synchronize()
+    c.check(*o2)
+    assert torch.equal(again[0], o2[0]) and torch.equal(again[1], o2[1])
+    join.replay()
+    torch.cuda.synchronize()
+    c.check(*o3)
+
+
+def test_behind_an_event_of_another_stream_and_behind_kernels_that_write_its_inputs():
+    c = Case(34, B=8, T=1, H=16, K=2000, rows=2000, dtype="bf16")  # (a list that is cut and joined)
+    q0, hot0 = c.q.clone(), c.hot.clone()
+    want = c.call()
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        c.q.zero_()
+        c.hot.zero_()
+        ready = torch.cuda.Event()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            torch.cuda._sleep(200_000)
+            c.hot.copy_(hot0)
+            ready.record()
+        torch.mul(q0, 1.0, out=c.q)
+        torch.cuda.current_stream().wait_event(ready)
+        got = c.call()
+        again = c.call(q=c.q, out=torch.empty_like(got[0]))
+        c.q.zero_()  # after both
+        assert torch.equal(got[0], want[0]) and torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+def test_one_workspace_and_outputs_for_calls_in_a_row():
+    c = Case(35, B=2, T=1, H=128, K=4000, rows=4000)
+    need = kv().attend_workspace(2, 1, 128, 4000, 0)
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    out, lse = torch.empty((2, 128, 512), dtype=torch.float16, device="cuda"), torch.empty((2, 128), device="cuda")
+    qs = [torch.randn_like(c.q) for _ in range(6)]
+    want = [c.call(q=q)[0].clone() for q in qs]
+    got = [c.call(q=q, out=out, lse=lse, workspace=ws)[0].clone() for q in qs]
+    for w, g in zip(want, got):
+        assert torch.equal(w.view_as(g), g)
+    assert c.co.attend_error() == 0
+
+
+def test_an_earlier_launch_that_gave_up_is_raised_by_the_next_call():
+    c = Case(36)
+    c.call()
+    torch.cuda.synchronize()
+    c.co._attend_err[0] = 0x103  # as the kernel leaves it
+    with pytest.raises(RuntimeError, match="0x103"):
+        c.call()
+    assert c.co.attend_error() == 0
+    c.check(*c.call())
+
+
+def test_hot_rows_elsewhere_are_refused():
+    c = Case(37)
+    with pytest.raises(ValueError, match="hot rows must be on"):
+        c.call(hot=c.hot.cpu())
+    with pytest.raises(ValueError, match="every tensor must be on"):
+        c.call(topk_device_slots=c.slots.cpu())
+
+
 def test_c_refusals():
     mod = kv()
     c = Case(19, B=2, T=1, H=4, K=16, D=1)
@@ -356,6 +445,9 @@ def test_c_refusals():
         (dict(tokens=0), "tokens"), (dict(tokens=65), "tokens"), (dict(heads=0), "heads"), (dict(heads=129), "heads"),
         (dict(drafts=65), "drafts"), (dict(top_k=(1 << 24) + 1), "out of range"),
         (dict(max_num_reqs=(1 << 16) + 1), "out of range"),
+        # 2^16 requests x 64 lists of 2^18 tiles: more pairs than a 32-bit number counts
+        (dict(max_num_reqs=1 << 16, tokens=64, slots_stride_token=16, top_k=1 << 24), "keys out of range"),
+        (dict(max_num_reqs=1 << 16, top_k=(1 << 24) - 64 * 8), "the workspace|keys out of range"),
     ]:
         with pytest.raises(RuntimeError, match=message):
             mod.attend_hot(**{**good, **change})
