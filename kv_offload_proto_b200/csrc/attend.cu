@@ -1145,14 +1145,17 @@ int sm_count()
 }
 
 // Queries per tile. A pair costs about the same for any number up to 64 (the rows' way into shared
-// memory), so a tile takes as many as there are, unless smaller tiles keep more SMs busy.
+// memory), so a tile takes as many as there are, unless there is little to do: then smaller tiles, whose
+// queries and outputs are fewer, are sooner done, up to four pairs an SM. Queries a tile, in us, for 128
+// heads x 2048 keys: one request 16: 14.1, 32: 18.4, 64: 19.5; four requests 23.3, 21.0, 24.2; one request's four
+// tokens 24.9, 23.2, 28.5.
 uint32_t queries_per_tile(const KvopsAttend &a, uint32_t lists, int sms)
 {
     const uint32_t rows = a.heads * (lists > 1 ? 1 : a.tokens);
     uint32_t nq = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     const uint64_t lists_all = static_cast<uint64_t>(a.max_num_reqs) * lists;
     const uint64_t tiles = (a.top_k + a.drafts + kTile - 1) / kTile;
-    while (nq > 16 && lists_all * ((rows + nq / 2 - 1) / (nq / 2)) * tiles <= static_cast<uint64_t>(sms)) nq /= 2;
+    while (nq > 16 && lists_all * ((rows + nq / 2 - 1) / (nq / 2)) * tiles <= 4 * static_cast<uint64_t>(sms)) nq /= 2;
     return nq;
 }
 
@@ -1168,15 +1171,15 @@ Plan make_plan(const KvopsAttend &a, uint32_t lists, uint32_t nq, int sms)
     const uint64_t units = static_cast<uint64_t>(a.max_num_reqs) * lists * p.qtiles, pairs = units * p.tiles;
     // Whole units need no joining, equal runs of pairs leave no SM idle. In tiles' times: a unit costs its
     // tiles and about two more for its queries and outputs, a cut unit these for each part; the joining
-    // costs four and, for its sums, more with wider tiles; and runs that cut a list's query tiles in different
-    // places read its rows at different times, which costs an eighth. Whole units against runs, in us: 64
-    // requests x 128 heads 74, 97; with four tokens 272, 327; 100 requests x 128 heads x 1024 keys 76, 88; 7 x
-    // 3 lists x 24 heads x 333 keys 16.7, 18.6; but 64 requests x 16 heads 88, 57; 16 requests x 12 tokens
-    // x 16 heads 103, 62.
+    // costs six; and runs that cut a list's query tiles in different places read its rows at different
+    // times, which costs an eighth. Whole units against runs, in us: 64 requests x 128 heads x 2048 8-bit keys 89,
+    // 97; 100 requests x 128 heads x 1024 keys 73, 76; 130 requests x 16 heads 55, 61; 7 x 3 lists x 24
+    // heads x 333 keys 14.8, 15.9; but 40 requests x 128 heads 67, 57; 80 requests 129, 98; 100 requests x
+    // 16 heads 54, 47; 64 requests x 16 heads 80, 45.
     const uint64_t whole = (units + sms - 1) / sms;
     const uint64_t run = (pairs + sms - 1) / sms;
     p.run_at_most = static_cast<uint32_t>(run);
-    const uint64_t cost_runs = run + (p.qtiles > 1 ? run / 8 : 0) + 2 * (run / p.tiles + 2) + 4 + nq / 8;
+    const uint64_t cost_runs = run + (p.qtiles > 1 ? run / 8 : 0) + 2 * (run / p.tiles + 2) + 6;
     if (p.tiles == 1 || whole * (p.tiles + 2) <= cost_runs) {
         p.whole = static_cast<uint32_t>(whole);
         p.ctas = static_cast<uint32_t>((units + whole - 1) / whole);
