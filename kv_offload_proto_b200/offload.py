@@ -90,6 +90,7 @@ class XdsOffloadCoordinator:
         self._seq_lens = None
         # pinned, where attend's launches leave their first errCode (made here, not in a call that may be captured)
         self._attend_err = torch.zeros(1, dtype=torch.int32, pin_memory=True).numpy() if dev.type == "cuda" else None
+        self._attend_err_at = self._attend_err.ctypes.data if dev.type == "cuda" else 0
 
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream if self.device.type == "cuda" else 0
@@ -191,15 +192,14 @@ class XdsOffloadCoordinator:
         tensor) of a word that receives errCode 0x103 if a wait inside the kernel gave up, which leaves
         outputs undefined; by default a word of the coordinator's, whose code the next call raises
         (and `attend_error()` returns, once the launch has ended)."""
-        shape = q.shape
+        shape, strides = q.shape, q.stride()
         squeeze = len(shape) == 3
-        if squeeze:
-            q = q.unsqueeze(1)
-            shape = q.shape
-        strides = q.stride()
-        if len(shape) != 4 or shape[3] != KEY_DIM or strides[3] != 1:
+        if len(shape) not in (3, 4) or shape[-1] != KEY_DIM or strides[-1] != 1:
             raise ValueError("attend: q must be [B, heads, 576] or [B, tokens, heads, 576] with unit last stride")
-        B, T, H, _ = shape
+        if squeeze:
+            (B, H, _), T, strides = shape, 1, (strides[0], 0, strides[1])
+        else:
+            B, T, H, _ = shape
         dtype = dtype_name(q.dtype)
         if B > self.max_num_reqs:
             raise ValueError("attend: {} batch rows, max_num_reqs is {}".format(B, self.max_num_reqs))
@@ -246,33 +246,41 @@ class XdsOffloadCoordinator:
         if err_word == 0 and dev.type == "cuda":
             if self._attend_err[0] != 0:
                 raise RuntimeError("attend: a wait inside an earlier call gave up (errCode 0x{:x})".format(self.attend_error()))
-            err_word = self._attend_err.ctypes.data
-        with contextlib.ExitStack() as stack:
-            if dev.type == "cuda":
-                if torch.cuda.current_device() != dev.index:
-                    stack.enter_context(torch.cuda.device(dev))
-                if stream is None:
-                    stream = torch._C._cuda_getCurrentRawStream(dev.index)  # (no Stream object: 4 us of a 25 us call)
-                elif out is None or lse is None or workspace is None:
-                    # what is allocated below belongs to the stream that uses it
-                    stack.enter_context(torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev)))
-            if out is None:
-                out = q.new_empty((B, H, VALUE_DIM) if squeeze else (B, T, H, VALUE_DIM))
-            if lse is None:
-                lse = q.new_empty((B, H) if squeeze else (B, T, H), dtype=torch.float32)
-            room = workspace.numel() if workspace is not None else 0
-            if workspace is None:
-                room = self._k.attend_workspace(B, T, H, K, D, row_format, dtype)
-                if room:
-                    workspace = q.new_empty(room, dtype=torch.uint8)
-            # (the stride of a dimension of one entry is never used)
-            self._k.attend_hot(
-                q.data_ptr(), strides[0] if B > 1 else 0, strides[1] if T > 1 else 0, strides[2] if H > 1 else 0, hot,
-                hot_req_stride_rows, hot_rows, self._req_pool_indices.data_ptr(), self.pool_size, slots.data_ptr(),
-                s_strides[0] if s_shape[0] > 1 else 0, s_strides[1] if len(s_shape) == 3 and T > 1 else 0,
-                self.num_real.data_ptr(), draft_at, draft_strides[0], draft_strides[1],
-                tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
-                workspace.data_ptr() if room else 0, room, B, T, H, K, D, row_format, dtype,
-                KEY_DIM ** -0.5 if scale is None else scale, stream or 0,
-                err_word=err_word if isinstance(err_word, int) else err_word.data_ptr())
+            err_word = self._attend_err_at
+        args = (q, B, T, H, K, D, squeeze, strides, slots, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale,
+                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word)
+        if dev.type == "cuda" and (stream is not None or torch.cuda.current_device() != dev.index):
+            with torch.cuda.device(dev):
+                if stream is None or (out is not None and lse is not None and workspace is not None):
+                    return self._attend(*args)
+                # what is allocated below belongs to the stream that uses it
+                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev)):
+                    return self._attend(*args)
+        return self._attend(*args)
+
+    def _attend(self, q, B, T, H, K, D, squeeze, strides, slots, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale,
+                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word):
+        """attend() on checked arguments and the current device."""
+        if stream is None:  # (no Stream object: 4 us of a 20 us call)
+            stream = torch._C._cuda_getCurrentRawStream(q.device.index) if q.is_cuda else 0
+        s_shape, s_strides = slots.shape, slots.stride()
+        if out is None:
+            out = q.new_empty((B, H, VALUE_DIM) if squeeze else (B, T, H, VALUE_DIM))
+        if lse is None:
+            lse = q.new_empty((B, H) if squeeze else (B, T, H), dtype=torch.float32)
+        room = workspace.numel() if workspace is not None else 0
+        if workspace is None:
+            room = self._k.attend_workspace(B, T, H, K, D, row_format, dtype)
+            if room:
+                workspace = q.new_empty(room, dtype=torch.uint8)
+        # (the stride of a dimension of one entry is never used)
+        self._k.attend_hot(
+            q.data_ptr(), strides[0] if B > 1 else 0, strides[1] if T > 1 else 0, strides[2] if H > 1 else 0, hot,
+            hot_req_stride_rows, hot_rows, self._req_pool_indices.data_ptr(), self.pool_size, slots.data_ptr(),
+            s_strides[0] if s_shape[0] > 1 else 0, s_strides[1] if len(s_shape) == 3 and T > 1 else 0,
+            self.num_real.data_ptr(), draft_at, draft_strides[0], draft_strides[1],
+            tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
+            workspace.data_ptr() if room else 0, room, B, T, H, K, D, row_format, dtype,
+            KEY_DIM ** -0.5 if scale is None else scale, stream,
+            err_word=err_word if isinstance(err_word, int) else err_word.data_ptr())
         return out, lse
