@@ -372,11 +372,13 @@ __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan
     }
 }
 
-// The word of the n-th tile of the run, once it is known; and the end of its use.
+// The word of the n-th tile of the run, once it is known, the same in every lane; and the end of its use.
+// After a wait has given up no tile has a key: its rows' addresses may never have been written.
 __device__ __forceinline__ uint32_t tile_word(Shared &sh, uint32_t n)
 {
     tc::mbar_wait(tc::smem_addr(&sh.meta_full[n % kAhead]), (n / kAhead) & 1, &sh.stop);
-    return *const_cast<volatile uint32_t *>(&sh.tile[n % kAhead]);
+    const uint32_t word = *const_cast<volatile uint32_t *>(&sh.tile[n % kAhead]);
+    return __shfl_sync(0xFFFFFFFFu, *const_cast<volatile uint32_t *>(&sh.stop) != 0 ? 0u : word, 0);
 }
 __device__ __forceinline__ void tile_done(Shared &sh, uint32_t n, int lane)
 {
@@ -573,7 +575,7 @@ __device__ __forceinline__ void each_tile(const Plan &plan, Shared &sh, uint32_t
     bool starts = true;
     const int lane = threadIdx.x & 31;
     for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
-        const bool any = __shfl_sync(0xFFFFFFFFu, tile_word(sh, n), 0) != 0;
+        const bool any = tile_word(sh, n) != 0;
         tile_done(sh, n, lane);
         if (any) body(starts, at);
         starts = !any && starts;
