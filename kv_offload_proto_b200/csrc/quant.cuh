@@ -20,6 +20,22 @@
 
 namespace kvb {
 
+// Two fp32 products, or sums, in one instruction (each rounded as __fmul_rn and __fadd_rn do).
+__device__ __forceinline__ float2 mul2(const float2 &a, const float2 &b)
+{
+    float2 d;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(const float2 &a, const float2 &b)
+{
+    float2 d;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // The 16-bit types of rows.
 struct Fp16 {
     static constexpr uint32_t kInf = 0x7C00u;  // magnitude bits from which a value is not finite
@@ -77,11 +93,12 @@ struct Int8 {
     __device__ static __forceinline__ float4 decode4(uint32_t v)
     {
         const uint32_t u = v ^ 0x80808080u;
-        const float k = 8388608.f + 128.f;
-        return make_float4(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)) - k,
-                           __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)) - k,
-                           __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)) - k,
-                           __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - k);
+        const float2 k = make_float2(-(8388608.f + 128.f), -(8388608.f + 128.f));
+        const float2 x = add2(make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)),
+                                          __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441))), k);
+        const float2 y = add2(make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)),
+                                          __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443))), k);
+        return make_float4(x.x, x.y, y.x, y.y);
     }
 };
 
@@ -128,9 +145,9 @@ __device__ __forceinline__ void encode_groups(const uint4 (&v)[8], int lane, uin
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 p = T::unpack(w[i]);
-            x[2 * i] = __fmul_rn(p.x, f);
-            x[2 * i + 1] = __fmul_rn(p.y, f);
+            const float2 p = mul2(T::unpack(w[i]), make_float2(f, f));
+            x[2 * i] = p.x;
+            x[2 * i + 1] = p.y;
         }
         codes[k] = make_uint2(Code::encode4(x[0], x[1], x[2], x[3]), Code::encode4(x[4], x[5], x[6], x[7]));
         if (f == 0.f) codes[k] = make_uint2(0u, 0u);  // (no product of 0 and inf or NaN, no negative zeros)
@@ -142,10 +159,10 @@ template <typename T, typename Code>
 __device__ __forceinline__ uint4 decode_unit(const uint2 &c, float scale)
 {
     const float4 a = Code::decode4(c.x), b = Code::decode4(c.y);
-    return make_uint4(T::pack(__fmul_rn(a.x, scale), __fmul_rn(a.y, scale)),
-                      T::pack(__fmul_rn(a.z, scale), __fmul_rn(a.w, scale)),
-                      T::pack(__fmul_rn(b.x, scale), __fmul_rn(b.y, scale)),
-                      T::pack(__fmul_rn(b.z, scale), __fmul_rn(b.w, scale)));
+    const float2 f = make_float2(scale, scale);
+    const float2 v[4] = {mul2(make_float2(a.x, a.y), f), mul2(make_float2(a.z, a.w), f), mul2(make_float2(b.x, b.y), f),
+                         mul2(make_float2(b.z, b.w), f)};
+    return make_uint4(T::pack(v[0].x, v[0].y), T::pack(v[1].x, v[1].y), T::pack(v[2].x, v[2].y), T::pack(v[3].x, v[3].y));
 }
 
 }  // namespace kvb
