@@ -7,10 +7,10 @@
 // Writing, a warp takes a tile of positions, one per lane, lists the rows it found in shared memory, and
 // takes them as one flat array of groups of 128 values: 16 units of 16 bytes, one for each lane of a
 // half-warp, which takes eight groups at a time, so that values are read once, from registers to codes.
-// No two warps wait for each other. 8192 rows of 61 layers, 903 MB: 189 us, 4.8 TB/s. The instructions
+// No two warps wait for each other. 8192 rows of 61 layers, 903 MB: 188 us, 4.8 TB/s. The instructions
 // were 63% of the issue slots with an address for each group; hence four groups to an address.
 // Reading, a CTA takes a tile, as rows.cu does, since few positions may be misses, and 16 codes (32
-// bytes) a thread at a time. 262,144 of 524,288 positions, 479 MB: 127 us, 3.8 TB/s; copying as many rows
+// bytes) a thread at a time. 262,144 of 524,288 positions, 479 MB: 123 to 135 us, 3.9 TB/s; copying as many rows
 // of these sizes from and to random places, without any rule or arithmetic, takes 98 us. (A warp a tile:
 // 136 us; the next tile's positions loaded ahead: 136 us; the memory is the limit, not the waits.)
 #include <stdint.h>
