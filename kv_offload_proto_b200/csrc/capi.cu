@@ -306,12 +306,11 @@ int make_codec(uint32_t format, uint32_t dtype, uint32_t quant, uint32_t plain, 
 // The gather of 16-bit hot rows from stored segment rows (or the scatter into them): build_gather
 // with the stored row's size, the hot rows' stride in 16-bit rows, and the codec's alignment.
 int gather_quant_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows, uint32_t plsr,
-                        uint32_t row_format,
-                        uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems, uint64_t topk_indices,
-                        uint64_t req_pool_indices, uint64_t req_host_base, uint64_t topk_device_slots, uint64_t flags,
-                        uint64_t num_real, uint64_t hot_row_base, uint32_t top_k, uint32_t max_num_reqs,
-                        uint32_t stripe_rows, uint64_t status, uint64_t stream, uint32_t block_dim,
-                        const KvopsRowOpts *opts, bool write)
+                        uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
+                        uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
+                        uint64_t topk_device_slots, uint64_t flags, uint64_t num_real, uint64_t hot_row_base,
+                        uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint64_t status, uint64_t stream,
+                        uint32_t block_dim, const KvopsRowOpts *opts, bool write)
 {
     const char *what = write ? "export_quant" : "import_quant";
     KV_REQUIRE_INIT();
@@ -744,6 +743,7 @@ int kvops_export_seg_alllayer(uint64_t channel, uint64_t seg_base, uint32_t per_
 int kvops_quant_row_bytes(uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
                           uint32_t *out_bytes)
 {
+    if (out_bytes == nullptr) return fail(KVOPS_E_INVALID, "quant_row_bytes: out_bytes is NULL");
     kvb::RowCodec c{};
     const int rc = make_codec(row_format, row_dtype, quant_elems, plain_elems, "quant_row_bytes", &c);
     if (rc != KVOPS_OK) return rc;

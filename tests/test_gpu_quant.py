@@ -265,3 +265,108 @@ def test_rows_beyond_four_gigabytes():
     for i in range(2):
         got = hot[at[i] * 1152:(at[i] + 1) * 1152].view(torch.bfloat16).cpu()
         assert torch.equal(got, dec[i])
+
+
+@pytest.mark.parametrize("fmt, dtype, quant, plain", [("e4m3", "fp16", 512, 64), ("int8", "bf16", 384, 8)])
+def test_many_rows_in_tiles_and_rounds(fmt, dtype, quant, plain):
+    """More rows than one round of the launch takes, written whole and by index and read back, over three segments."""
+    mod = kv()
+    layers, cnt, N, S, dbs = 3, 20_001, 3, 7, 1500
+    rows = make_rows(12, (4000, quant + plain), dtype)
+    src = rows.cuda()[torch.arange(layers * cnt, device="cuda") % 4000].view(layers, cnt, -1).contiguous()
+    enc = quant_model.encode(rows, fmt, quant)
+    dec = quant_model.decode(enc, fmt, dtype, quant).cuda()
+    plsr = (cnt + S - 1) // S // N * S + S
+    width = enc.shape[1]
+    segs = [torch.zeros((layers, plsr, width), dtype=torch.uint8, device="cuda") for _ in range(N)]
+    bases = [s.data_ptr() for s in segs]
+    mod.export_quant_alllayer(bases, plsr, fmt, dtype, quant, plain, 0, cnt, layers, src.data_ptr(), src.stride(0) * 2, S, 0,
+                              0, 1, injective=True)
+    at = torch.arange(cnt, device="cuda")
+    g = at // S
+    place_of, seg_of = (g // N) * S + at % S, g % N
+    want = torch.from_numpy(enc).cuda()
+    for layer in range(layers):
+        for n in range(N):
+            mine = at[seg_of == n]
+            assert torch.equal(segs[n][layer, place_of[mine]], want[(layer * cnt + mine) % 4000]), (layer, n)
+    # every row of layer 1 is read back into hot rows of 16 requests, half of them flagged, then written to layer 2
+    R, K = 16, 1250
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    pos = torch.randperm(R * K, generator=gen, device="cuda").view(R, K).to(torch.int32)
+    slots = torch.argsort(torch.rand((R, dbs), generator=gen, device="cuda"), 1)[:, :K].to(torch.int32).contiguous()
+    flags = (torch.rand((R, K), generator=gen, device="cuda") < 0.5).to(torch.int8)
+    idx, zero = torch.arange(R, device="cuda"), torch.zeros(R, dtype=torch.int64, device="cuda")
+    real = torch.tensor([R], dtype=torch.int32, device="cuda")
+    hot = torch.zeros((R, dbs, quant + plain), dtype=src.dtype, device="cuda")
+    ptrs = [x.data_ptr() for x in (pos, idx, zero, slots, flags, real, hot)]
+    mod.import_quant(bases, plsr, plsr, fmt, dtype, quant, plain, *ptrs, K, R, S, 0, 0, 1, hot_req_stride_rows=dbs,
+                     injective=True)
+    expect = torch.zeros_like(hot)
+    r, k = flags.nonzero(as_tuple=True)
+    expect[r, slots[r, k].long()] = dec[(cnt + pos[r, k].long()) % 4000]
+    assert torch.equal(hot.view(torch.int16), expect.view(torch.int16))
+    for s in segs:
+        s[2].zero_()
+    mod.export_quant(bases, 2 * plsr, plsr, fmt, dtype, quant, plain, *ptrs, K, R, S, 0, 0, 1, hot_req_stride_rows=dbs,
+                     injective=True)
+    p = pos[r, k].long()
+    again = torch.from_numpy(quant_model.encode(dec.cpu(), fmt, quant)).cuda()
+    for n in range(N):
+        mine = p[seg_of[p] == n]
+        assert torch.equal(segs[n][2, place_of[mine]], again[(cnt + mine) % 4000])
+        rest = torch.ones(plsr, dtype=torch.bool, device="cuda")
+        rest[place_of[mine]] = False
+        assert (segs[n][2][rest] == 0).all()
+
+
+def test_captured_and_on_two_streams():
+    """The three launches in one graph, replayed with new rows, beside the same on another stream."""
+    mod = kv()
+    cnt, K = 600, 200
+    one = torch.tensor([1], dtype=torch.int32, device="cuda")
+    idx, zero = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+
+    class Set:
+        def __init__(self, seed):
+            self.rows = make_rows(seed, (cnt, 576), "fp16").cuda()
+            self.seg = torch.zeros((cnt, 656), dtype=torch.uint8, device="cuda")
+            self.back = torch.zeros((1, cnt, 656), dtype=torch.uint8, device="cuda")
+            self.hot = torch.zeros((K, 576), dtype=torch.float16, device="cuda")
+            self.pos = torch.randperm(cnt, device="cuda")[:K].to(torch.int32)
+            self.slots = torch.randperm(K, device="cuda").to(torch.int32)
+            self.flags = torch.ones(K, dtype=torch.int8, device="cuda")
+
+        def run(self):
+            s = torch.cuda.current_stream().cuda_stream
+            p = [x.data_ptr() for x in (self.pos, idx, zero, self.slots, self.flags, one, self.hot)]
+            codec = ("e4m3", "fp16", 512, 64)
+            mod.export_quant_alllayer([self.seg.data_ptr()], cnt, *codec, 0, cnt, 1, self.rows.data_ptr(), 0, 1, 0, s)
+            mod.import_quant([self.seg.data_ptr()], 0, cnt, *codec, *p, K, 1, 1, 0, s)
+            mod.export_quant([self.back.data_ptr()], 0, cnt, *codec, *p, K, 1, 1, 0, s)
+
+        def check(self):
+            enc = quant_model.encode(self.rows.cpu(), "e4m3", 512)
+            dec = quant_model.decode(enc, "e4m3", "fp16", 512)
+            pos = self.pos.cpu().long()
+            assert torch.equal(self.seg.cpu(), torch.from_numpy(enc))
+            assert torch.equal(self.hot.cpu()[self.slots.cpu().long()], dec[pos])
+            assert torch.equal(self.back[0].cpu()[pos], torch.from_numpy(quant_model.encode(dec[pos], "e4m3", 512)))
+
+    a, b = Set(21), Set(22)
+    a.run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.run()
+    side = torch.cuda.Stream()
+    for seed in (23, 24):
+        a.rows.copy_(make_rows(seed, (cnt, 576), "fp16"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(5):
+                b.run()
+        for _ in range(5):
+            graph.replay()
+        torch.cuda.synchronize()
+        a.check()
+        b.check()

@@ -149,3 +149,18 @@ def test_attend_needs_a_batch():
         co.attend(Q, HOT, hot_req_stride_rows=16)
     with pytest.raises(RuntimeError, match="kvops not inited"):
         coordinator().attend(Q, HOT, hot_req_stride_rows=16)
+
+
+def test_null_outputs_are_refused_at_the_c_entries():
+    import ctypes
+    import os
+
+    import kv_offload_proto_b200 as kp
+
+    kp.install_kvops_ext()
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(kp.__file__), "libkvops_b200.so"))
+    lib.kvops_last_error.restype = ctypes.c_char_p
+    assert lib.kvops_quant_row_bytes(1, 0, 512, 64, None) != 0
+    assert b"NULL" in lib.kvops_last_error()
+    size = ctypes.c_uint32()
+    assert lib.kvops_quant_row_bytes(1, 0, 512, 64, ctypes.byref(size)) == 0 and size.value == 656
