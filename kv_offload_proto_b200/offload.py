@@ -55,6 +55,18 @@ def tree_masks(parents):
     return masks
 
 
+def _word_address(word, device):
+    """The address of an error word: an int as it is, or an int32 tensor of one element that kernels on `device` can
+    write (there, or in pinned host memory). Only the address is looked at, never the word."""
+    if isinstance(word, int):
+        return word
+    if not isinstance(word, torch.Tensor) or word.dtype != torch.int32 or word.numel() != 1:
+        raise ValueError("err_word must be an address or an int32 tensor of one element")
+    if word.device != device and not (word.device.type == "cpu" and word.is_pinned()):
+        raise ValueError("err_word must be on {} or in pinned host memory".format(device))
+    return word.data_ptr()
+
+
 class XdsOffloadCoordinator:
     """Per-layer SIEVE state and decode-step driver for one device."""
 
@@ -189,9 +201,9 @@ class XdsOffloadCoordinator:
         batch rows below num_real only. A token without any key gets out 0 and lse -inf. out, lse
         and workspace (uint8, at least _kvops.attend_workspace(...) bytes, used by one call at a
         time) may be given; otherwise they are allocated for the call. err_word: address (or int32
-        tensor) of a word that receives errCode 0x103 if a wait inside the kernel gave up, which leaves
-        outputs undefined; by default a word of the coordinator's, whose code the next call raises
-        (and `attend_error()` returns, once the launch has ended)."""
+        tensor of one element, on this device or pinned) of a word that receives errCode 0x103 if a wait
+        inside the kernel gave up, which leaves outputs undefined; by default a word of the coordinator's,
+        whose code the next call raises (and `attend_error()` returns, once the launch has ended)."""
         shape, strides = q.shape, q.stride()
         squeeze = len(shape) == 3
         if len(shape) not in (3, 4) or shape[-1] != KEY_DIM or strides[-1] != 1:
@@ -243,6 +255,7 @@ class XdsOffloadCoordinator:
         for x in (q, slots, draft_rows, tree, out, lse, workspace):
             if x is not None and x.device != dev:
                 raise ValueError("attend: every tensor must be on {}".format(dev))
+        err_word = _word_address(err_word, dev)
         if err_word == 0 and dev.type == "cuda":
             if self._attend_err[0] != 0:
                 raise RuntimeError("attend: a wait inside an earlier call gave up (errCode 0x{:x})".format(self.attend_error()))
@@ -281,6 +294,5 @@ class XdsOffloadCoordinator:
             self.num_real.data_ptr(), draft_at, draft_strides[0], draft_strides[1],
             tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
             workspace.data_ptr() if room else 0, room, B, T, H, K, D, row_format, dtype,
-            KEY_DIM ** -0.5 if scale is None else scale, stream,
-            err_word=err_word if isinstance(err_word, int) else err_word.data_ptr())
+            KEY_DIM ** -0.5 if scale is None else scale, stream, err_word=err_word)
         return out, lse

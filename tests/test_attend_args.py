@@ -1,0 +1,56 @@
+"""Arguments of XdsOffloadCoordinator.attend without a GPU: what reaches the launch, and what is refused."""
+import pytest
+import torch
+
+from kv_offload_proto_b200.offload import XdsOffloadCoordinator
+
+REQS, HEADS, ROWS = 2, 4, 16
+
+
+class Launches:
+    """In the place of the launch module: keeps what a call of attend passes on."""
+
+    def __init__(self):
+        self.calls = []
+
+    def attend_workspace(self, *args):
+        return 0
+
+    def attend_hot(self, *args, **named):
+        self.calls.append((args, named))
+
+
+class HostCoordinator(XdsOffloadCoordinator):
+    _require_cuda = False
+
+
+def coordinator(k=8):
+    co = HostCoordinator("cpu", 1, REQS, ROWS, k, REQS, 64)
+    co._req_pool_indices = torch.arange(REQS)
+    co._k = Launches()
+    return co
+
+
+def attend(co, **change):
+    args = dict(q=torch.zeros((REQS, HEADS, 576), dtype=torch.float16),
+                hot_row_base=torch.zeros((REQS * ROWS, 576), dtype=torch.float16), hot_req_stride_rows=ROWS, scale=0.07)
+    args.update(change)
+    return co.attend(args.pop("q"), args.pop("hot_row_base"), **args)
+
+
+@pytest.mark.parametrize("value", [0, 0x103])
+def test_an_error_word_is_passed_on_by_its_address(value):
+    co, word = coordinator(), torch.full((1,), value, dtype=torch.int32)
+    attend(co, err_word=word.data_ptr())
+    assert co._k.calls[-1][1]["err_word"] == word.data_ptr()
+    attend(co, err_word=word)
+    assert [c[1]["err_word"] for c in co._k.calls] == [word.data_ptr()] * 2 and word.item() == value
+
+
+@pytest.mark.parametrize("word", [torch.zeros(1, dtype=torch.int64), torch.zeros(2, dtype=torch.int32),
+                                  torch.zeros(0, dtype=torch.int32), torch.zeros(1), None, "0"])
+def test_error_words_of_other_kinds_are_refused(word):
+    co = coordinator()
+    with pytest.raises(ValueError, match="err_word"):
+        attend(co, err_word=word)
+    assert not co._k.calls
