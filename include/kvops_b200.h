@@ -55,6 +55,7 @@ extern "C" {
 #define KVOPS_ERR_ROW_BASE 0x200u  /* 0x200 + (index & 0xFF) + (1 << 16): row out of the segment */
 #define KVOPS_ERR_COPY_TIMEOUT 0x102u  /* kvops_sieve_import: a copy CTA stopped waiting for a walk list */
 #define KVOPS_ERR_ATTEND_TIMEOUT 0x103u  /* kvops_attend_hot: a wait inside the kernel gave up; outputs are not valid */
+#define KVOPS_ERR_ATTEND_SLOT 0x104u  /* kvops_attend_hot: a slot from hot_rows on, where report_slots asks for it */
 
 /* Largest node count of one layout (common/kv_layout.h:45, KvLayoutValidate). */
 #define KVOPS_MAX_NODES 64
@@ -348,13 +349,15 @@ typedef struct KvopsAttend {
     uint64_t lse;                  /* fp32 [max_num_reqs, tokens, heads], 0: not wanted */
     uint64_t workspace;            /* kvops_attend_workspace bytes, 16-byte aligned; one launch at a time */
     uint64_t workspace_bytes;
-    uint64_t err_word;             /* as KvopsRowOpts.err_word: KVOPS_ERR_ATTEND_TIMEOUT; 0: none */
+    uint64_t err_word;             /* as KvopsRowOpts.err_word: KVOPS_ERR_ATTEND_*; 0: none */
     uint32_t max_num_reqs, tokens, heads, top_k, drafts; /* tokens and drafts <= 64, heads <= 128 */
-    uint32_t hot_rows;             /* rows per request that a slot may name */
+    uint32_t hot_rows;             /* rows per request that a slot may name (kvops_sieve_update gives a position
+                                      behind the prefill the slot padded_buffer_size + position - prefill) */
     uint32_t pool_size;
     uint32_t row_format;           /* KVOPS_ROW_RAW, or how the hot rows are stored */
     uint32_t row_dtype;            /* of q, the 16-bit rows and out */
     float scale;
+    uint32_t report_slots;         /* 1: a slot from hot_rows on, still no key, sets KVOPS_ERR_ATTEND_SLOT */
 } KvopsAttend;
 
 /* Bytes of workspace that kvops_attend_hot needs for this shape on the current device. */

@@ -347,6 +347,7 @@ __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan
     Fetched next[2];  // two tiles on their way
     if (begin < end) next[0] = fetch();
     if (begin + 1 < end) next[1] = fetch();
+    bool behind = false;  // whether a slot named a row behind the request's last
     for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
         const Fetched f = next[0];
         next[0] = next[1];
@@ -358,12 +359,13 @@ __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const uint32_t k = f.tile * kTile + lane + 32 * j;
-            const bool listed = in_pool && f.slot[j] >= 0 && static_cast<uint32_t>(f.slot[j]) < a.hot_rows;
+            const bool named = in_pool && f.slot[j] >= 0, listed = named && static_cast<uint32_t>(f.slot[j]) < a.hot_rows;
             const bool drafted = k >= plan.list_end && k - plan.list_end < a.drafts;
             sh.row[buf][lane + 32 * j] =
                 listed ? a.hot_row_base + (f.pool * a.hot_req_stride_rows + f.slot[j]) * kRowBytes : 0;
             sh.kind[buf][lane + 32 * j] = listed ? kList : drafted ? kDraft : kNone;
             mine |= listed || drafted;
+            behind |= named && !listed;
         }
         const bool any = __any_sync(0xFFFFFFFFu, mine);
         if (lane == 0) {
@@ -376,6 +378,8 @@ __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&sh.meta_full[buf]));
     }
+    if (a.report_slots != 0 && __any_sync(0xFFFFFFFFu, behind) && lane == 0 && a.err_word != 0)
+        atomicCAS_system(reinterpret_cast<uint32_t *>(a.err_word), 0u, KVOPS_ERR_ATTEND_SLOT);
 }
 
 // The word of the n-th tile of the run, once it is known, the same in every lane; and the end of its use.
@@ -1138,6 +1142,7 @@ int check_shape(const KvopsAttend *a)
         return invalid("attend_hot: top_k / max_num_reqs out of range");
     if (a->row_format > KVOPS_ROW_INT8) return invalid("attend_hot: row_format must be 0, 1 or 2");
     if (a->row_dtype > KVOPS_DTYPE_BF16) return invalid("attend_hot: row_dtype must be 0 or 1");
+    if (a->report_slots > 1) return invalid("attend_hot: report_slots must be 0 or 1");
     return KVOPS_OK;
 }
 

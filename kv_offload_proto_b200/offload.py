@@ -18,6 +18,9 @@ __all__ = ["XdsOffloadCoordinator", "align", "compute_ht_size", "tree_masks"]
 
 KEY_DIM, VALUE_DIM = 576, 512  # values of a row that attention scores use, and that it sums
 ROW_BYTES = {"raw": 1152, "e4m3": 656, "int8": 656}
+ATTEND_ERRORS = {0x103: "a wait inside an earlier call gave up",
+                 0x104: "an earlier call's slots named rows that its hot rows have no place for (tokens generated since "
+                        "the prompt have the slots from padded_buffer_size on; hot_rows given leaves them out)"}
 
 
 def align(v, a):
@@ -195,15 +198,20 @@ class XdsOffloadCoordinator:
         first 512 values are its value. hot_row_base: the layer's hot rows (a tensor, or an
         address), hot_req_stride_rows from one pool row to the next (0: shared), of row_format
         "raw" (the type of q) or stored in 8 bits. hot_rows: rows a slot may name (default: the
-        stride, or device_buffer_size for shared rows). scale: of the scores, default 576 ** -0.5.
+        stride; for shared rows those that the tensor holds, or device_buffer_size where an address is
+        given). sieve_update gives a token generated since the prompt, position t >= prefill_len, the
+        slot padded_buffer_size + t - prefill_len; its row belongs there, so the stride (or the shared
+        rows) must reach that far. Where sieve_update's own slots do not fit the default, errCode 0x104
+        says so; with hot_rows given they are left out. scale: of the scores, default 576 ** -0.5.
 
         Returns (out, lse): [.., heads, 512] in q's type and fp32 [.., heads], written for the
         batch rows below num_real only. A token without any key gets out 0 and lse -inf. out, lse
         and workspace (uint8, at least _kvops.attend_workspace(...) bytes, used by one call at a
         time) may be given; otherwise they are allocated for the call. err_word: address (or int32
         tensor of one element, on this device or pinned) of a word that receives errCode 0x103 if a wait
-        inside the kernel gave up, which leaves outputs undefined; by default a word of the coordinator's,
-        whose code the next call raises (and `attend_error()` returns, once the launch has ended)."""
+        inside the kernel gave up, which leaves outputs undefined, or 0x104 (above); by default a word of
+        the coordinator's, whose code the next call raises (and `attend_error()` returns, once the launch
+        has ended)."""
         shape, strides = q.shape, q.stride()
         squeeze = len(shape) == 3
         if len(shape) not in (3, 4) or shape[-1] != KEY_DIM or strides[-1] != 1:
@@ -225,8 +233,11 @@ class XdsOffloadCoordinator:
         K = s_shape[-1]
         if row_format not in ROW_BYTES:
             raise ValueError("attend: row_format must be 'raw', 'e4m3' or 'int8', got {!r}".format(row_format))
+        report_slots = hot_rows is None and slots is self.top_k_device_slots
         if hot_rows is None:
             hot_rows = hot_req_stride_rows or self.device_buffer_size
+            if hot_req_stride_rows == 0 and isinstance(hot_row_base, torch.Tensor):
+                hot_rows = max(hot_rows, hot_row_base.numel() * hot_row_base.element_size() // ROW_BYTES[row_format])
         D, draft_at, draft_strides = 0, 0, (0, 0)
         if draft_rows is not None:
             if draft_rows.dim() != 3 or draft_rows.shape[0] < B or draft_rows.shape[2] != KEY_DIM or \
@@ -258,10 +269,11 @@ class XdsOffloadCoordinator:
         err_word = _word_address(err_word, dev)
         if err_word == 0 and dev.type == "cuda":
             if self._attend_err[0] != 0:
-                raise RuntimeError("attend: a wait inside an earlier call gave up (errCode 0x{:x})".format(self.attend_error()))
+                code = self.attend_error()
+                raise RuntimeError("attend: {} (errCode 0x{:x})".format(ATTEND_ERRORS.get(code, "an earlier call failed"), code))
             err_word = self._attend_err_at
         args = (q, B, T, H, K, D, squeeze, strides, slots, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale,
-                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word)
+                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word, report_slots)
         if dev.type == "cuda" and (stream is not None or torch.cuda.current_device() != dev.index):
             with torch.cuda.device(dev):
                 if stream is None or (out is not None and lse is not None and workspace is not None):
@@ -272,7 +284,7 @@ class XdsOffloadCoordinator:
         return self._attend(*args)
 
     def _attend(self, q, B, T, H, K, D, squeeze, strides, slots, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale,
-                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word):
+                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word, report_slots):
         """attend() on checked arguments and the current device."""
         if stream is None:  # (no Stream object: 4 us of a 20 us call)
             stream = torch._C._cuda_getCurrentRawStream(q.device.index) if q.is_cuda else 0
@@ -294,5 +306,5 @@ class XdsOffloadCoordinator:
             self.num_real.data_ptr(), draft_at, draft_strides[0], draft_strides[1],
             tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
             workspace.data_ptr() if room else 0, room, B, T, H, K, D, row_format, dtype,
-            KEY_DIM ** -0.5 if scale is None else scale, stream, err_word=err_word)
+            KEY_DIM ** -0.5 if scale is None else scale, stream, err_word=err_word, report_slots=report_slots)
         return out, lse

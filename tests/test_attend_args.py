@@ -54,3 +54,29 @@ def test_error_words_of_other_kinds_are_refused(word):
     with pytest.raises(ValueError, match="err_word"):
         attend(co, err_word=word)
     assert not co._k.calls
+
+
+def shape_of(call):
+    """(hot_req_stride_rows, hot_rows, report_slots) of a launch."""
+    args, named = call
+    return args[5], args[6], named["report_slots"]
+
+
+@pytest.mark.parametrize("change, want", [
+    (dict(), (ROWS, ROWS, True)),
+    (dict(hot_rows=12), (ROWS, 12, False)),
+    (dict(topk_device_slots=torch.zeros((REQS, 5), dtype=torch.int32)), (ROWS, ROWS, False)),
+    (dict(hot_req_stride_rows=0), (0, REQS * ROWS, True)),         # shared: all that the tensor holds
+    (dict(hot_req_stride_rows=0, hot_rows=20), (0, 20, False)),
+    (dict(hot_req_stride_rows=0, hot_row_base=1 << 20), (0, ROWS, True)),  # an address tells no size
+    (dict(hot_req_stride_rows=0, row_format="int8", hot_row_base=torch.zeros((30, 656), dtype=torch.uint8)), (0, 30, True)),
+])
+def test_which_rows_a_slot_may_name(change, want):
+    co = coordinator()
+    attend(co, **change)
+    assert shape_of(co._k.calls[-1]) == want
+
+
+def test_shared_rows_hold_the_buffer():
+    with pytest.raises(ValueError, match="hot rows must"):
+        attend(coordinator(), hot_req_stride_rows=0, hot_row_base=torch.zeros((ROWS - 1, 576), dtype=torch.float16))

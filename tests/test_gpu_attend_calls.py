@@ -3,6 +3,8 @@ which rows a slot may name, types, workspaces, and launches that give up."""
 import pytest
 import torch
 
+from gpu_util import kv
+from kv_offload_proto_b200.offload import XdsOffloadCoordinator
 from test_gpu_attend import Case
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +48,66 @@ def test_a_tensor_as_error_word_in_a_captured_call():
     torch.cuda.synchronize()
     c.check(*out)
     assert word.item() == 0
+
+
+def with_generated_tokens(rows, shared):
+    """A step in which SIEVE names tokens behind the prompt: a buffer of 20 slots (32 padded), a prompt of 40, three more."""
+    kv()
+    dbs, prefill, new, K, R, H = 20, 40, 3, 12, 2, 5
+    co = XdsOffloadCoordinator("cuda", 1, R, dbs, K, R, 64)
+    co.admit_all([prefill] * R, [0] * R)
+    co.set_batch(torch.arange(R, device="cuda"), torch.full((R,), prefill + new, dtype=torch.int32, device="cuda"))
+    co.sieve_update(0, torch.tensor([[0, 1, 2, 40, 41, 42, 3, 4, 5, 6, -1, 7], [40, 0, 9, 8, 7, 6, 5, 4, 3, 2, 1, 42]],
+                                    dtype=torch.int32, device="cuda"))
+    assert co.padded_buffer_size == 32 and int((co.top_k_device_slots >= 32).sum()) == 5
+    c = Case.__new__(Case)
+    c.B, c.T, c.H, c.K, c.D, c.rows, c.scale, c.co = R, 1, H, K, 0, rows, 0.07, co
+    g = torch.Generator(device="cuda").manual_seed(1)
+    c.q = torch.randn((R, 1, H, 576), generator=g, device="cuda").half()
+    c.read = torch.randn((rows if shared else R * rows, 576), generator=g, device="cuda").half()
+    c.draft = c.tree = None
+    c.idx, c.stride, c.slots = co._req_pool_indices, 0 if shared else rows, co.top_k_device_slots
+    return c
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_tokens_generated_since_the_prompt_are_keys(shared):
+    c = with_generated_tokens(35, shared)
+    c.check(*c.co.attend(c.q, c.read, hot_req_stride_rows=c.stride, scale=c.scale))
+    torch.cuda.synchronize()
+    assert c.co.attend_error() == 0
+
+
+@pytest.mark.parametrize("rows", [20, 34])
+@pytest.mark.parametrize("shared", [False, True])
+def test_generated_tokens_without_a_row_are_reported(shared, rows):
+    """The last (or every) generated token has no row: the outputs are without it, and the next call raises."""
+    c = with_generated_tokens(rows, shared)
+    out = c.co.attend(c.q, c.read, hot_req_stride_rows=c.stride, scale=c.scale)
+    torch.cuda.synchronize()
+    c.check(*out)
+    with pytest.raises(RuntimeError, match="padded_buffer_size.*0x104"):
+        c.co.attend(c.q, c.read, hot_req_stride_rows=c.stride, scale=c.scale)
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    c.co.attend(c.q, c.read, hot_req_stride_rows=c.stride, scale=c.scale, err_word=word)
+    assert word.item() == 0x104 and c.co.attend_error() == 0
+
+
+@pytest.mark.parametrize("change", [dict(hot_rows=20), dict(topk_device_slots="copy"), dict(num_real=0), dict(idx=7)])
+def test_slots_left_out_on_purpose_are_not_reported(change):
+    """hot_rows given, a list that is not SIEVE's own, batch rows behind num_real, and requests without hot rows."""
+    c = with_generated_tokens(20, False)
+    args = dict(hot_req_stride_rows=20, scale=c.scale)
+    if "hot_rows" in change:
+        args.update(change)
+    if "topk_device_slots" in change:
+        args["topk_device_slots"] = c.slots.clone()
+    if "num_real" in change:
+        c.co.num_real.fill_(0)
+    if "idx" in change:
+        c.idx.fill_(7)  # no such pool row
+    out = c.co.attend(c.q, c.read, **args)
+    torch.cuda.synchronize()
+    assert c.co.attend_error() == 0
+    if "num_real" not in change:
+        c.check(*out)
