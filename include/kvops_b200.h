@@ -358,6 +358,8 @@ typedef struct KvopsAttend {
     uint32_t row_dtype;            /* of q, the 16-bit rows and out */
     float scale;
     uint32_t report_slots;         /* 1: a slot from hot_rows on, still no key, sets KVOPS_ERR_ATTEND_SLOT */
+    uint32_t wait_clocks;          /* SM clocks that a tile of 64 keys may keep the next ones waiting before the
+                                      launch gives up; 0, and for every other wait inside the kernel: 2^30 */
 } KvopsAttend;
 
 /* Bytes of workspace that kvops_attend_hot needs for this shape on the current device. */

@@ -161,9 +161,10 @@ struct Shared {
         meta_full[kAhead], meta_empty[kAhead];
     uint64_t row[kAhead][kTile];  // where the tile's hot rows start, 0: no hot row
     uint8_t kind[kAhead][kTile];  // of the tile's keys: kNone, kList, kDraft or kBadDraft
-    // 0 for a tile without any key, else 1 | lo << 8 | hi << 16: rows 4 lo .. 4 hi - 1 are drafted ones
+    // 0 for a tile without any key, else kKeys | lo << 8 | hi << 16: rows 4 lo .. 4 hi - 1 are drafted ones
     uint32_t tile[kAhead];
-    uint32_t tmem, stop;
+    uint64_t drained[2];  // the products of the score and the weigh warp
+    uint32_t tmem, stop;  // stop: a wait has given up
 };
 enum : uint8_t { kNone = 0, kList = 1, kDraft = 2, kBadDraft = 3 };
 
@@ -303,6 +304,13 @@ __device__ __forceinline__ uint4 draft_unit(const uint8_t *from, uint8_t *kind)
     return v;
 }
 
+constexpr uint32_t kKeys = 1, kOver = 2;  // of a tile's word: it has a key; no tile, a wait has given up
+// Whether a wait of the CTA has given up (the lanes may see it at different times).
+__device__ __forceinline__ bool given_up(const Shared &sh)
+{
+    return *const_cast<const volatile uint32_t *>(&sh.stop) != 0;
+}
+
 // The rows of each tile, for the other warps: lane l looks at keys l and l + 32.
 template <int NQ, bool kStored>
 __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan, Shared &sh, uint32_t begin, uint32_t end)
@@ -347,13 +355,23 @@ __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan
     Fetched next[2];  // two tiles on their way
     if (begin < end) next[0] = fetch();
     if (begin + 1 < end) next[1] = fetch();
+    const long long limit = a.wait_clocks != 0 ? a.wait_clocks : kWaitClocks;
     bool behind = false;  // whether a slot named a row behind the request's last
     for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
         const Fetched f = next[0];
         next[0] = next[1];
         if (at + 2 < end) next[1] = fetch();
         const uint32_t buf = n % kAhead;
-        if (n >= kAhead) mbar_wait(smem_addr(&sh.meta_empty[buf]), (n / kAhead - 1) & 1, &sh.stop);
+        if (n >= kAhead) {
+            // The caller's limit is looked at here, where a wait lasts as long as the slowest warp's tile, and after
+            // the wait, since the barrier instruction itself may take longer than a short limit. (The other
+            // waits have a constant one: read from shared memory it cost 4%.)
+            const long long start = clock64();
+            mbar_wait(smem_addr(&sh.meta_empty[buf]), (n / kAhead - 1) & 1, &sh.stop);
+            if (clock64() - start > limit) *const_cast<volatile uint32_t *>(&sh.stop) = 1u;
+            __syncwarp();
+        }
+        if (__any_sync(0xFFFFFFFFu, given_up(sh))) break;
         const bool in_pool = f.pool >= 0 && f.pool < static_cast<int64_t>(a.pool_size);
         bool mine = false;
 #pragma unroll
@@ -373,7 +391,7 @@ __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan
             const uint32_t lo = plan.list_end <= t0 ? 0 : min(plan.list_end - t0, static_cast<uint32_t>(kTile));
             const uint32_t till = plan.list_end + ((a.drafts + 3) & ~3u);
             const uint32_t hi = a.drafts == 0 || till <= t0 ? lo : max(lo, min(till - t0, static_cast<uint32_t>(kTile)));
-            sh.tile[buf] = any ? 1u | (lo / 4) << 8 | (hi / 4) << 16 : 0u;
+            sh.tile[buf] = any ? kKeys | (lo / 4) << 8 | (hi / 4) << 16 : 0u;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&sh.meta_full[buf]));
@@ -383,12 +401,13 @@ __device__ __forceinline__ void find_warp(const KvopsAttend &a, const Plan &plan
 }
 
 // The word of the n-th tile of the run, once it is known, the same in every lane; and the end of its use.
-// After a wait has given up no tile has a key: its rows' addresses may never have been written.
+// After a wait has given up it is kOver, which has no key: rows' addresses may never have been written. A warp that
+// got it asks for no further tile, for which each time it would wait as long as the barrier instruction does.
 __device__ __forceinline__ uint32_t tile_word(Shared &sh, uint32_t n)
 {
     tc::mbar_wait(tc::smem_addr(&sh.meta_full[n % kAhead]), (n / kAhead) & 1, &sh.stop);
     const uint32_t word = *const_cast<volatile uint32_t *>(&sh.tile[n % kAhead]);
-    return __shfl_sync(0xFFFFFFFFu, *const_cast<volatile uint32_t *>(&sh.stop) != 0 ? 0u : word, 0);
+    return __shfl_sync(0xFFFFFFFFu, given_up(sh) ? kOver : word, 0);
 }
 __device__ __forceinline__ void tile_done(Shared &sh, uint32_t n, int lane)
 {
@@ -485,7 +504,7 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
     }
     for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
         const uint32_t word = tile_word(sh, n);
-        if (word != 0) {
+        if ((word & kKeys) != 0) {
             const int lo = word >> 8 & 0xFF, hi = word >> 16;
             const bool first = !q_loaded;
             q_loaded = true;
@@ -523,7 +542,7 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
                 sent = false;
                 if (at + 1 < end) {  // the next tile's, into the place that was just read
                     const uint32_t w = tile_word(sh, n + 1);
-                    sent = w != 0;
+                    sent = (w & kKeys) != 0;
                     if (sent) send(n + 1, w >> 8 & 0xFF, w >> 16);
                 }
                 if (turn > 0) mbar_wait(smem_addr(&sh.empty[place]), (turn - 1) & 1, &sh.stop);
@@ -561,6 +580,8 @@ __device__ __forceinline__ void load_warps(const KvopsAttend &a, const Plan &pla
 #pragma unroll
             for (int i = 0; i < 4; ++i) ring.next();
             ++done;
+        } else if (word == kOver) {
+            break;
         }
         tile_done(sh, n, lane);
         if (++tile == plan.tiles) {
@@ -585,9 +606,11 @@ __device__ __forceinline__ void each_tile(const Plan &plan, Shared &sh, uint32_t
     bool starts = true;
     const int lane = threadIdx.x & 31;
     for (uint32_t at = begin, n = 0; at < end; ++at, ++n) {
-        const bool any = tile_word(sh, n) != 0;
+        const uint32_t word = tile_word(sh, n);
+        const bool any = (word & kKeys) != 0;
         tile_done(sh, n, lane);
         if (any) body(starts, at);
+        else if (word == kOver) break;
         starts = !any && starts;
         if (++tile == plan.tiles) {
             tile = 0;
@@ -644,6 +667,7 @@ __device__ __forceinline__ void score_warp(const Plan &plan, Shared &sh, uint32_
         commit(elected, smem_addr(&sh.s_full[buf]));
         ++n;
     });
+    if (n > 0) drain(elected, smem_addr(&sh.drained[0]));
 }
 
 // The second product of each tile, as soon as its probabilities are there.
@@ -676,6 +700,7 @@ __device__ __forceinline__ void weigh_warp(const Plan &plan, Shared &sh, uint32_
         commit(elected, smem_addr(&sh.done[buf]));
         ++n;
     });
+    if (n > 0) drain(elected, smem_addr(&sh.drained[1]));
 }
 
 // ---- the softmax and the outputs ---------------------------------------------------------------
@@ -719,6 +744,7 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
     };
     uint32_t done = 0, unit = begin / plan.tiles, tile = begin - unit * plan.tiles, start_tile = tile;
     bool fresh = true, started = false, open = false;
+    uint32_t word = 0;
     Unit u{};
     float ref = -INFINITY;   // of `column`
     float sum[2 * kBlocks];  // of this thread's keys, by its columns
@@ -740,9 +766,9 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 group_barrier(3, kSoftmaxWarps * 32);
             }
         }
-        const uint32_t word = tile_word(sh, meta);
-        // (through a barrier: after a wait has given up, too, the warps of a half must agree)
-        const bool any = group_any(1 + half, 128, word != 0);
+        // (to its end also after a wait has given up, since the warps meet at barriers; the warps of a half must agree)
+        if (word != kOver) word = tile_word(sh, meta);
+        const bool any = group_any(1 + half, 128, (word & kKeys) != 0);
         if (any) {
             mbar_wait(smem_addr(&sh.s_full[done & 1]), (done >> 1) & 1, &sh.stop);
             fence_after_sync();
@@ -967,6 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_addr(&sh.s_full[b]), 1);
             mbar_init(smem_addr(&sh.done[b]), 1);
             mbar_init(smem_addr(&sh.p_full[b]), kSoftmaxWarps);
+            mbar_init(smem_addr(&sh.drained[b]), 1);
         }
         for (uint32_t b = 0; b < kAhead; ++b) {
             mbar_init(smem_addr(&sh.meta_full[b]), 1);
@@ -983,8 +1010,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t units = real_units(a, plan);
     const uint32_t run = run_length(plan, units), pairs = units * plan.tiles;
     const uint32_t begin = min(blockIdx.x * run, pairs), end = min(begin + run, pairs);
-    // A wait that gives up sets sh.stop and every role goes on to its end without waiting again, so
-    // that no thread is left at a barrier.
+    // A wait that gives up sets sh.stop and every role goes on to its end without waiting for a tile
+    // again, so that no thread is left at a barrier. What is under way by then still ends before the memory
+    // that it uses is given back: the load warps wait for their copies, the product warps for their products.
     if (warp < kSoftmaxWarps) {
         softmax_warps<T, kStored, NQ>(a, plan, sh, smem, begin, end);
     } else if (warp < kSoftmaxWarps + kLoadWarps) {

@@ -224,7 +224,7 @@ void attend_hot(uint64_t q, uint64_t q_stride_req, uint64_t q_stride_token, uint
                 uint64_t draft_stride_row, uint64_t tree, uint64_t out, uint64_t lse, uint64_t workspace,
                 uint64_t workspace_bytes, uint32_t max_num_reqs, uint32_t tokens, uint32_t heads, uint32_t top_k,
                 uint32_t drafts, const std::string &row_format, const std::string &row_dtype, float scale,
-                uint64_t stream, uint64_t err_word, bool report_slots)
+                uint64_t stream, uint64_t err_word, bool report_slots, uint32_t wait_clocks)
 {
     KvopsAttend a = attend_shape(max_num_reqs, tokens, heads, top_k, drafts, row_format, row_dtype);
     a.q = q;
@@ -251,6 +251,7 @@ void attend_hot(uint64_t q, uint64_t q_stride_req, uint64_t q_stride_token, uint
     a.scale = scale;
     a.err_word = err_word;
     a.report_slots = report_slots ? 1u : 0u;
+    a.wait_clocks = wait_clocks;
     check(kvops_attend_hot(&a, stream));
 }
 
@@ -363,7 +364,8 @@ PYBIND11_MODULE(_kvops, m)
           py::arg("draft_stride_row"), py::arg("tree"), py::arg("out"), py::arg("lse"), py::arg("workspace"),
           py::arg("workspace_bytes"), py::arg("max_num_reqs"), py::arg("tokens"), py::arg("heads"), py::arg("top_k"),
           py::arg("drafts"), py::arg("row_format"), py::arg("row_dtype"), py::arg("scale"), py::arg("stream") = 0,
-          py::kw_only(), py::arg("err_word") = 0, py::arg("report_slots") = false);
+          py::kw_only(), py::arg("err_word") = 0, py::arg("report_slots") = false,
+          py::arg("wait_clocks") = 0);
     m.def("sieve_update", &sieve_update, py::arg("topk_indices"), py::arg("req_pool_indices"), py::arg("seq_lens"),
           py::arg("prefill_lens"), py::arg("device_buffer_tokens"), py::arg("device_buffer_visited"),
           py::arg("device_buffer_ht"), py::arg("sieve_hand"), py::arg("topk_device_slots"), py::arg("is_miss"),

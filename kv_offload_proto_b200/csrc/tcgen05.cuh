@@ -95,6 +95,17 @@ __device__ __forceinline__ void commit(uint32_t elected, uint32_t bar)
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar), "r"(elected)
         : "memory");
 }
+// Waits until every matrix instruction that the elected lane issued has ended, and every arrival that it
+// committed has been made, whether or not another wait has given up: `bar` is a barrier of one arrival that nothing
+// else uses. Issued instructions always end; the limit only keeps the wait bounded.
+__device__ __forceinline__ void drain(uint32_t elected, uint32_t bar)
+{
+    commit(elected, bar);
+    const long long start = clock64();
+    while (!mbar_try(bar, 0))
+        if (clock64() - start > kWaitClocks) break;
+    __syncwarp();
+}
 // 1 in one lane of the converged warp.
 __device__ __forceinline__ uint32_t elect()
 {

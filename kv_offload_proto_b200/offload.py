@@ -186,7 +186,7 @@ class XdsOffloadCoordinator:
 
     def attend(self, q, hot_row_base, *, hot_req_stride_rows=0, hot_rows=None, row_format="raw", scale=None,
                topk_device_slots=None, draft_rows=None, tree=None, out=None, lse=None, workspace=None, stream=None,
-               err_word=0):
+               err_word=0, wait_clocks=0):
         """Attention of this step's tokens over one layer's hot rows (kvops_attend_hot).
 
         q: float16 or bfloat16 [B, heads, 576] (one token a request) or [B, tokens, heads, 576],
@@ -211,7 +211,8 @@ class XdsOffloadCoordinator:
         tensor of one element, on this device or pinned) of a word that receives errCode 0x103 if a wait
         inside the kernel gave up, which leaves outputs undefined, or 0x104 (above); by default a word of
         the coordinator's, whose code the next call raises (and `attend_error()` returns, once the launch
-        has ended)."""
+        has ended). wait_clocks: SM clocks that a tile of 64 keys may keep the next ones
+        waiting (0: 2^30, half a second, as for every other wait inside the kernel)."""
         shape, strides = q.shape, q.stride()
         squeeze = len(shape) == 3
         if len(shape) not in (3, 4) or shape[-1] != KEY_DIM or strides[-1] != 1:
@@ -273,7 +274,7 @@ class XdsOffloadCoordinator:
                 raise RuntimeError("attend: {} (errCode 0x{:x})".format(ATTEND_ERRORS.get(code, "an earlier call failed"), code))
             err_word = self._attend_err_at
         args = (q, B, T, H, K, D, squeeze, strides, slots, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale,
-                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word, report_slots)
+                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word, report_slots, wait_clocks)
         if dev.type == "cuda" and (stream is not None or torch.cuda.current_device() != dev.index):
             with torch.cuda.device(dev):
                 if stream is None or (out is not None and lse is not None and workspace is not None):
@@ -284,7 +285,8 @@ class XdsOffloadCoordinator:
         return self._attend(*args)
 
     def _attend(self, q, B, T, H, K, D, squeeze, strides, slots, hot, hot_req_stride_rows, hot_rows, row_format, dtype, scale,
-                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word, report_slots):
+                draft_at, draft_strides, tree, out, lse, workspace, stream, err_word, report_slots,
+                wait_clocks):
         """attend() on checked arguments and the current device."""
         if stream is None:  # (no Stream object: 4 us of a 20 us call)
             stream = torch._C._cuda_getCurrentRawStream(q.device.index) if q.is_cuda else 0
@@ -306,5 +308,6 @@ class XdsOffloadCoordinator:
             self.num_real.data_ptr(), draft_at, draft_strides[0], draft_strides[1],
             tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
             workspace.data_ptr() if room else 0, room, B, T, H, K, D, row_format, dtype,
-            KEY_DIM ** -0.5 if scale is None else scale, stream, err_word=err_word, report_slots=report_slots)
+            KEY_DIM ** -0.5 if scale is None else scale, stream, err_word=err_word, report_slots=report_slots,
+            wait_clocks=wait_clocks)
         return out, lse

@@ -111,3 +111,32 @@ def test_slots_left_out_on_purpose_are_not_reported(change):
     assert c.co.attend_error() == 0
     if "num_real" not in change:
         c.check(*out)
+
+
+@pytest.mark.parametrize("shape", [
+    dict(B=64, T=1, H=128, K=2048, rows=2048, fmt="raw"),
+    dict(B=40, T=1, H=128, K=2048, rows=2048, fmt="e4m3"),         # lists that are cut and joined
+    dict(B=20, T=12, H=16, K=2048, rows=2048, D=12, fmt="int8", dtype="bf16"),
+    dict(B=300, T=1, H=16, K=500, rows=512, fmt="raw", holes=0.3),  # several requests a run
+], ids=lambda s: "-".join(map(str, s.values())))
+def test_a_launch_whose_waits_run_out_says_so_and_leaves_nothing_behind(shape):
+    """A limit shorter than a tile takes: the launch ends with errCode 0x103, and the launch behind it, which starts as it
+    ends, is right. Limits near a tile's time give up in the middle of the work, or not at all."""
+    c = Case(42, **shape)
+    want = c.call()
+    c.check(*want)
+    for clocks in (1, 1, 200, 800, 1500, 2500, 3500, 5000, 8000, 20000):
+        word = torch.zeros(1, dtype=torch.int32, device="cuda")
+        cut = c.call(err_word=word, wait_clocks=clocks)
+        behind = c.call()
+        code = word.item()
+        assert code == 0x103 if clocks == 1 else code in (0, 0x103)
+        if code == 0:
+            assert torch.equal(cut[0], want[0]) and torch.equal(cut[1], want[1])
+        assert torch.equal(behind[0], want[0]) and torch.equal(behind[1], want[1])
+    assert c.co.attend_error() == 0
+    c.call(wait_clocks=1)  # by default the next call raises it
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="0x103"):
+        c.call()
+    c.check(*c.call())
