@@ -241,7 +241,7 @@ int kvops_sieve_import(uint64_t topk_indices, uint64_t req_pool_indices, uint64_
                        uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts);
 
 /* KVOPS_STEP_COOP, _FUSED or _SPLIT: the path the calling thread's last successful
- * kvops_sieve_import ran (KVOPS_STEP_AUTO before any). No counterpart in the reference. */
+ * kvops_sieve_import or kvops_sieve_import_quant ran (KVOPS_STEP_AUTO before any). No counterpart in the reference. */
 uint32_t kvops_last_step_path(void);
 
 /* Does, without launching, the one-time setup the first kvops_sieve_import of this shape on
@@ -317,6 +317,19 @@ int kvops_import_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t la
                        uint64_t req_host_base, uint64_t topk_device_slots, uint64_t is_miss, uint64_t num_real,
                        uint64_t hot_row_base, uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows,
                        uint64_t status, uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts);
+
+/* kvops_sieve_import over stored rows: kvops_sieve_update, then kvops_import_quant as its programmatic dependent
+ * (KVOPS_STEP_SPLIT, the only path besides AUTO: the one-kernel paths move rows unchanged, and
+ * opts->copy_wait_polls is theirs). A call with a bad argument launches neither. */
+int kvops_sieve_import_quant(uint64_t topk_indices, uint64_t req_pool_indices, uint64_t seq_lens, uint64_t prefill_lens,
+                             uint64_t device_buffer_tokens, uint64_t device_buffer_visited, uint64_t device_buffer_ht,
+                             uint64_t sieve_hand, uint64_t topk_device_slots, uint64_t is_miss, uint64_t num_real,
+                             uint32_t top_k, uint32_t device_buffer_size, uint32_t padded_buffer_size,
+                             uint32_t visited_stride_b, uint32_t max_num_reqs, uint32_t pool_size, uint32_t node_num,
+                             const uint64_t *seg_bases, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
+                             uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
+                             uint64_t req_host_base, uint64_t hot_row_base, uint32_t stripe_rows, uint64_t status,
+                             uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts);
 
 /* ---- attention over the hot rows (no counterpart in the reference) --------------------------
  *

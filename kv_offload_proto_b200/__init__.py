@@ -24,7 +24,7 @@ C_ABI_SYMBOLS = (
     "kvops_ipc_close_handle", "kvops_import_multi_noalloc", "kvops_sieve_import",
     "kvops_last_step_path", "kvops_step_prepare", "kvops_export_seg", "kvops_set_sieve_tier",
     "kvops_last_sieve_tier", "kvops_quant_row_bytes", "kvops_export_quant_alllayer", "kvops_export_quant",
-    "kvops_import_quant", "kvops_attend_workspace", "kvops_attend_hot",
+    "kvops_import_quant", "kvops_sieve_import_quant", "kvops_attend_workspace", "kvops_attend_hot",
 )
 
 _lib = None

@@ -305,6 +305,33 @@ int make_codec(uint32_t format, uint32_t dtype, uint32_t quant, uint32_t plain, 
 
 // The gather of 16-bit hot rows from stored segment rows (or the scatter into them): build_gather
 // with the stored row's size, the hot rows' stride in 16-bit rows, and the codec's alignment.
+int build_gather_quant(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows, uint32_t plsr,
+                       uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
+                       uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
+                       uint64_t topk_device_slots, uint64_t flags, uint64_t num_real, uint64_t hot_row_base,
+                       uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint64_t status, uint64_t stream,
+                       uint32_t block_dim, const KvopsRowOpts *opts, const char *what, kvb::RowCodec *c,
+                       kvb::GatherParams *p, DeviceState **ds)
+{
+    KV_REQUIRE_INIT();
+    if (node_num == 0 || node_num > KVOPS_MAX_NODES)
+        return fail(KVOPS_E_INVALID, std::string(what) + " node_num must be in [1, 64]");
+    if (seg_bases == nullptr) return fail(KVOPS_E_INVALID, std::string(what) + ": seg_bases is NULL");
+    int rc = make_codec(row_format, row_dtype, quant_elems, plain_elems, what, c);
+    if (rc != KVOPS_OK) return rc;
+    uint64_t bases = hot_row_base;
+    for (uint32_t n = 0; n < node_num; ++n) bases |= seg_bases[n];
+    if (bases % 16 != 0)
+        return fail(KVOPS_E_INVALID, std::string(what) + ": hot rows and segments must be 16-byte aligned");
+    rc = build_gather(node_num, seg_bases, 0, node_num, kvb::kAllNodes, layer_offset_rows, plsr,
+                      kvb::codec_stored_bytes(*c), topk_indices, req_pool_indices, req_host_base, topk_device_slots,
+                      flags, num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream, block_dim, opts,
+                      p, ds, what);
+    if (rc != KVOPS_OK) return rc;
+    p->hot_req_stride_bytes = (opts ? opts->hot_req_stride_rows : 0) * kvb::codec_row_bytes(*c);
+    return KVOPS_OK;
+}
+
 int gather_quant_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t layer_offset_rows, uint32_t plsr,
                         uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
                         uint64_t topk_indices, uint64_t req_pool_indices, uint64_t req_host_base,
@@ -312,26 +339,14 @@ int gather_quant_common(uint32_t node_num, const uint64_t *seg_bases, uint32_t l
                         uint32_t top_k, uint32_t max_num_reqs, uint32_t stripe_rows, uint64_t status, uint64_t stream,
                         uint32_t block_dim, const KvopsRowOpts *opts, bool write)
 {
-    const char *what = write ? "export_quant" : "import_quant";
-    KV_REQUIRE_INIT();
-    if (node_num == 0 || node_num > KVOPS_MAX_NODES)
-        return fail(KVOPS_E_INVALID, std::string(what) + " node_num must be in [1, 64]");
-    if (seg_bases == nullptr) return fail(KVOPS_E_INVALID, std::string(what) + ": seg_bases is NULL");
     kvb::RowCodec c{};
-    int rc = make_codec(row_format, row_dtype, quant_elems, plain_elems, what, &c);
-    if (rc != KVOPS_OK) return rc;
-    uint64_t bases = hot_row_base;
-    for (uint32_t n = 0; n < node_num; ++n) bases |= seg_bases[n];
-    if (bases % 16 != 0)
-        return fail(KVOPS_E_INVALID, std::string(what) + ": hot rows and segments must be 16-byte aligned");
     kvb::GatherParams p{};
     DeviceState *ds = nullptr;
-    rc = build_gather(node_num, seg_bases, 0, node_num, kvb::kAllNodes, layer_offset_rows, plsr,
-                      kvb::codec_stored_bytes(c), topk_indices, req_pool_indices, req_host_base, topk_device_slots,
-                      flags, num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream, block_dim, opts,
-                      &p, &ds, what);
+    const int rc = build_gather_quant(node_num, seg_bases, layer_offset_rows, plsr, row_format, row_dtype, quant_elems,
+                                      plain_elems, topk_indices, req_pool_indices, req_host_base, topk_device_slots,
+                                      flags, num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream,
+                                      block_dim, opts, write ? "export_quant" : "import_quant", &c, &p, &ds);
     if (rc != KVOPS_OK) return rc;
-    p.hot_req_stride_bytes = (opts ? opts->hot_req_stride_rows : 0) * kvb::codec_row_bytes(c);
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const cudaError_t e = write ? kvb::launch_scatter_quant(p, c, s, ds->sm_count)
                                 : kvb::launch_gather_quant(p, c, s, ds->sm_count);
@@ -912,6 +927,46 @@ int kvops_sieve_import(uint64_t topk_indices, uint64_t req_pool_indices, uint64_
     }
     cudaError_t e = kvb::launch_gather(gp, st, ds->sm_count);
     if (e != cudaSuccess) return cuda_fail(e, "launch kvc_gather_rows");
+    return KVOPS_OK;
+}
+
+int kvops_sieve_import_quant(uint64_t topk_indices, uint64_t req_pool_indices, uint64_t seq_lens, uint64_t prefill_lens,
+                             uint64_t device_buffer_tokens, uint64_t device_buffer_visited, uint64_t device_buffer_ht,
+                             uint64_t sieve_hand, uint64_t topk_device_slots, uint64_t is_miss, uint64_t num_real,
+                             uint32_t top_k, uint32_t device_buffer_size, uint32_t padded_buffer_size,
+                             uint32_t visited_stride_b, uint32_t max_num_reqs, uint32_t pool_size, uint32_t node_num,
+                             const uint64_t *seg_bases, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
+                             uint32_t row_format, uint32_t row_dtype, uint32_t quant_elems, uint32_t plain_elems,
+                             uint64_t req_host_base, uint64_t hot_row_base, uint32_t stripe_rows, uint64_t status,
+                             uint64_t stream, uint32_t block_dim, const KvopsRowOpts *opts)
+{
+    KV_REQUIRE_INIT();
+    const uint32_t path = opts ? opts->step_path : KVOPS_STEP_AUTO;
+    if (path != KVOPS_STEP_AUTO && path != KVOPS_STEP_SPLIT)
+        return fail(KVOPS_E_INVALID, "sieve_import_quant: step_path must be KVOPS_STEP_AUTO or KVOPS_STEP_SPLIT");
+    kvb::SieveParams sp{};
+    DeviceState *sds = nullptr;  // null: the SIEVE step has nothing to do
+    int rc = build_sieve(topk_indices, req_pool_indices, seq_lens, prefill_lens, device_buffer_tokens,
+                         device_buffer_visited, device_buffer_ht, sieve_hand, topk_device_slots, is_miss, num_real,
+                         top_k, device_buffer_size, padded_buffer_size, visited_stride_b, max_num_reqs, pool_size,
+                         stream, 1u, &sp, &sds);
+    if (rc != KVOPS_OK) return rc;
+    kvb::RowCodec c{};
+    kvb::GatherParams gp{};
+    DeviceState *ds = nullptr;
+    rc = build_gather_quant(node_num, seg_bases, layer_offset_rows, per_layer_seg_rows, row_format, row_dtype,
+                            quant_elems, plain_elems, topk_indices, req_pool_indices, req_host_base, topk_device_slots,
+                            is_miss, num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream, block_dim,
+                            opts, "sieve_import_quant", &c, &gp, &ds);
+    if (rc != KVOPS_OK) return rc;
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (sds != nullptr) {
+        const cudaError_t e = kvb::launch_sieve_update(sp, st, sds->sm_count);
+        if (e != cudaSuccess) return cuda_fail(e, "launch hisp_sieve_update");
+    }
+    t_last_step_path = KVOPS_STEP_SPLIT;
+    const cudaError_t e = kvb::launch_gather_quant(gp, c, st, ds->sm_count);
+    if (e != cudaSuccess) return cuda_fail(e, "launch sieve_import_quant");
     return KVOPS_OK;
 }
 

@@ -194,6 +194,27 @@ void import_quant(const std::vector<uint64_t> &seg_bases, uint32_t layer_offset_
                              num_real, hot_row_base, top_k, max_num_reqs, stripe_rows, status, stream, block_dim, &o));
 }
 
+void sieve_import_quant(uint64_t topk_indices, uint64_t req_pool_indices, uint64_t seq_lens, uint64_t prefill_lens,
+                        uint64_t device_buffer_tokens, uint64_t device_buffer_visited, uint64_t device_buffer_ht,
+                        uint64_t sieve_hand, uint64_t topk_device_slots, uint64_t is_miss, uint64_t num_real,
+                        uint32_t top_k, uint32_t device_buffer_size, uint32_t padded_buffer_size,
+                        uint32_t visited_stride_b, uint32_t max_num_reqs, uint32_t pool_size,
+                        const std::vector<uint64_t> &seg_bases, uint32_t layer_offset_rows, uint32_t per_layer_seg_rows,
+                        const std::string &row_format, const std::string &row_dtype, uint32_t quant_elems,
+                        uint32_t plain_elems, uint64_t req_host_base, uint64_t hot_row_base, uint32_t stripe_rows,
+                        uint64_t status, uint64_t stream, uint32_t block_dim, uint64_t hot_req_stride_rows,
+                        bool injective, uint64_t err_word)
+{
+    const KvopsRowOpts o = row_opts(hot_req_stride_rows, injective, err_word);
+    check(kvops_sieve_import_quant(topk_indices, req_pool_indices, seq_lens, prefill_lens, device_buffer_tokens,
+                                   device_buffer_visited, device_buffer_ht, sieve_hand, topk_device_slots, is_miss,
+                                   num_real, top_k, device_buffer_size, padded_buffer_size, visited_stride_b,
+                                   max_num_reqs, pool_size, static_cast<uint32_t>(seg_bases.size()), seg_bases.data(),
+                                   layer_offset_rows, per_layer_seg_rows, row_format_of(row_format),
+                                   row_dtype_of(row_dtype), quant_elems, plain_elems, req_host_base, hot_row_base,
+                                   stripe_rows, status, stream, block_dim, &o));
+}
+
 KvopsAttend attend_shape(uint32_t max_num_reqs, uint32_t tokens, uint32_t heads, uint32_t top_k, uint32_t drafts,
                          const std::string &row_format, const std::string &row_dtype)
 {
@@ -355,6 +376,16 @@ PYBIND11_MODULE(_kvops, m)
           py::arg("top_k"), py::arg("max_num_reqs"), py::arg("stripe_rows"), py::arg("status"), py::arg("stream") = 0,
           py::arg("block_dim") = 1, py::kw_only(), py::arg("hot_req_stride_rows") = 0, py::arg("injective") = false,
           py::arg("err_word") = 0);
+    m.def("sieve_import_quant", &sieve_import_quant, py::arg("topk_indices"), py::arg("req_pool_indices"),
+          py::arg("seq_lens"), py::arg("prefill_lens"), py::arg("device_buffer_tokens"),
+          py::arg("device_buffer_visited"), py::arg("device_buffer_ht"), py::arg("sieve_hand"),
+          py::arg("topk_device_slots"), py::arg("is_miss"), py::arg("num_real"), py::arg("top_k"),
+          py::arg("device_buffer_size"), py::arg("padded_buffer_size"), py::arg("visited_stride_b"),
+          py::arg("max_num_reqs"), py::arg("pool_size"), py::arg("seg_bases"), py::arg("layer_offset_rows"),
+          py::arg("per_layer_seg_rows"), py::arg("row_format"), py::arg("row_dtype"), py::arg("quant_elems"),
+          py::arg("plain_elems"), py::arg("req_host_base"), py::arg("hot_row_base"), py::arg("stripe_rows"),
+          py::arg("status"), py::arg("stream") = 0, py::arg("block_dim") = 1, py::kw_only(),
+          py::arg("hot_req_stride_rows") = 0, py::arg("injective") = false, py::arg("err_word") = 0);
     m.def("attend_workspace", &attend_workspace, py::arg("max_num_reqs"), py::arg("tokens"), py::arg("heads"),
           py::arg("top_k"), py::arg("drafts"), py::arg("row_format") = "raw", py::arg("row_dtype") = "fp16");
     m.def("attend_hot", &attend_hot, py::arg("q"), py::arg("q_stride_req"), py::arg("q_stride_token"),

@@ -300,18 +300,21 @@ class DevicePool:
 
     def _sieve_and_read_quant(self, coord, layer_id, topk_indices, hot_row_base, stream, block_dim,
                               hot_req_stride_rows, path, publish, err_word):
-        """The layer-step when the read converts rows: the SIEVE kernel, then the read launched as
-        its programmatic dependent (the one-kernel paths move rows unchanged)."""
+        """The layer-step when the read converts rows: the SIEVE kernel, then the read launched as its programmatic
+        dependent (the one-kernel paths, whose copy_wait_polls is, move rows unchanged); neither is launched if
+        an argument of the other is refused."""
         if path not in ("auto", "split"):
             raise ValueError("sieve_and_read: rows stored in 8 bits run path 'auto' or 'split', got {!r}".format(path))
         status = self.next_status() if publish else 0
-        coord.sieve_update(layer_id, topk_indices, stream=stream)
-        self._k.import_quant(self.seg_bases, layer_id * self.per_layer_seg_rows, self.per_layer_seg_rows,
-                             *self._hot_codec, _ptr(topk_indices), _ptr(coord._req_pool_indices),
-                             _ptr(coord.req_host_base), _ptr(coord.top_k_device_slots), _ptr(coord.is_miss),
-                             _ptr(coord.num_real), _ptr(hot_row_base), coord.top_k, coord.max_num_reqs,
-                             self.stripe_rows, status, stream, block_dim, hot_req_stride_rows=hot_req_stride_rows,
-                             injective=self.injective, err_word=_ptr(err_word))
+        self._k.sieve_import_quant(
+            _ptr(topk_indices), _ptr(coord._req_pool_indices), _ptr(coord._seq_lens), _ptr(coord.prefill_lens),
+            _ptr(coord.device_buffer_tokens[layer_id]), _ptr(coord.device_buffer_visited[layer_id]),
+            _ptr(coord.device_buffer_ht[layer_id]), _ptr(coord.sieve_hand[layer_id]), _ptr(coord.top_k_device_slots),
+            _ptr(coord.is_miss), _ptr(coord.num_real), coord.top_k, coord.device_buffer_size,
+            coord.padded_buffer_size, coord.visited_stride_b, coord.max_num_reqs, coord.pool_size, self.seg_bases,
+            layer_id * self.per_layer_seg_rows, self.per_layer_seg_rows, *self._hot_codec, _ptr(coord.req_host_base),
+            _ptr(hot_row_base), self.stripe_rows, status, stream, block_dim, hot_req_stride_rows=hot_req_stride_rows,
+            injective=self.injective, err_word=_ptr(err_word))
         return status
 
     def batch_write(self, layer_id, topk_indices, req_pool_indices, req_host_base, topk_device_slots, export_flags,
