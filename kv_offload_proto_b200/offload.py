@@ -197,7 +197,8 @@ class XdsOffloadCoordinator:
         [B, tokens], see tree_masks; None: a chain, token t seeing drafted rows 0..t). A row's
         first 512 values are its value. hot_row_base: the layer's hot rows (a tensor, or an
         address), hot_req_stride_rows from one pool row to the next (0: shared), of row_format
-        "raw" (the type of q) or stored in 8 bits. hot_rows: rows a slot may name (default: the
+        "raw" (the type of q; a floating-point tensor of another type is refused, one of integers taken as it
+        is) or stored in 8 bits. hot_rows: rows a slot may name (default: the
         stride; for shared rows those that the tensor holds, or device_buffer_size where an address is
         given). sieve_update gives a token generated since the prompt, position t >= prefill_len, the
         slot padded_buffer_size + t - prefill_len; its row belongs there, so the stride (or the shared
@@ -255,6 +256,10 @@ class XdsOffloadCoordinator:
             need = ((self.pool_size - 1) * hot_req_stride_rows + hot_rows) * ROW_BYTES[row_format]
             if hot_row_base.numel() * hot_row_base.element_size() < need or not hot_row_base.is_contiguous():
                 raise ValueError("attend: hot rows must be contiguous and hold {} bytes".format(need))
+            if hot_row_base.is_floating_point() and (hot_row_base.dtype != q.dtype if row_format == "raw" else
+                                                     hot_row_base.element_size() > 1):
+                raise ValueError("attend: hot rows of row_format {!r} must be {}, got {}".format(
+                    row_format, q.dtype if row_format == "raw" else "bytes", hot_row_base.dtype))
             if hot_row_base.device != self.top_k_device_slots.device:
                 raise ValueError("attend: hot rows must be on {}".format(self.top_k_device_slots.device))
             hot = hot_row_base.data_ptr()

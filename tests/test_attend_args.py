@@ -80,3 +80,37 @@ def test_which_rows_a_slot_may_name(change, want):
 def test_shared_rows_hold_the_buffer():
     with pytest.raises(ValueError, match="hot rows must"):
         attend(coordinator(), hot_req_stride_rows=0, hot_row_base=torch.zeros((ROWS - 1, 576), dtype=torch.float16))
+
+
+RAW, STORED = (REQS * ROWS, 576), (REQS * ROWS, 656)
+
+
+@pytest.mark.parametrize("hot, row_format", [
+    (torch.zeros(RAW, dtype=torch.bfloat16), "raw"), (torch.zeros(RAW), "raw"), (torch.zeros(RAW, dtype=torch.float64), "raw"),
+    (torch.zeros(RAW, dtype=torch.float16), "e4m3"), (torch.zeros(STORED), "int8"),
+])
+def test_hot_rows_of_another_type_are_refused(hot, row_format):
+    co = coordinator()
+    with pytest.raises(ValueError, match="hot rows of row_format"):
+        attend(co, hot_row_base=hot, row_format=row_format)
+    assert not co._k.calls
+
+
+@pytest.mark.parametrize("hot, row_format", [
+    (torch.zeros(RAW, dtype=torch.float16), "raw"), (torch.zeros(RAW, dtype=torch.int16), "raw"),
+    (torch.zeros((REQS * ROWS, 1152), dtype=torch.uint8), "raw"), (torch.zeros((REQS * ROWS, 288), dtype=torch.int32), "raw"),
+    (torch.zeros(STORED, dtype=torch.uint8), "int8"), (torch.zeros(STORED, dtype=torch.int8), "e4m3"),
+    (torch.zeros((REQS * ROWS, 164), dtype=torch.int32), "e4m3"),
+])
+def test_hot_rows_as_bytes_and_integers(hot, row_format):
+    co = coordinator()
+    attend(co, hot_row_base=hot, row_format=row_format)
+    assert co._k.calls[-1][0][4] == hot.data_ptr()
+
+
+def test_bf16_rows_with_a_bf16_q():
+    co = coordinator()
+    attend(co, q=torch.zeros((REQS, HEADS, 576), dtype=torch.bfloat16), hot_row_base=torch.zeros(RAW, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="hot rows of row_format"):
+        attend(co, q=torch.zeros((REQS, HEADS, 576), dtype=torch.bfloat16))
+    assert len(co._k.calls) == 1
