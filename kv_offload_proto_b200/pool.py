@@ -165,7 +165,8 @@ class DevicePool:
     batch_read and sieve_and_read read the miss rows back into 16-bit hot rows. With
     hot_quantized=True the hot rows are stored rows too (seg_row_bytes each): batch_read,
     sieve_and_read and batch_write move them unchanged, `XdsOffloadCoordinator.attend` reads them
-    as they are, and only batch_write_alllayers quantises.
+    as they are, and only batch_write_alllayers quantises. Rows given as a floating-point tensor of
+    another type are refused; bytes, integers and addresses are taken as they are.
     """
 
     def __init__(self, device_id: int, layer_num: int, layer_rows: int, row_bytes: int, stripe_rows: int = 1,
@@ -226,6 +227,16 @@ class DevicePool:
         self._status_base = self._k.alloc_status(self._status_count)
         self._status_cursor = 0
 
+    def _check_type(self, rows, stored):
+        """Refuses a floating-point tensor that cannot hold what this pool takes it for: 16-bit rows of its row_dtype, or
+        (stored) bytes. A pool that stores rows as they are takes any."""
+        if self._codec is None or not hasattr(rows, "is_floating_point") or not rows.is_floating_point():
+            return
+        want = "torch.float16" if self._codec[1] == "fp16" else "torch.bfloat16"
+        if rows.element_size() > 1 if stored else str(rows.dtype) != want:
+            raise ValueError("this pool's {} rows are {}, got {}".format(
+                "stored" if stored else "16-bit", "bytes" if stored else want, rows.dtype))
+
     def next_status(self) -> int:
         """Round-robin 64-byte status slot (xds_ems_pool.py:182-185)."""
         addr = self._status_base + self._status_cursor * 64
@@ -248,6 +259,7 @@ class DevicePool:
         fused=True issues one launch over all segments (import_multi); fused=False issues the
         reference's one import_seg launch per segment. Both publish the same status pages. Rows
         stored in 8 bits are read back by one launch over all segments either way."""
+        self._check_type(hot_row_base, self.hot_quantized)
         status = self.next_status()
         off = layer_id * self.per_layer_seg_rows
         a = [_ptr(topk_indices), _ptr(req_pool_indices), _ptr(req_host_base), _ptr(topk_device_slots),
@@ -283,6 +295,7 @@ class DevicePool:
         import torch
         if topk_indices.dtype != torch.int32:
             raise ValueError("topk_indices must be int32")
+        self._check_type(hot_row_base, self.hot_quantized)
         if self._hot_codec is not None:
             return self._sieve_and_read_quant(coord, layer_id, topk_indices, hot_row_base, stream, block_dim,
                                               hot_req_stride_rows, path, publish, err_word)
@@ -323,6 +336,7 @@ class DevicePool:
         decode-increment export of doc/kv_offload_design.md:394-396): batch_read's arguments and
         rules in the opposite direction, one launch per segment (one for all, where rows are
         quantised on the way). Returns the status address."""
+        self._check_type(hot_row_base, self.hot_quantized)
         status = self.next_status()
         off = layer_id * self.per_layer_seg_rows
         a = [_ptr(topk_indices), _ptr(req_pool_indices), _ptr(req_host_base), _ptr(topk_device_slots),
@@ -342,6 +356,7 @@ class DevicePool:
         """Export rows [row_lo, row_lo+row_cnt) of every layer to their segments
         (xds_ems_pool.py:220-230): one launch per segment, as in the reference (one for all segments
         where rows are stored in 8 bits)."""
+        self._check_type(src_layer0_base, False)
         status = self.next_status()
         if self._codec is not None:
             self._k.export_quant_alllayer(self.seg_bases, self.per_layer_seg_rows, *self._codec, row_lo, row_cnt,
