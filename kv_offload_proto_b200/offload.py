@@ -203,7 +203,8 @@ class XdsOffloadCoordinator:
         given). sieve_update gives a token generated since the prompt, position t >= prefill_len, the
         slot padded_buffer_size + t - prefill_len; its row belongs there, so the stride (or the shared
         rows) must reach that far. Where sieve_update's own slots do not fit the default, errCode 0x104
-        says so; with hot_rows given they are left out. scale: of the scores, default 576 ** -0.5.
+        says so; with hot_rows given they are left out. scale: of the scores. It has to be given: it is the
+        model's, mostly the inverse square root of its heads' own width, which a row of 576 does not tell.
 
         Returns (out, lse): [.., heads, 512] in q's type and fp32 [.., heads], written for the
         batch rows below num_real only. A token without any key gets out 0 and lse -inf. out, lse
@@ -305,6 +306,8 @@ class XdsOffloadCoordinator:
             room = self._k.attend_workspace(B, T, H, K, D, row_format, dtype)
             if room:
                 workspace = q.new_empty(room, dtype=torch.uint8)
+        if scale is None:
+            raise ValueError("attend: scale must be given (mostly the inverse square root of the heads' own width)")
         # (the stride of a dimension of one entry is never used)
         self._k.attend_hot(
             q.data_ptr(), strides[0] if B > 1 else 0, strides[1] if T > 1 else 0, strides[2] if H > 1 else 0, hot,
@@ -313,6 +316,6 @@ class XdsOffloadCoordinator:
             self.num_real.data_ptr(), draft_at, draft_strides[0], draft_strides[1],
             tree.data_ptr() if tree is not None else 0, out.data_ptr(), lse.data_ptr(),
             workspace.data_ptr() if room else 0, room, B, T, H, K, D, row_format, dtype,
-            KEY_DIM ** -0.5 if scale is None else scale, stream, err_word=err_word, report_slots=report_slots,
+            scale, stream, err_word=err_word, report_slots=report_slots,
             wait_clocks=wait_clocks)
         return out, lse

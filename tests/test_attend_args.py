@@ -114,3 +114,12 @@ def test_bf16_rows_with_a_bf16_q():
     with pytest.raises(ValueError, match="hot rows of row_format"):
         attend(co, q=torch.zeros((REQS, HEADS, 576), dtype=torch.bfloat16))
     assert len(co._k.calls) == 1
+
+
+def test_the_scale_has_no_default():
+    co = coordinator()
+    with pytest.raises(ValueError, match="scale must be given"):
+        attend(co, scale=None)
+    assert not co._k.calls
+    attend(co, scale=192 ** -0.5)
+    assert co._k.calls[-1][0][28] == 192 ** -0.5
