@@ -60,17 +60,22 @@ constexpr int kScoreWarp = kSoftmaxWarps + kLoadWarps, kWeighWarp = kScoreWarp +
 constexpr int kThreads = (kFindWarp + 1) * 32;  // five warps to a scheduler leave a thread 96 registers, six 80
 constexpr uint32_t kAhead = 4;  // tiles whose rows are known at a time
 
-// A column's running reference: probabilities are 2^(score - reference), and it is set kLift (in powers of
-// two) below the largest score so far when a score passes it by kLift + kSlack. They stay below
-// 2^15, which is an fp16 number; moving the reference means scaling the outputs in tensor memory, so it should
-// be rare: kSlack is what a later score may exceed the first tile's largest by. (Normal scores of variance
-// 3, as of unit-variance queries and rows: with a slack of 4, 106 us for 64 requests x 128 heads, with
-// 11, 81.) fp16's smallest step is 2^-24, that is 2^-28 of the largest probability at the least: with 2^16 keys
-// all rounded by half of it the same way, 2^-13 of the output, below its own rounding. bf16 has no such limit.
-template <typename T>
-constexpr float kLift = std::is_same<T, Bf16>::value ? -5.f : 4.f;
-template <typename T>
-constexpr float kSlack = 15.f - kLift<T>;
+// A column's running reference: probabilities are 2^(score - reference), and it is set Plan::lift (in powers of
+// two) below the largest score so far when a score passes it by kMost. They stay below 2^kMost, which is an
+// fp16 number; moving the reference means scaling the outputs in tensor memory, so it should be rare: what a
+// later score may exceed the first tile's largest by is kMost less the lift. (Normal scores of variance 3,
+// as of unit-variance queries and rows, 64 requests x 128 heads: 4 of it 106 us, 11 of it 81.)
+// fp16's smallest step is 2^-24: each probability that the second product takes is off by 2^-25 at the most
+// besides its relative rounding (those below become 0), while the sum, which has them in fp32, is 2^lift or
+// more. n keys all rounded the same way are off by n 2^-(25 + lift) of the largest value: with a lift of 4, 2^-13 for
+// 2^16 keys, below the output's own rounding. n counts the keys of one CTA's part, each of which has its own
+// references; where that can be more, the lift is 14, which leaves 2^-15 for 2^24 keys. (It costs less the longer
+// a part is: in us with 4 and 14, 64 requests x 128 heads, 32 tiles a part, 65 and 94; 8 requests x 16 heads x 2^17 keys,
+// 111 tiles, 197 and 203; 148 requests x 16 heads x 2^17, 2048 tiles, 2906 and 2913.)
+// bf16 has no such limit.
+constexpr float kMost = 15.f;
+constexpr float kLiftFp16 = 4.f, kLiftFp16Long = 14.f, kLiftBf16 = -5.f;
+constexpr uint32_t kLongPart = 1u << 16;
 
 // How the (query tile, key tile) pairs are dealt out. Units are query tiles: group (a request, or a
 // request's token where every token has its own list) by group.
@@ -82,6 +87,7 @@ struct Plan {
     uint32_t tiles;       // key tiles per unit
     uint32_t ctas;
     uint32_t run_at_most; // pairs of a run, with every request real
+    float lift;           // see kMost
     uint32_t whole;       // > 0: every CTA takes this many whole units; 0: runs of pairs of one length
     float2 *part_ml;      // [2 * ctas][NQ] reference and sum of a unit's part
     float *part_o;        // [2 * ctas][NQ * 512] its weighted sums, in part_at's order
@@ -818,12 +824,11 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
             scores();
             bool move_all = !started;
             if (started) {
-                // The references only have to move when a score passes one by kLift + kSlack, which each
-                // thread's largest excess tells. The probabilities are worked out as if none had, so that
+                // The references only have to move when a score passes one by kMost, which each thread's largest excess tells. The probabilities are worked out as if none had, so that
                 // the warps need not wait for one another before, and again in the rare tile where one has.
                 const float excess = lower();
                 write();
-                move_all = group_any(1 + half, 128, excess > kLift<T> + kSlack<T> || (open && excess > -INFINITY));
+                move_all = group_any(1 + half, 128, excess > kMost || (open && excess > -INFINITY));
                 if (move_all) scores();
             }
             if (move_all) {
@@ -836,9 +841,9 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 // the same decision in the four warps of this half
                 top = fmaxf(fmaxf(sh.top[half][0][column], sh.top[half][1][column]),
                             fmaxf(sh.top[half][2][column], sh.top[half][3][column]));
-                const bool move = top > ref + (kLift<T> + kSlack<T>) || (ref == -INFINITY && top > -INFINITY);
+                const bool move = top > ref + kMost || (ref == -INFINITY && top > -INFINITY);
                 const float was = ref;
-                if (move) ref = top - kLift<T>;
+                if (move) ref = top - plan.lift;
                 if (started && __any_sync(0xFFFFFFFFu, move)) {
                     spread(move ? exp2_fast(was - ref) : 1.f);
                     ended(done - 1);
@@ -1227,6 +1232,8 @@ Plan make_plan(const KvopsAttend &a, uint32_t lists, uint32_t nq, int sms)
     } else {
         p.ctas = static_cast<uint32_t>(pairs < static_cast<uint64_t>(sms) ? pairs : sms);
     }
+    const uint64_t part = p.whole > 0 || run > p.tiles ? p.tiles : run;  // tiles of a list that one CTA takes at the most
+    p.lift = a.row_dtype == KVOPS_DTYPE_BF16 ? kLiftBf16 : part * kTile <= kLongPart ? kLiftFp16 : kLiftFp16Long;
     return p;
 }
 

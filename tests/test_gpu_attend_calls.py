@@ -1,5 +1,7 @@
 """Calls of the attention over the hot rows as its documentation allows them, around the launch itself: where errCodes go,
 which rows a slot may name, types, workspaces, and launches that give up."""
+import math
+
 import pytest
 import torch
 
@@ -140,3 +142,44 @@ def test_a_launch_whose_waits_run_out_says_so_and_leaves_nothing_behind(shape):
     with pytest.raises(RuntimeError, match="0x103"):
         c.call()
     c.check(*c.call())
+
+
+@pytest.mark.parametrize("K", [2 ** 16 + 1, 100_000])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("first", [True, False])
+def test_the_tail_of_a_long_list_counts(first, dtype, K):
+    """One key whose value is 0 takes nearly all, and n = K - 1 keys of value 1 are e^-20.25 (2^-29.2) of it each: out is
+    t = n e^-20.25 / (1 + n e^-20.25) in every dimension. Probabilities are rounded (u, and in fp16 by 2^-39 of the
+    largest each: all the same way, n 2^-39), the output is (u t, and half an fp16 step below the normal numbers), the
+    fp32 sums over K keys are off by K 2^-23 of t, and the exponent of 2 (29.2, an fp32 number) by 2^-20 of t at the most."""
+    c = Case(43, B=148, H=4, K=K, rows=4, holes=0, dtype=dtype)  # a whole list to an SM
+    c.q.zero_()
+    c.q[..., 575] = 1
+    c.hot.zero_()
+    c.hot.view(148, 4, 576)[:, 0, :512] = 1
+    c.hot.view(148, 4, 576)[:, 1, 575] = 20.25
+    c.slots.zero_()
+    c.slots[:, 0 if first else K - 1] = 1
+    out, lse = c.call(scale=1.0)
+    n = K - 1
+    t = n * math.exp(-20.25) / (1 + n * math.exp(-20.25))
+    u = torch.finfo(c.q.dtype).eps / 2
+    tol = 2 * u * t + n * 2.0 ** -39 + K * 2.0 ** -23 * t + 2.0 ** -20 * t + (2.0 ** -25 if dtype == "fp16" else 0)
+    assert (out.double() - t).abs().max() <= tol
+    assert (lse.double() - (20.25 + math.log1p(n * math.exp(-20.25)))).abs().max() <= 2.0 ** -17
+
+
+def test_probabilities_of_a_list_of_two_to_the_sixteen():
+    """The longest list of the small lift: every tail key is off by 2^-29 of the largest at the most, 2^-13 in all."""
+    K = 2 ** 16
+    c = Case(44, B=148, H=2, K=K, rows=4, holes=0)
+    c.q.zero_()
+    c.q[..., 575] = 1
+    c.hot.zero_()
+    c.hot.view(148, 4, 576)[:, 0, :512] = 1
+    c.hot.view(148, 4, 576)[:, 1, 575] = 20.25
+    c.slots.zero_()
+    c.slots[:, 0] = 1
+    out, _ = c.call(scale=1.0)
+    t = (K - 1) * math.exp(-20.25) / (1 + (K - 1) * math.exp(-20.25))
+    assert (out.double() - t).abs().max() <= 2.0 ** -13 + 2.0 ** -10 * t
