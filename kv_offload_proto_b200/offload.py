@@ -270,6 +270,8 @@ class XdsOffloadCoordinator:
             if x is not None and (x.dtype != want or not x.is_contiguous() or x.numel() != B * T * H * each):
                 raise ValueError("attend: {} must be a contiguous {} of {} elements".format(name, want, B * T * H * each))
         dev = self.top_k_device_slots.device
+        if workspace is not None and not workspace.is_contiguous():
+            raise ValueError("attend: workspace must be contiguous")
         for x in (q, slots, draft_rows, tree, out, lse, workspace):
             if x is not None and x.device != dev:
                 raise ValueError("attend: every tensor must be on {}".format(dev))
@@ -301,7 +303,7 @@ class XdsOffloadCoordinator:
             out = q.new_empty((B, H, VALUE_DIM) if squeeze else (B, T, H, VALUE_DIM))
         if lse is None:
             lse = q.new_empty((B, H) if squeeze else (B, T, H), dtype=torch.float32)
-        room = workspace.numel() if workspace is not None else 0
+        room = workspace.numel() * workspace.element_size() if workspace is not None else 0
         if workspace is None:
             room = self._k.attend_workspace(B, T, H, K, D, row_format, dtype)
             if room:

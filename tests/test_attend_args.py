@@ -123,3 +123,13 @@ def test_the_scale_has_no_default():
     assert not co._k.calls
     attend(co, scale=192 ** -0.5)
     assert co._k.calls[-1][0][28] == 192 ** -0.5
+
+
+def test_a_workspace_is_contiguous_bytes():
+    co, room = coordinator(), torch.zeros((64, 2), dtype=torch.uint8)
+    with pytest.raises(ValueError, match="workspace must be contiguous"):
+        attend(co, workspace=room[:, 0])  # what lies between its bytes is not its own
+    assert not co._k.calls
+    for ws in (room, torch.zeros(32, dtype=torch.float32)):
+        attend(co, workspace=ws)
+        assert co._k.calls[-1][0][19:21] == (ws.data_ptr(), 128)
