@@ -272,7 +272,9 @@ class XdsOffloadCoordinator:
         dev = self.top_k_device_slots.device
         if workspace is not None and not workspace.is_contiguous():
             raise ValueError("attend: workspace must be contiguous")
-        for x in (q, slots, draft_rows, tree, out, lse, workspace):
+        if not self._req_pool_indices.is_contiguous():
+            raise ValueError("attend: set_batch()'s req_pool_indices must be contiguous")
+        for x in (q, slots, draft_rows, tree, out, lse, workspace, self._req_pool_indices):
             if x is not None and x.device != dev:
                 raise ValueError("attend: every tensor must be on {}".format(dev))
         err_word = _word_address(err_word, dev)

@@ -133,3 +133,19 @@ def test_a_workspace_is_contiguous_bytes():
     for ws in (room, torch.zeros(32, dtype=torch.float32)):
         attend(co, workspace=ws)
         assert co._k.calls[-1][0][19:21] == (ws.data_ptr(), 128)
+
+
+def test_pool_indices_with_gaps_are_refused():
+    co = coordinator()
+    co._req_pool_indices = torch.arange(2 * REQS)[::2]
+    with pytest.raises(ValueError, match="req_pool_indices must be contiguous"):
+        attend(co)
+    assert not co._k.calls
+
+
+def test_pool_indices_elsewhere_are_refused():
+    co = coordinator()
+    co._req_pool_indices = torch.zeros(REQS, dtype=torch.int64, device="meta")
+    with pytest.raises(ValueError, match="every tensor must be on"):
+        attend(co)
+    assert not co._k.calls
