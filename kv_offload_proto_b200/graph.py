@@ -5,8 +5,8 @@ layers' kernels.
 The captured calls publish no status words (there is no host work in a replay to zero them);
 completion is the stream's. Device-side errCodes (a row past its segment, a null segment, a
 cooperative copy that stopped waiting) go to one device error word shared by the captured
-calls (KvopsRowOpts.err_word): `error()` reads it after a replay and `clear_error()` resets it. Everything a captured call reads is fixed at capture time: the
-coordinator's batch tensors (`set_batch`), its state tensors and `self.topk` — so a decode loop
+calls (KvopsRowOpts.err_word): `error()` reads it after a replay and `clear_error()` resets it. Everything a captured
+call reads is fixed at capture time: the coordinator's batch tensors (`set_batch`), its state tensors and `self.topk` — so a decode loop
 copies each step's top-K indices into `self.topk` (and refreshes the batch tensors in place)
 before `replay()`. The reference has no counterpart (its driver issues the calls one by one,
 xds/xds_decode.py:225-233).
@@ -24,11 +24,13 @@ class StepGraph:
     topk: optional int32 tensor [layers, max_num_reqs, top_k] to read; allocated if None.
     after_layer: optional callable(layer) whose CUDA work is captured right after that layer's
     call, e.g. a reduction of the layer's outputs (coord.is_miss, coord.top_k_device_slots),
-    which the next layer overwrites.
+    which the next layer overwrites, or `coord.attend`.
+    err: optional int32 tensor of one element to use as the error word, for after_layer's calls to share (attend's
+    err_word; without it their codes go to the coordinator's word, `coord.attend_error()`). It is zeroed.
     """
 
     def __init__(self, pool, coord, hot: Sequence, layers: Optional[int] = None, *, path: str = "auto",
-                 block_dim: int = 1, hot_req_stride_rows: int = 0, topk=None, after_layer=None):
+                 block_dim: int = 1, hot_req_stride_rows: int = 0, topk=None, after_layer=None, err=None):
         import torch
         if coord._req_pool_indices is None:
             raise RuntimeError("StepGraph: call coord.set_batch() before capturing")
@@ -38,12 +40,17 @@ class StepGraph:
         if topk.dtype != torch.int32 or tuple(topk.shape) != (self.layers, coord.max_num_reqs, coord.top_k):
             raise ValueError("StepGraph: topk must be int32 [layers, max_num_reqs, top_k]")
         self.topk = topk
+        if err is None:
+            err = torch.zeros(1, dtype=torch.int32, device=coord.device)
+        elif err.dtype != torch.int32 or err.numel() != 1 or err.device != topk.device:
+            raise ValueError("StepGraph: err must be an int32 tensor of one element on the coordinator's device")
+        err.zero_()
+        self.err = err
         k = pool._k
         # The first call of a shape sets up device scratch and kernel limits; do that now,
         # outside the capture.
         k.step_prepare(coord.top_k, coord.device_buffer_size, coord.padded_buffer_size, coord.visited_stride_b,
                        coord.max_num_reqs)
-        self.err = torch.zeros(1, dtype=torch.int32, device=coord.device)
         self.graph = torch.cuda.CUDAGraph()
         self.stream = torch.cuda.Stream(device=coord.device)
         with torch.cuda.graph(self.graph, stream=self.stream):

@@ -81,3 +81,29 @@ def test_a_step_in_one_call_is_the_two_calls():
         assert int(one.co.miss_count()) > 0
     one.pool.destroy()
     two.pool.destroy()
+
+
+@pytest.mark.parametrize("room", [0, 2])
+def test_a_captured_attention_reports_to_its_step(room):
+    """The step's error word is the attention's too: generated tokens without a place among the hot rows are in error()."""
+    s = Step("raw")
+    s.co.set_batch(torch.arange(R, device="cuda"), torch.full((R,), CTX + 2, dtype=torch.int32, device="cuda"))
+    stride = s.co.padded_buffer_size + room
+    hot = torch.zeros((R * stride, 576), dtype=torch.float16, device="cuda")
+    q = torch.randn((R, 8, 576), device="cuda").half()
+    word = torch.full((1,), 7, dtype=torch.int32, device="cuda")
+    graph = StepGraph(s.pool, s.co, [hot], hot_req_stride_rows=stride, err=word,
+                      after_layer=lambda layer: s.co.attend(q, hot, hot_req_stride_rows=stride, scale=0.1, err_word=word))
+    s.topk[:, -2:] = torch.tensor([CTX, CTX + 1], device="cuda")
+    graph.topk[0].copy_(s.topk)
+    assert graph.error() == 0
+    for _ in range(2):
+        graph.replay()
+        assert graph.error() == (0 if room else 0x104)
+    graph.clear_error()
+    assert word.item() == 0 and s.co.attend_error() == 0
+    for bad in (torch.zeros(1, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="err must be"):
+            StepGraph(s.pool, s.co, [hot], hot_req_stride_rows=stride, err=bad)
+    del graph
+    s.pool.destroy()
