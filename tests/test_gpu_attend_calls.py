@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+import quant_model
 from gpu_util import kv
 from kv_offload_proto_b200.offload import XdsOffloadCoordinator
 from test_gpu_attend import Case
@@ -183,3 +184,41 @@ def test_probabilities_of_a_list_of_two_to_the_sixteen():
     out, _ = c.call(scale=1.0)
     t = (K - 1) * math.exp(-20.25) / (1 + (K - 1) * math.exp(-20.25))
     assert (out.double() - t).abs().max() <= 2.0 ** -13 + 2.0 ** -10 * t
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("fmt", ["raw", "e4m3"])
+@pytest.mark.parametrize("H, K", [(4, 70), (40, 3000)])  # a whole list, and one that is cut and joined
+@pytest.mark.parametrize("dim", [3, 540])  # of a row's value, and of its rotary part, which only the score has
+def test_a_listed_hot_row_that_is_not_finite(dim, H, K, fmt, bad):
+    """It is NaN where the formula is (a score of NaN or +inf, or an infinite value times 0), and nowhere else."""
+    c = Case(47, B=2, H=H, K=K, rows=200, fmt=fmt, dtype="bf16")
+    c.slots[0, 1] = 17
+    row = 17 + int(c.idx[0]) * 200
+    c.read[row, dim] = bad
+    if fmt == "raw":
+        c.hot = c.read
+    else:
+        stored = quant_model.encode(c.read.cpu(), fmt, 512)
+        c.hot, c.read = torch.from_numpy(stored).cuda(), quant_model.decode(stored, fmt, "bf16", 512).cuda()
+    out, lse = c.call()
+    for r in range(2):
+        k = c.keys(r, 0)
+        s = c.q[r, 0].double() @ k.T * c.scale
+        want, log = (torch.softmax(s, 1) @ k[:, :512]).isnan(), torch.logsumexp(s, 1)
+        assert torch.equal(out[r, 0].isnan(), want)
+        assert torch.equal(lse[r, 0].isnan(), log.isnan() | (log == math.inf))
+        assert want.any() == (r == 0)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("H, K", [(4, 70), (40, 3000)])
+def test_a_query_that_is_not_finite_harms_no_other(H, K, bad):
+    c = Case(48, B=2, H=H, K=K, rows=200)
+    want = c.call()
+    c.q[1, 0, 2, 7] = bad
+    out, lse = c.call()
+    hit = torch.zeros_like(lse, dtype=torch.bool)
+    hit[1, 0, 2] = True
+    assert out[hit].isnan().all() and lse[hit].isnan().all()
+    assert torch.equal(out[~hit], want[0][~hit]) and torch.equal(lse[~hit], want[1][~hit])
