@@ -26,11 +26,12 @@
 // and the 64 rotary dimensions (8 KB). The groups go through a ring of places that the second product
 // frees one by one, so rows travel while earlier ones are still in use.
 //
-// Measured, 2048 keys a request: 64 requests x 128 heads, fp16 rows, 68 us (2.5 TB/s, 540 TFLOP/s; 3300 cycles
-// a tile, of which the operands take 2500, and 20 of 148 SMs have no list); four tokens each 254 us (575
-// TFLOP/s); 64 requests x 16 heads 34 us (4.9 TB/s), with 8-bit rows 45 us: converting codes is the load
-// warps' longest part (1450 of 3700 cycles a tile); one request x 128 heads 14 us, chains of loads
-// (the count, the slots, the rows), two products, the outputs and the joining.
+// Measured, 2048 keys a request (here and below without the call from Python: a captured graph of 20 launches):
+// 64 requests x 128 heads, fp16 rows, 65 us (2.6 TB/s, 563 TFLOP/s; 3300 cycles a tile, of which the operands take
+// 2500, and 20 of 148 SMs have no list); four tokens each 253 us (577 TFLOP/s); 64 requests x 16 heads
+// 37 us (154 MB, 4.2 TB/s), with 8-bit rows 45 us: a load warp has one place for codes, so the next tile's are
+// fetched behind the conversion of this one's only, 1450 of 3700 cycles a tile; one request x 128 heads
+// 13 us, chains of loads (the count, the slots, the rows), two products, the outputs and the joining.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stddef.h>
@@ -810,7 +811,12 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
                 }
                 return excess;
             };
-            const auto write = [&]() {  // the probabilities, to where the second product reads them
+            // The probabilities, to where the second product reads them: rounded to the rows' type, since the
+            // matrix unit takes both its operands in one type, and the rows in 32 bits would take twice the
+            // shared memory that bounds the products. The sums stay fp32, as lse is. (Errors against 64 bits:
+            // fp16 2.4e-4 to 2.6e-4 where probabilities in fp32 leave 2.1e-4, the output's own rounding; bf16
+            // 1.9e-3 to 2.1e-3 and 1.7e-3.)
+            const auto write = [&]() {
                 const uint32_t to = smem + Layout<NQ, kStored>::rope + (done & 1) * kChunkBytes + key * 128 + pair * 2;
 #pragma unroll
                 for (int b = 0; b < kBlocks; ++b) {
@@ -971,8 +977,8 @@ __device__ __forceinline__ void softmax_warps(const KvopsAttend &a, const Plan &
 // The roles' code is long and each warp goes through its own once a tile, which is slow where it does not stay in
 // the instruction caches: unrolled, the products' 36 + 16 instructions with their descriptors and the
 // conversion of a row's 128 codes had warps waiting for instructions more than a quarter of the time
-// (64 requests x 128 heads 80 us, now 72; x 16 heads 42, 37; 8-bit rows 58, 48). So these are loops of short
-// bodies, and the waits' slow halves are a function.
+// (then, 64 requests x 128 heads took 80 us unrolled and 72 in loops; x 16 heads 42 and 37; 8-bit rows 58 and 48).
+// So these are loops of short bodies, and the waits' slow halves are a function.
 template <typename T, typename Code, bool kStored, int NQ>
 __global__ void __launch_bounds__(kThreads, 1)
     attend_kernel(const KvopsAttend a, const Plan plan)
@@ -1193,8 +1199,8 @@ int sm_count()
 // Queries per tile. A pair costs about the same for any number up to 64 (the rows' way into shared
 // memory), so a tile takes as many as there are, unless there is little to do: then smaller tiles, whose
 // queries and outputs are fewer, are sooner done, up to four pairs an SM. Queries a tile, in us, for 128
-// heads x 2048 keys: one request 16: 14.1, 32: 18.4, 64: 19.5; four requests 23.3, 21.0, 24.2; one request's four
-// tokens 24.9, 23.2, 28.5.
+// heads x 2048 keys: one request 16: 13.2, 32: 17.5, 64: 18.6; two requests 16.3, 16.7, 24.1; four requests 22.5, 20.1,
+// 23.3; one request's four tokens 24.1, 22.2, 27.6; eight requests 30.5, 28.0, 28.0.
 uint32_t queries_per_tile(const KvopsAttend &a, uint32_t lists, int sms)
 {
     const uint32_t rows = a.heads * (lists > 1 ? 1 : a.tokens);
@@ -1218,10 +1224,11 @@ Plan make_plan(const KvopsAttend &a, uint32_t lists, uint32_t nq, int sms)
     // Whole units need no joining, equal runs of pairs leave no SM idle. In tiles' times: a unit costs its
     // tiles and about two more for its queries and outputs, a cut unit these for each part; the joining
     // costs six; and runs that cut a list's query tiles in different places read its rows at different
-    // times, which costs an eighth. Whole units against runs, in us: 64 requests x 128 heads x 2048 8-bit keys 89,
-    // 97; 100 requests x 128 heads x 1024 keys 73, 76; 130 requests x 16 heads 55, 61; 7 x 3 lists x 24
-    // heads x 333 keys 14.8, 15.9; but 40 requests x 128 heads 67, 57; 80 requests 129, 98; 100 requests x
-    // 16 heads 54, 47; 64 requests x 16 heads 80, 45.
+    // times, which costs an eighth. Whole units against runs, in us: 64 requests x 128 heads x 2048 keys 65, 79
+    // (8-bit 90, 97); 100 requests x 128 heads x 1024 keys 72, 75; 130 requests x 16 heads 57, 64 (8-bit 84,
+    // 84); but 40 requests x 128 heads 66, 56; 80 requests 130, 97; 100 requests x 16 heads 54, 51 (8-bit 84,
+    // 65); 64 requests x 16 heads 52, 37 (8-bit 83, 45). For few short lists the joining is counted too dear:
+    // 7 x 3 lists x 24 heads x 333 keys take whole units here, 13.6, where runs take 12.4 (8-bit 20.0, 14.5).
     const uint64_t whole = (units + sms - 1) / sms;
     const uint64_t run = (pairs + sms - 1) / sms;
     p.run_at_most = static_cast<uint32_t>(run);

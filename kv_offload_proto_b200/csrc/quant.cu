@@ -10,7 +10,7 @@
 // No two warps wait for each other. 8192 rows of 61 layers, 903 MB: 188 us, 4.8 TB/s. The instructions
 // were 63% of the issue slots with an address for each group; hence four groups to an address.
 // Reading, a CTA takes a tile, as rows.cu does, since few positions may be misses, and 16 codes (32
-// bytes) a thread at a time. 262,144 of 524,288 positions, 479 MB: 123 to 135 us, 3.9 TB/s; copying as many rows
+// bytes) a thread at a time. 262,144 of 524,288 positions, 479 MB: 132 us, 3.6 TB/s (123 to 135 by the GPU); copying as many rows
 // of these sizes from and to random places, without any rule or arithmetic, takes 98 us. (A warp a tile:
 // 136 us; the next tile's positions loaded ahead: 136 us; the memory is the limit, not the waits.)
 #include <stdint.h>
@@ -286,7 +286,7 @@ Shape shape_of(uint64_t positions, int sm_count, bool write)
         while (s.tile > 1 && positions <= ctas * kWarps * (s.tile / 2)) s.tile /= 2;
     } else {
         // One for every thread, since few may be misses; fewer where that leaves CTAs without any (131,072
-        // positions, a fifth of them misses: 18 us, with 64 positions a tile 25).
+        // positions, a fifth of them misses: 19 us, with 64 positions a tile 25).
         s.tile = kThreads;
         while (s.tile > 16 && positions <= ctas * (s.tile / 2)) s.tile /= 2;
     }
