@@ -10,9 +10,9 @@
 // No two warps wait for each other. 8192 rows of 61 layers, 903 MB: 188 us, 4.8 TB/s. The instructions
 // were 63% of the issue slots with an address for each group; hence four groups to an address.
 // Reading, a CTA takes a tile, as rows.cu does, since few positions may be misses, and 16 codes (32
-// bytes) a thread at a time. 262,144 of 524,288 positions, 479 MB: 132 us, 3.6 TB/s (123 to 135 by the GPU); copying as many rows
-// of these sizes from and to random places, without any rule or arithmetic, takes 98 us. (A warp a tile:
-// 136 us; the next tile's positions loaded ahead: 136 us; the memory is the limit, not the waits.)
+// bytes) a thread at a time. 262,144 of 524,288 positions, 479 MB: 132 us, 3.6 TB/s (123 to 135 on different
+// GPUs); copying as many rows of these sizes from and to random places, without any rule or arithmetic, takes
+// 98 us. Neither a warp a tile (136 us) nor the next tile's positions loaded ahead (136 us) came nearer to it.
 #include <stdint.h>
 
 #include "kvops_internal.cuh"
