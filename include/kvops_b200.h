@@ -346,7 +346,8 @@ int kvops_sieve_import_quant(uint64_t topk_indices, uint64_t req_pool_indices, u
  * step; tree 0 (no words) stands for a chain, token t seeing drafted rows 0..t.
  * Scores, sums and outputs are accumulated in fp32; the probabilities are rounded to the rows'
  * type for the second product, as its matrix unit takes them, and out is rounded to it once. In fp16 the
- * smallest probabilities are lost there: over all keys 2^-13 of the largest value at the most. */
+ * smallest probabilities are lost there: over all keys 2^-13 of the largest value at the most (bf16: those
+ * below 2^-121). */
 typedef struct KvopsAttend {
     uint64_t q;                    /* [max_num_reqs, tokens, heads, 576], 16-bit, 16-byte aligned rows */
     uint64_t q_stride_req, q_stride_token, q_stride_head; /* in values, multiples of 8 */

@@ -73,7 +73,7 @@ constexpr uint32_t kAhead = 4;  // tiles whose rows are known at a time
 // references; where that can be more, the lift is 14, which leaves 2^-15 for 2^24 keys. (It costs less the longer
 // a part is: in us with 4 and 14, 64 requests x 128 heads, 32 tiles a part, 65 and 94; 8 requests x 16 heads x 2^17 keys,
 // 111 tiles, 197 and 203; 148 requests x 16 heads x 2^17, 2048 tiles, 2906 and 2913.)
-// bf16 has no such limit.
+// bf16 has the range of fp32: what is lost is below 2^-121 of the largest.
 constexpr float kMost = 15.f;
 constexpr float kLiftFp16 = 4.f, kLiftFp16Long = 14.f, kLiftBf16 = -5.f;
 constexpr uint32_t kLongPart = 1u << 16;
